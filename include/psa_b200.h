@@ -424,6 +424,60 @@ int psa_fwd_images_scatter(const void* q, const void* kimg, const void* vimg, co
                            int64_t seq_k, int head_dim, int block_m, int block_n, int tile_n, int mask_width, float sm_scale,
                            int compat_quirk, int dtype, int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * The answering side of the vision-language call site: what a decoder needs around the causal attention of the prompt.  The
+ * reference hands single tokens back to the model's own attention (qwen2.5-vl-example/src/attention/qwen2vl_attention.py), so
+ * these have no counterpart there.  Row strides are in elements; channels are neighbours; every pointer is 16-byte aligned.
+ * `status` is the int32 word described above: PSA_ERR_ARG is written into it where a page number, slot, length or count found
+ * on the device is out of range (the access is skipped) or a request could not be given pages. */
+
+/* Rotary positions with several axes.  n operands (1 or 2: queries, keys) src[i] -> dst[i], [batch][heads[i]][seq][head_dim]
+ * with strides {batch, head, token} each (multiples of 16 bytes).  Channel pair p - (p, p + head_dim/2) if half, else (2p, 2p + 1) - of
+ * token (b, t) is turned by positions[axis_of_pair[p]][b][t] * turns[p] / 2^64 whole turns, modulo 2^64 (inverse: back, which is
+ * the gradient).  positions: int32 or int64 (position_bits), strides {axis, batch, token}.  turns, axis_of_pair: HOST arrays of
+ * head_dim/2 entries.  head_dim: a multiple of 16 up to 256. */
+int psa_rotate_axes(const void* const* src, const int64_t* src_strides, void* const* dst, const int64_t* dst_strides,
+                    const int32_t* heads, int n, const void* positions, int position_bits, const int64_t* position_strides,
+                    const uint64_t* turns, const uint8_t* axis_of_pair, int axes, int64_t batch, int64_t seq, int head_dim,
+                    int half, int inverse, int dtype, void* stream);
+
+/* Room for counts[b] (0..tokens) more tokens of every request: table [requests][width] (pages of each, in order), lengths, the
+ * pool of free page numbers and how many of them are free (free_in[0], taken from the top) -> the same after the call, and
+ * slots [requests][tokens] = page * page_size + place of each new token, -1 behind the last one.  Requests that need pages are served in
+ * order while the running total of all needs fits the pool; one that is not served, would outgrow its row or has a count or
+ * length out of range is given nothing.  Outputs may be the inputs' own memory.  page_size: a multiple of 16. */
+size_t psa_plan_pages_scratch_bytes(int64_t requests);
+int psa_plan_pages(const int32_t* table, const int32_t* lengths, const int32_t* counts, const int32_t* pool, const int32_t* free_in,
+                   int32_t* table_out, int32_t* lengths_out, int32_t* free_out, int32_t* slots, void* scratch,
+                   size_t scratch_bytes, int64_t requests, int64_t width, int64_t pool_size, int page_size, int64_t tokens,
+                   int32_t* status, void* stream);
+/* The pages of the requests with which[b] != 0 go back on top of the pool, in an order that undoes psa_plan_pages; their lengths
+ * become 0. */
+int psa_release_pages(const int32_t* table, int32_t* lengths, const uint8_t* which, int32_t* pool, int32_t* free_count,
+                      int64_t requests, int64_t width, int64_t pool_size, int page_size, int32_t* status, void* stream);
+
+/* A cache of keys and values held in 4 bits: data [pages][kv_heads][page_size/16][psa_kv4_slice_bytes], f16/bf16, head_dim 64/128,
+ * groups of 32, 64 or 128 channels with a step and a lowest value of the type each (16 * (head_dim + 8 * head_dim / group) bytes
+ * for 16 tokens of a head; 0 = unsupported sizes).  psa_kv4_append quantises rows k, v [batch][kv_heads][tokens][head_dim]
+ * (strides {batch, head, token} of k, then of v) into the slots [batch][tokens] (-1: the row is skipped; a slot named twice holds
+ * bytes of either row).  psa_kv4_read gives the values that slots hold, zeros for -1. */
+size_t psa_kv4_slice_bytes(int head_dim, int group);
+int psa_kv4_append(void* data, const void* k, const void* v, const int64_t* strides, const int32_t* slots, int64_t pages,
+                   int kv_heads, int page_size, int64_t batch, int64_t tokens, int head_dim, int group, int dtype,
+                   int32_t* status, void* stream);
+int psa_kv4_read(const void* data, void* k, void* v, const int64_t* strides, const int32_t* slots, int64_t pages, int kv_heads,
+                 int page_size, int64_t batch, int64_t tokens, int head_dim, int group, int dtype, int32_t* status, void* stream);
+
+/* Attention of the last counts[b] (null: tokens) tokens of every request over that cache: q, out [batch][heads][tokens][head_dim],
+ * query i of request b stands at lengths[b] - counts[b] + i and sees the keys up to its own place; query head h reads key head
+ * h / (heads / kv_heads).  Rows without a key, and rows from counts[b] on, give 0 (lse -inf).  lse: optional
+ * [batch][heads][tokens], natural logarithm.  table [batch][width].  scratch needs no initialising. */
+size_t psa_kv4_attention_scratch_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim);
+int psa_kv4_attention(const void* q, const int64_t* q_strides, const void* data, const int32_t* table, const int32_t* lengths,
+                      const int32_t* counts, void* out, const int64_t* out_strides, float* lse, void* scratch,
+                      size_t scratch_bytes, int64_t pages, int page_size, int64_t width, int64_t batch, int64_t tokens, int heads,
+                      int kv_heads, int head_dim, int group, float sm_scale, int dtype, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

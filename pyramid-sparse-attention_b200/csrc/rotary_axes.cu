@@ -1,0 +1,144 @@
+// Rotary positions with several axes (text, or time / height / width of a video's tokens), applied to queries and keys in one
+// launch; the backward pass is the same kernel with the angles negated.
+//
+// Channel pair i of token (b, t) is turned by the angle pos[axis(i)][b][t] * freq(i).  The angle is kept in turns as a 64-bit
+// fraction: turns(i) = freq(i) / 2 pi * 2^64 comes from the host, the product with the position is taken modulo 2^64 - whole turns
+// drop out of an integer product by themselves - and its upper half, as a signed number of 2^-32 turns, goes through sincospif.
+// The error is |pos| * 2^-65 turns plus the rounding of that number to 24 bits (2^-25 half turns), at any position a model reaches;
+// pos * freq in 32 bits is off by 2^-25 * pos radians (0.004 at position 131072).
+#include "psa_common.cuh"
+
+namespace psa {
+namespace {
+
+constexpr int kMaxPairs = 128, kMaxAxes = 8;
+
+struct RotaryArgs {
+  const void* src[2];
+  void* dst[2];
+  int64_t src_stride[2][3], dst_stride[2][3];   // batch, head, token; in elements
+  int heads[2];
+  const void* pos;
+  int64_t pos_stride[3];                        // axis, batch, token; in elements
+  int64_t batch, seq;
+  uint64_t turns[kMaxPairs];
+  uint8_t axis[kMaxPairs];
+  int pos64, inverse;
+};
+
+union Word {
+  uint4 u;
+  float f[4];
+  __half h[8];
+  __nv_bfloat16 b[8];
+};
+template <typename T> __device__ __forceinline__ T* word_of(Word& w);
+template <> __device__ __forceinline__ float* word_of<float>(Word& w) { return w.f; }
+template <> __device__ __forceinline__ __half* word_of<__half>(Word& w) { return w.h; }
+template <> __device__ __forceinline__ __nv_bfloat16* word_of<__nv_bfloat16>(Word& w) { return w.b; }
+
+// A thread owns V pairs of one token - two 16-byte words of a row - computes their sines and cosines once and walks the heads
+// with them.  HALF: pair i is channels (i, i + D/2); otherwise neighbours (2i, 2i + 1).
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant__ RotaryArgs a, int head_dim, int parts) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int chunks = head_dim / 2 / V;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int chunk = (int)(i % chunks);
+  const int64_t token = i / chunks;
+  if (token >= a.batch * a.seq) return;
+  const int64_t b = token / a.seq, t = token - b * a.seq;
+  float cs[V], sn[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int pair = chunk * V + j;
+    const int64_t at = a.axis[pair] * a.pos_stride[0] + b * a.pos_stride[1] + t * a.pos_stride[2];
+    const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : static_cast<const int32_t*>(a.pos)[at];
+    const int32_t turn = (int32_t)(((uint64_t)p * a.turns[pair]) >> 32);
+    sincospif((float)turn * 4.656612873077393e-10f, &sn[j], &cs[j]);   // 2^-31 half turns
+    if (a.inverse) sn[j] = -sn[j];
+  }
+  const int first = HALF ? chunk * V : chunk * 2 * V, second = HALF ? first + head_dim / 2 : first + V;
+  const int heads = a.heads[0] + a.heads[1];
+  for (int h = blockIdx.y; h < heads; h += parts) {
+    const int z = h >= a.heads[0], hh = z ? h - a.heads[0] : h;
+    const T* src = static_cast<const T*>(a.src[z]) + b * a.src_stride[z][0] + hh * a.src_stride[z][1] + t * a.src_stride[z][2];
+    T* dst = static_cast<T*>(a.dst[z]) + b * a.dst_stride[z][0] + hh * a.dst_stride[z][1] + t * a.dst_stride[z][2];
+    Word w0, w1;
+    w0.u = *reinterpret_cast<const uint4*>(src + first);
+    w1.u = *reinterpret_cast<const uint4*>(src + second);
+    T *e0 = word_of<T>(w0), *e1 = word_of<T>(w1);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      T& r0 = HALF ? e0[j] : (j < V / 2 ? e0[2 * j] : e1[2 * j - V]);
+      T& r1 = HALF ? e1[j] : (j < V / 2 ? e0[2 * j + 1] : e1[2 * j + 1 - V]);
+      const float x0 = Elem<T>::to_f(r0), x1 = Elem<T>::to_f(r1);
+      r0 = Elem<T>::from_f(x0 * cs[j] - x1 * sn[j]);
+      r1 = Elem<T>::from_f(x1 * cs[j] + x0 * sn[j]);
+    }
+    *reinterpret_cast<uint4*>(dst + first) = w0.u;
+    *reinterpret_cast<uint4*>(dst + second) = w1.u;
+  }
+}
+
+template <typename T>
+int launch(const RotaryArgs& a, int head_dim, int half, cudaStream_t st) {
+  const int64_t threads = a.batch * a.seq * (head_dim / 2 / (16 / (int)sizeof(T)));
+  const int64_t blocks = cdiv64(threads, 128);
+  PSA_REQUIRE(blocks < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_rotate_axes: too many tokens");
+  const int heads = a.heads[0] + a.heads[1];
+  int parts = 1;   // few tokens: the heads are shared out over blocks
+  while (parts < heads && blocks * parts < 148 * 8) parts *= 2;
+  if (parts > heads) parts = heads;
+  const dim3 grid((unsigned)blocks, (unsigned)parts);
+  if (half) rotary_axes_kernel<T, true><<<grid, 128, 0, st>>>(a, head_dim, parts);
+  else rotary_axes_kernel<T, false><<<grid, 128, 0, st>>>(a, head_dim, parts);
+  PSA_CHECK_LAUNCH("psa_rotate_axes");
+  return PSA_OK;
+}
+
+}  // namespace
+}  // namespace psa
+
+extern "C" int psa_rotate_axes(const void* const* src, const int64_t* src_strides, void* const* dst, const int64_t* dst_strides,
+                               const int32_t* heads, int n, const void* positions, int position_bits, const int64_t* position_strides,
+                               const uint64_t* turns, const uint8_t* axis_of_pair, int axes, int64_t batch, int64_t seq, int head_dim,
+                               int half, int inverse, int dtype, void* stream) {
+  using namespace psa;
+  PSA_REQUIRE(src && src_strides && dst && dst_strides && heads && positions && position_strides && turns && axis_of_pair, PSA_ERR_ARG,
+              "psa_rotate_axes: null pointer");
+  PSA_REQUIRE(n == 1 || n == 2, PSA_ERR_ARG, "psa_rotate_axes: 1 or 2 operands");
+  PSA_REQUIRE(head_dim >= 16 && head_dim <= 2 * kMaxPairs && head_dim % 16 == 0, PSA_ERR_ARG,
+              "psa_rotate_axes: head_dim=%d (a multiple of 16 up to %d)", head_dim, 2 * kMaxPairs);
+  PSA_REQUIRE(axes >= 1 && axes <= kMaxAxes, PSA_ERR_ARG, "psa_rotate_axes: %d axes (1 to %d)", axes, kMaxAxes);
+  PSA_REQUIRE(position_bits == 32 || position_bits == 64, PSA_ERR_ARG, "psa_rotate_axes: positions of %d bits (32 or 64)", position_bits);
+  PSA_REQUIRE(batch > 0 && seq > 0 && batch < ((int64_t)1 << 31) && seq < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_rotate_axes: bad shape");
+  const int elem = dtype == PSA_F32 ? 4 : 2;
+  RotaryArgs a = {};
+  for (int i = 0; i < n; ++i) {
+    PSA_REQUIRE(src[i] && dst[i] && src[i] != dst[i] && heads[i] > 0, PSA_ERR_ARG, "psa_rotate_axes: operand %d", i);
+    PSA_REQUIRE((((uintptr_t)src[i] | (uintptr_t)dst[i]) & 15) == 0, PSA_ERR_ARG, "psa_rotate_axes: operand %d is not 16-byte aligned", i);
+    for (int d = 0; d < 3; ++d) {
+      PSA_REQUIRE(src_strides[3 * i + d] * elem % 16 == 0 && dst_strides[3 * i + d] * elem % 16 == 0, PSA_ERR_ARG,
+                  "psa_rotate_axes: strides of operand %d must be multiples of 16 bytes", i);
+      a.src_stride[i][d] = src_strides[3 * i + d];
+      a.dst_stride[i][d] = dst_strides[3 * i + d];
+    }
+    a.src[i] = src[i];
+    a.dst[i] = dst[i];
+    a.heads[i] = heads[i];
+  }
+  for (int i = 0; i < head_dim / 2; ++i) {
+    PSA_REQUIRE(axis_of_pair[i] < axes, PSA_ERR_ARG, "psa_rotate_axes: pair %d is of axis %d of %d", i, axis_of_pair[i], axes);
+    a.turns[i] = turns[i];
+    a.axis[i] = axis_of_pair[i];
+  }
+  a.pos = positions;
+  for (int d = 0; d < 3; ++d) a.pos_stride[d] = position_strides[d];
+  a.batch = batch;
+  a.seq = seq;
+  a.pos64 = position_bits == 64;
+  a.inverse = inverse != 0;
+  PSA_DISPATCH_DTYPE(dtype, T, return launch<T>(a, head_dim, half, (cudaStream_t)stream));
+  return PSA_OK;
+}

@@ -86,6 +86,15 @@ SIGNATURES = {
     "psa_legacy_bwd_tc": (_i, [_p] * 17 + [_i64, _i64, _i, _i, _f, _i, _i, _p]),
     "psa_legacy_bwd_scratch_bytes": (_sz, [_i64, _i64, _i]),
     "psa_legacy_bwd_tcgen05": (_i, [_p] * 11 + [_sz, _i64, _i64, _i, _i, _f, _i, _i, _p, _p]),
+    "psa_rotate_axes": (_i, [_p] * 5 + [_i, _p, _i, _p, _p, _p, _i, _i64, _i64, _i, _i, _i, _i, _p]),
+    "psa_plan_pages_scratch_bytes": (_sz, [_i64]),
+    "psa_plan_pages": (_i, [_p] * 10 + [_sz, _i64, _i64, _i64, _i, _i64, _p, _p]),
+    "psa_release_pages": (_i, [_p] * 5 + [_i64, _i64, _i64, _i, _p, _p]),
+    "psa_kv4_slice_bytes": (_sz, [_i, _i]),
+    "psa_kv4_append": (_i, [_p] * 5 + [_i64, _i, _i, _i64, _i64, _i, _i, _i, _p, _p]),
+    "psa_kv4_read": (_i, [_p] * 5 + [_i64, _i, _i, _i64, _i64, _i, _i, _i, _p, _p]),
+    "psa_kv4_attention_scratch_bytes": (_sz, [_i64, _i64, _i, _i, _i]),
+    "psa_kv4_attention": (_i, [_p] * 10 + [_sz, _i64, _i, _i64, _i64, _i64, _i, _i, _i, _i, _f, _i, _p, _p]),
 }
 for _name, (_res, _args) in SIGNATURES.items():
     _fn = getattr(lib, _name)          # AttributeError here = the library does not export a declared symbol

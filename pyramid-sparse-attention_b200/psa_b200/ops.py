@@ -5,6 +5,7 @@ import contextlib
 import ctypes as C
 import functools
 import math
+from fractions import Fraction
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -56,7 +57,8 @@ def _mask32(mask: torch.Tensor) -> torch.Tensor:
 
 
 # One status word per device, shared by every launch of the tensor-core attention kernels: a kernel whose bounded
-# device-side wait expired writes PSA_ERR_TIMEOUT into it and nothing ever clears it except check_status().  Calls stay
+# device-side wait expired writes PSA_ERR_TIMEOUT into it (the kernels of a cache in pages: PSA_ERR_ARG where a number read on
+# the device is out of range) and nothing ever clears it except check_status().  Calls stay
 # free of host synchronisation; a run asks once, at the end (PSAAttention.check_status, close_logger).
 _STATUS: Dict[int, torch.Tensor] = {}
 
@@ -71,14 +73,16 @@ def status_word(device) -> torch.Tensor:
 
 def check_status(device=None, reset: bool = True) -> None:
     """Raise PSAKernelError if any attention kernel launched so far on `device` (default: every device used) gave up
-    on a bounded wait - its output is then incomplete.  Synchronises the device."""
+    on a bounded wait, or met a page, slot or length out of range - its output is then incomplete.  Synchronises the device."""
     words = list(_STATUS.items()) if device is None else [(None, status_word(device))]
     for _, w in words:
         code = int(w.item())
         if code != 0:
             if reset:
                 w.zero_()
-            raise _lib.PSAKernelError(f"a PSA kernel on {w.device} reported status {code} (bounded device-side wait expired); "
+            why = ("a page, slot, length or count was out of range, or the pool of pages was empty" if code == _lib.PSA_ERR_ARG
+                   else "bounded device-side wait expired")
+            raise _lib.PSAKernelError(f"a PSA kernel on {w.device} reported status {code} ({why}); "
                                       "outputs produced since the last check are incomplete")
 
 
@@ -818,3 +822,297 @@ def legacy_backward(q, k, v, mask, o, lse, do, causal: bool, sm_scale: float, py
                 B * H, S, D, mask.shape[-1], float(sm_scale), int(causal), _dt(q), _stream(q))
     check(rc, "psa_legacy_bwd")
     return dq, dk, dv
+
+
+# ------------------------------------------------------------------------------------------------
+# The answering side of the vision-language call site: rotary positions with several axes, a cache in pages that holds keys and
+# values in 4 bits, and the attention of new tokens over it.
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [B, H, S, D] itself if the kernels can read its rows word by word (any batch, head and token strides), else a copy."""
+    fits = x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(n == 1 or s * x.element_size() % 16 == 0
+                                                              for n, s in zip(x.shape[:3], x.stride()[:3]))
+    return x if fits else x.clone(memory_format=torch.contiguous_format)
+
+
+def _row_strides(*xs: torch.Tensor):
+    return (C.c_int64 * (3 * len(xs)))(*[s if n > 1 else 0 for x in xs for n, s in zip(x.shape[:3], x.stride()[:3])])
+
+
+def _empty_rows(x: torch.Tensor) -> torch.Tensor:
+    """Memory for a result of x's shape in x's order of dimensions (a transposed view gives one), rows of whole 16-byte words."""
+    out = torch.empty_like(x)
+    return out if out.stride(3) == 1 and all(n == 1 or s >= x.shape[3] for n, s in zip(x.shape[:3], out.stride()[:3])) \
+        else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+_TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+@functools.lru_cache(maxsize=64)
+def _rotary_plan(head_dim: int, sections: Tuple[int, ...], theta: float, per_axis: bool, inv_freq: Optional[Tuple[float, ...]]):
+    """Turns a position (of 2^64) and axis of every channel pair, as psa_rotate_axes takes them: plain numbers, kept by value."""
+    pairs = head_dim // 2
+    if inv_freq is None:
+        if per_axis:
+            inv_freq = [theta ** -(j / n) for n in sections for j in range(n)]
+        else:
+            inv_freq = [theta ** -(j / pairs) for j in range(pairs)]
+    turns = [round(Fraction(f) * 2 ** 64 / _TWO_PI) % 2 ** 64 for f in inv_freq]
+    axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    return (C.c_uint64 * pairs)(*turns), (C.c_uint8 * pairs)(*axis)
+
+
+def _rotate(xs, positions: torch.Tensor, plan, half: bool, inverse: bool):
+    """xs: 1 or 2 tensors [B, H, S, D], positions [axes, B or 1, S] -> turned copies."""
+    xs = [_aligned_rows(x) for x in xs]
+    B, _, S, D = xs[0].shape
+    with _on(xs[0]):
+        outs = [_empty_rows(x) for x in xs]
+        if B * S > 0:
+            strides = (C.c_int64 * 3)(positions.stride(0), positions.stride(1) if positions.shape[1] > 1 else 0, positions.stride(2))
+            n = len(xs)
+            rc = lib.psa_rotate_axes((C.c_void_p * n)(*[x.data_ptr() for x in xs]), _row_strides(*xs),
+                                     (C.c_void_p * n)(*[o.data_ptr() for o in outs]), _row_strides(*outs),
+                                     (C.c_int32 * n)(*[x.shape[1] for x in xs]), n, _ptr(positions), 8 * positions.element_size(), strides,
+                                     plan[0], plan[1], positions.shape[0], B, S, D, int(half), int(inverse), _dt(xs[0]), _stream(xs[0]))
+            check(rc, "psa_rotate_axes")
+    return outs
+
+
+class _RotateAxes(torch.autograd.Function):
+    """The gradient of a rotation is the rotation back, through the same function: it can be differentiated again."""
+
+    @staticmethod
+    def forward(ctx, positions, plan, half, inverse, *xs):
+        ctx.save_for_backward(positions)
+        ctx.how = plan, half, inverse
+        ctx.set_materialize_grads(False)
+        return tuple(_rotate(xs, positions, plan, half, inverse))
+
+    @staticmethod
+    def backward(ctx, *grads):
+        plan, half, inverse = ctx.how
+        wanted = [g is not None and need for g, need in zip(grads, ctx.needs_input_grad[4:])]
+        if not any(wanted):
+            return (None,) * (4 + len(grads))
+        back = iter(_RotateAxes.apply(ctx.saved_tensors[0], plan, half, not inverse, *[g for g, w in zip(grads, wanted) if w]))
+        return (None,) * 4 + tuple(next(back) if w else None for w in wanted)
+
+
+def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, sections: Sequence[int], theta: float = 10000.0,
+                layout: str = "half", per_axis: bool = False, inv_freq: Optional[Sequence[float]] = None):
+    """Rotary positions with several axes (text; time, height, width of images and video), q and k in one launch.
+
+    q [B, H, S, D], k [B, Hkv, S, D] or None (float32, float16 or bfloat16, any strides; D a multiple of 16 up to 256).
+    positions: int32 or int64, [axes, S] or [axes, B, S].  sections: channel pairs of each axis, in order, D/2 in all.  Pair i turns
+    by positions[axis of i] * frequency of i: theta^(-i / (D/2)), or with per_axis theta^(-j / n) for the j-th of an axis' n pairs;
+    inv_freq: D/2 frequencies instead.  layout: "half" pairs channels (i, i + D/2), "pairs" (2i, 2i + 1).  A position of zero
+    leaves a token as it is.  Angles are exact to 2^-24 turns at any position; values are computed in 32 bits and rounded once.
+    Returns the turned copies (q, or (q, k)), in the order of dimensions of their inputs; differentiable in q and k."""
+    xs = [q] if k is None else [q, k]
+    if any(x.dim() != 4 for x in xs) or any((x.shape[0], *x.shape[2:]) != (q.shape[0], *q.shape[2:]) or x.dtype != q.dtype
+                                            or x.device != q.device for x in xs):
+        raise ValueError("rotate_axes: q [B, H, S, D] and k [B, Hkv, S, D] of one dtype and device")
+    B, _, S, D = q.shape
+    if D % 16 or not 16 <= D <= 256:
+        raise ValueError(f"rotate_axes: head_dim {D} (a multiple of 16 up to 256)")
+    _dt(q)
+    sections = tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 8 or any(n < 0 for n in sections) or sum(sections) != D // 2:
+        raise ValueError(f"rotate_axes: sections {sections} are not {D // 2} channel pairs of 1 to 8 axes")
+    if layout not in ("half", "pairs"):
+        raise ValueError(f"rotate_axes: layout must be 'half' or 'pairs', got {layout!r}")
+    if inv_freq is not None:
+        inv_freq = tuple(float(f) for f in inv_freq)
+        if len(inv_freq) != D // 2 or not all(math.isfinite(f) for f in inv_freq):
+            raise ValueError(f"rotate_axes: inv_freq must be {D // 2} finite numbers")
+    elif not (math.isfinite(theta) and theta > 0):
+        raise ValueError(f"rotate_axes: theta must be positive, got {theta}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"rotate_axes: positions must be int32 or int64, got {positions.dtype}")
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(1)
+    if positions.dim() != 3 or positions.shape[0] != len(sections) or positions.shape[1] not in (1, B) or positions.shape[2] != S:
+        raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{len(sections)}, {B}, {S}]")
+    _need_cuda(*xs, positions)
+    if positions.device != q.device:
+        raise ValueError(f"rotate_axes: positions on {positions.device}, q on {q.device}")
+    plan = _rotary_plan(D, sections, float(theta), bool(per_axis), inv_freq)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        outs = _RotateAxes.apply(positions, plan, layout == "half", False, *xs)
+    else:
+        outs = _rotate(xs, positions, plan, layout == "half", False)
+    return outs[0] if k is None else tuple(outs)
+
+
+def _state32(name: str, t: torch.Tensor, shape, device=None) -> torch.Tensor:
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or (device is not None and t.device != device):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}" + ("" if device is None else f" on {device}"))
+    return t
+
+
+def _ints32(name: str, t: torch.Tensor, shape, device) -> torch.Tensor:
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError(f"{name} must be an int32 or int64 tensor of shape {tuple(shape)} on {device}")
+    return t.to(torch.int32).contiguous()
+
+
+def plan_pages(table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, pool: torch.Tensor, free: torch.Tensor, page_size: int,
+               tokens: int, out=None):
+    """Room for counts[b] (0 .. tokens) more tokens of every request of a cache in pages, without the host knowing any length.
+
+    table int32 [requests, width]: pages of each request, in order; lengths int32 [requests]; pool int32 [n]: free page numbers, of
+    which the first free[0] are there (int32 [1]; taken from the top).  Requests that need pages are served in order while the
+    running total of all needs fits the pool; one that is not served, outgrows its row or has a count out of range gets nothing, and
+    check_status() says so.  Returns (table, lengths, free, slots): the state after it, and int32 [requests, tokens] with the
+    slot (page * page_size + place) of each new token, -1 behind a request's last one.  out: (table, lengths, free) to write
+    into, the inputs themselves for instance; new tensors otherwise."""
+    if table.dim() != 2 or pool.dim() != 1 or min(table.shape) < 1 or pool.numel() < 1:
+        raise ValueError("plan_pages: table [requests, width] and pool [n] must not be empty")
+    if page_size < 16 or page_size % 16 or tokens < 1:
+        raise ValueError(f"plan_pages: page_size {page_size} (a multiple of 16), tokens {tokens} (1 or more)")
+    n, width = table.shape
+    _need_cuda(table, lengths, counts, pool, free)
+    dev = table.device
+    _state32("table", table, (n, width)), _state32("lengths", lengths, (n,), dev)
+    _state32("pool", pool, (pool.numel(),), dev), _state32("free", free, (1,), dev)
+    counts = _ints32("counts", counts, (n,), dev)
+    with _on(table):
+        if out is None:
+            out = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(free)
+        else:
+            for name, t, like in zip(("table", "lengths", "free"), out, (table, lengths, free)):
+                _state32("out " + name, t, like.shape, dev)
+        slots = torch.empty((n, tokens), dtype=torch.int32, device=dev)
+        nbytes = lib.psa_plan_pages_scratch_bytes(n)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = lib.psa_plan_pages(_ptr(table), _ptr(lengths), _ptr(counts), _ptr(pool), _ptr(free), *[t.data_ptr() for t in out], _ptr(slots),
+                                _ptr(scratch), nbytes, n, width, pool.numel(), page_size, tokens, _ptr(status_word(dev)), _stream(table))
+    check(rc, "psa_plan_pages")
+    return (*out, slots)
+
+
+def release_pages(table: torch.Tensor, lengths: torch.Tensor, which: torch.Tensor, pool: torch.Tensor, free: torch.Tensor, page_size: int) -> None:
+    """The pages of the requests marked in which (bool [requests]) go back to the pool and their lengths become 0, in place; an
+    order that undoes plan_pages."""
+    if table.dim() != 2 or pool.dim() != 1 or which.dtype != torch.bool or which.shape != table.shape[:1]:
+        raise ValueError("release_pages: table [requests, width], which bool [requests], pool [n]")
+    if page_size < 16 or page_size % 16:
+        raise ValueError(f"release_pages: page_size {page_size} (a multiple of 16)")
+    _need_cuda(table, lengths, which, pool, free)
+    n, dev = table.shape[0], table.device
+    _state32("table", table, table.shape), _state32("lengths", lengths, (n,), dev)
+    _state32("pool", pool, (pool.numel(),), dev), _state32("free", free, (1,), dev)
+    if which.device != dev:
+        raise ValueError(f"release_pages: which must be on {dev}")
+    which = which.contiguous()
+    with _on(table):
+        rc = lib.psa_release_pages(_ptr(table), _ptr(lengths), _ptr(which), _ptr(pool), _ptr(free), n, table.shape[1], pool.numel(), page_size,
+                                   _ptr(status_word(dev)), _stream(table))
+    check(rc, "psa_release_pages")
+
+
+def kv4_slice_bytes(head_dim: int, group: int) -> int:
+    """Bytes of 16 tokens of one head in a cache held in 4 bits."""
+    nbytes = lib.psa_kv4_slice_bytes(int(head_dim), int(group))
+    if nbytes == 0:
+        raise ValueError(f"a cache in 4 bits has head_dim 64 or 128 and groups of 32, 64 or 128 channels within it (got {head_dim}, {group})")
+    return nbytes
+
+
+def kv4_empty(pages: int, kv_heads: int, page_size: int, head_dim: int, group: int, device) -> torch.Tensor:
+    """Memory for a cache held in 4 bits: uint8 [pages, kv_heads, page_size / 16, slice]."""
+    if pages < 1 or kv_heads < 1 or page_size < 16 or page_size % 16:
+        raise ValueError(f"a cache in 4 bits: {pages} pages of {page_size} tokens (a multiple of 16), {kv_heads} heads")
+    return torch.empty((pages, kv_heads, page_size // 16, kv4_slice_bytes(head_dim, group)), dtype=torch.uint8, device=device)
+
+
+def _kv4_data(data: torch.Tensor, head_dim: int, group: int, dtype: torch.dtype) -> torch.Tensor:
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"a cache in 4 bits is of float16 or bfloat16 tensors, got {dtype}")
+    if data.dtype != torch.uint8 or data.dim() != 4 or not data.is_contiguous() or data.shape[3] != kv4_slice_bytes(head_dim, group) \
+            or min(data.shape) < 1:
+        raise ValueError(f"data must be a contiguous uint8 [pages, kv_heads, page_size / 16, {kv4_slice_bytes(head_dim, group)}] tensor for "
+                         f"head_dim {head_dim} and groups of {group}")
+    return data
+
+
+def kv4_append(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, group: int) -> None:
+    """Quantises rows k, v [B, Hkv, n, D] (float16 or bfloat16, any strides) to 4 bits and writes them into the cache at slots [B, n]
+    (page * page_size + place; -1: nowhere), in place.  Of each group of channels: lowest = min, step = (max - min) / 15 cut off to
+    the type, code = (x - lowest) / step rounded; a group with an infinity or a NaN reads as NaN.  The slots of a call are
+    different ones (as plan_pages gives them).  No gradient."""
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+        raise ValueError("kv4_append: k and v [B, Hkv, n, D] of one shape, dtype and device")
+    B, H, n, D = k.shape
+    _kv4_data(data, D, group, k.dtype)
+    if data.shape[1] != H:
+        raise ValueError(f"kv4_append: rows of {H} heads, a cache of {data.shape[1]}")
+    _need_cuda(data, k, v, slots)
+    if k.device != data.device:
+        raise ValueError(f"kv4_append: rows on {k.device}, cache on {data.device}")
+    slots = _ints32("slots", slots, (B, n), data.device)
+    if B * n == 0:
+        return
+    k, v = _aligned_rows(k), _aligned_rows(v)
+    with _on(data):
+        rc = lib.psa_kv4_append(_ptr(data), _ptr(k), _ptr(v), _row_strides(k, v), _ptr(slots), data.shape[0], H, 16 * data.shape[2], B, n, D,
+                                group, _dt(k), _ptr(status_word(data.device)), _stream(data))
+    check(rc, "psa_kv4_append")
+
+
+def kv4_read(data: torch.Tensor, slots: torch.Tensor, head_dim: int, group: int, dtype: torch.dtype):
+    """The keys and values that slots [B, n] of the cache hold, as two [B, Hkv, n, D] tensors of dtype (that of the rows which were
+    appended); zeros where a slot is -1."""
+    _kv4_data(data, head_dim, group, dtype)
+    if slots.dim() != 2:
+        raise ValueError("kv4_read: slots [B, n]")
+    _need_cuda(data, slots)
+    slots = _ints32("slots", slots, slots.shape, data.device)
+    B, n = slots.shape
+    with _on(data):
+        k, v = (torch.empty((B, data.shape[1], n, head_dim), dtype=dtype, device=data.device) for _ in range(2))
+        if B * n == 0:
+            return k, v
+        rc = lib.psa_kv4_read(_ptr(data), _ptr(k), _ptr(v), _row_strides(k, v), _ptr(slots), data.shape[0], data.shape[1], 16 * data.shape[2], B,
+                              n, head_dim, group, _DT[dtype], _ptr(status_word(data.device)), _stream(data))
+    check(rc, "psa_kv4_read")
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, data: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, group: int,
+                  counts: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None, return_lse: bool = False):
+    """softmax(q k^T sm_scale) v of the newest tokens of every request over a cache held in 4 bits.
+
+    q [B, H, n, D] (float16 or bfloat16, any strides; H a multiple of the cache's heads, neighbouring heads share one); table int32
+    [B, width]: each request's pages; lengths int32 [B]: tokens in the cache, the new ones among them; counts [B]: how many of the n
+    query rows are a request's own (None: all of them).  Row i < counts[b] stands at lengths[b] - counts[b] + i and sees the keys up
+    to its own place; rows that see nothing, and rows behind counts[b], are 0.  What lies behind a length is not read into the result.
+    Returns [B, H, n, D] in q's order of dimensions, with return_lse also the logarithms of the sums, float32 [B, H, n] (-inf for a
+    row of nothing).  No gradient."""
+    if q.dim() != 4:
+        raise ValueError("kv4_attention: q [B, H, n, D]")
+    B, H, n, D = q.shape
+    _kv4_data(data, D, group, q.dtype)
+    if H < 1 or H % data.shape[1]:
+        raise ValueError(f"kv4_attention: {H} query heads on {data.shape[1]} key heads")
+    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1:
+        raise ValueError(f"kv4_attention: table [{B}, width]")
+    _need_cuda(q, data, table, lengths, counts)
+    if q.device != data.device:
+        raise ValueError(f"kv4_attention: q on {q.device}, cache on {data.device}")
+    _state32("table", table, table.shape, data.device), _state32("lengths", lengths, (B,), data.device)
+    counts = None if counts is None else _ints32("counts", counts, (B,), data.device)
+    sm_scale = D ** -0.5 if sm_scale is None else float(sm_scale)
+    q = _aligned_rows(q)
+    with _on(q):
+        out = _empty_rows(q)
+        lse = torch.empty((B, H, n), dtype=torch.float32, device=q.device) if return_lse else None
+        if B * n > 0:
+            nbytes = lib.psa_kv4_attention_scratch_bytes(B, n, H, data.shape[1], D)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            rc = lib.psa_kv4_attention(_ptr(q), _row_strides(q), _ptr(data), _ptr(table), _ptr(lengths), _ptr(counts), _ptr(out),
+                                       _row_strides(out), _ptr(lse), _ptr(scratch), nbytes, data.shape[0], 16 * data.shape[2], table.shape[1], B,
+                                       n, H, data.shape[1], D, group, sm_scale, _dt(q), _ptr(status_word(q.device)), _stream(q))
+            check(rc, "psa_kv4_attention")
+    return (out, lse) if return_lse else out
