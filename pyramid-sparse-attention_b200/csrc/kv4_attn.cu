@@ -1,5 +1,30 @@
 // Attention of the newest tokens of every request over the cache held in 4 bits (kv4.cuh).
+//
+// Scores and outputs without a decoded copy of the cache.  With s, lo the step and lowest value of group g and n the codes,
+//
+//   q . k  = sum_g  s (sum_d q_d n_d) + lo sum_d q_d                      sum over d in g: one product of q with the codes, on
+//                                                                         the tensor cores, scaled in 32 bits
+//   o_d    = sum_t (p_t s_t) (n_td - 8) + sum_t p_t (lo_t + 8 s_t)        the first sum is a product of codes with the weights
+//                                                                         times the step, the second a number per row and group
+//
+// Codes are exact in 16 bits.  The weights times the step are split into two bf16 terms (16 bits, and the exponents of 32-bit
+// numbers), so nothing but the output is rounded to the tensors' type; codes less 8 keep the accumulators near zero, where the
+// truncation of the tensor cores' sums does not add up.
+//
+// Work: one tile is 64 tokens of one key head, for up to R = 8 NT query rows (new tokens x query heads of that key head).  All tiles of
+// all requests stand in one line, and every block takes an equal stretch of it, computed from the lengths on the device: requests of
+// any mix of lengths load the GPU evenly.  A row's tiles may lie in several blocks; their parts (running maximum, sum, output) are
+// joined in order by a second kernel.  A block: one warp copies slices (16 tokens, contiguous) into a ring, four warps take a slice of
+// each tile.  A slice's bytes go from shared memory to matrix operands with masks and shifts: tokens are the 16 rows of
+// m16n8k16, query rows its 8 columns, and the channel order within a product is whatever the stored words give, the same for q.
+//
+// The bound is the cache's bytes (160 a token and key head at head_dim 128, groups of 32).  mma.sync and not tcgen05: 8 query rows
+// against 128 rows of a tcgen05 tile, and operands that are made in registers; the products take a fifth of a warp's issue slots.
+#include <type_traits>
+
 #include "kv4.cuh"
+#include "mma_sync.cuh"
+#include "tc_common.cuh"
 
 namespace psa {
 namespace {
@@ -15,93 +40,599 @@ struct AttnArgs {
   int64_t pages;
   int batch, tokens, heads, kv_heads, width, page;
   float scale;
+  int least_tiles;     // a block takes at least so many
+  int row_tiles;       // of a request that brings all `tokens`
+  int2* owners;        // [batch][kv_heads][row_tiles]: first and last block of a unit (rows of a tile x a key head)
+  float* parts;        // [blocks][2]: what a block has of a unit that began before it, and of one that goes on behind it
 };
 
-// One query row a block: a thread scores one of 128 tokens, then gathers one channel over them.
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(128) kv4_attn_rows_kernel(const AttnArgs a) {
-  using L = Kv4<D, G>;
-  __shared__ float q[D], p[128], red[4];
-  __shared__ int64_t at[128];
-  const int i = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, group = a.heads / a.kv_heads;
-  int64_t length = a.lengths[b];
-  const int count = a.counts ? a.counts[b] : a.tokens;
-  if (length < 0 || length > (int64_t)a.width * a.page || count < 0 || count > a.tokens) {
-    if (tid == 0) *a.status = PSA_ERR_ARG;
-    length = min(max(length, (int64_t)0), (int64_t)a.width * a.page);
+template <typename T>
+__device__ __forceinline__ void write_row(const AttnArgs& a, int b, int head, int i, int d, float4 o, float top, float sum) {
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  T* to = static_cast<T*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + i * a.out_stride[2] + d;
+  uint2 w;
+  w.x = MmaOp<T>::pack(o.x * f, o.y * f);
+  w.y = MmaOp<T>::pack(o.z * f, o.w * f);
+  *reinterpret_cast<uint2*>(to) = w;
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + head) * a.tokens + i] = sum == 0.f ? -INFINITY : 0.6931471805599453f * (top + log2f(sum));
+}
+
+
+constexpr int kWarps = 4, kThreads = 32 * (kWarps + 1), kTile = 16 * kWarps;
+constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has seen nothing: exp2(-inf - kLowest) is 0
+constexpr float kLazy = 8.f;                   // a row's reference moves when a score is more than this above it (log2)
+
+template <int D, int G, int NT>
+struct Shape {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kSlice = Kv4<D, G>::kSlice;
+  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kOutRow = D + 4;                                            // floats; 4 more spread the banks
+  static constexpr int kOut = kStages * kWarps * kSlice;                           // [warps][rows][kOutRow]
+  static constexpr int kStats = kOut + kWarps * kRows * kOutRow * 4;               // [warps][rows][2]
+  static constexpr int kBars = kStats + kWarps * kRows * 2 * 4;                    // full, empty
+  static constexpr int kMore = kBars + 2 * kStages * 8;                            // valid[stages], scan[8], abort
+  static constexpr int kBytes = kMore + (kStages + 16) * 8;
+  // scratch: [ctas][2 parts] of output rows and {maximum, sum}
+  static constexpr int64_t kPart = (int64_t)kRows * (D + 2);
+};
+
+struct Span {   // a request's place in the line of tiles
+  int rows, row_tiles, tiles;
+  int64_t work;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_tile, int& length, int& count) {
+  length = a.lengths[b];
+  count = a.counts ? a.counts[b] : a.tokens;
+  const int most = a.width * a.page;
+  if (length < 0 || length > most || count < 0 || count > a.tokens) {
+    *a.status = PSA_ERR_ARG;
+    length = min(max(length, 0), most);
+    count = min(max(count, 0), a.tokens);
   }
-  const int64_t seen = i < count ? length - count + i + 1 : 0;
-  const T* row = static_cast<const T*>(a.q) + b * a.q_stride[0] + head * a.q_stride[1] + i * a.q_stride[2];
-  if (tid < D) q[tid] = Elem<T>::to_f(row[tid]);
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int64_t t0 = 0; t0 < seen; t0 += 128) {
+  Span s;
+  s.rows = count * (a.heads / a.kv_heads);
+  s.row_tiles = (s.rows + rows_per_tile - 1) / rows_per_tile;
+  s.tiles = (length + kTile - 1) / kTile;
+  s.work = (int64_t)s.tiles * s.row_tiles * a.kv_heads;
+  return s;
+}
+
+// The block's stretch [first, last) of the line, and the request that `first` lies in with the place where that begins.
+struct Stretch {
+  int64_t first, last, base, work, blocks;
+  int request;
+};
+__device__ __forceinline__ Stretch stretch_of(const AttnArgs& a, int rows_per_tile, int64_t* scan) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int length, count;
+  Stretch s;
+  int64_t mine = 0;
+  for (int b = threadIdx.x; b < a.batch; b += kThreads) mine += span_of(a, b, rows_per_tile, length, count).work;
+#pragma unroll
+  for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(~0u, mine, d);
+  if (lane == 0) scan[warp] = mine;
+  __syncthreads();
+  s.work = 0;
+#pragma unroll
+  for (int w = 0; w <= kWarps; ++w) s.work += scan[w];
+  s.blocks = min((int64_t)gridDim.x, (s.work + a.least_tiles - 1) / a.least_tiles);
+  s.first = s.last = s.base = 0;
+  s.request = 0;
+  if (blockIdx.x >= s.blocks) return s;
+  s.first = blockIdx.x * s.work / s.blocks;
+  s.last = (blockIdx.x + 1) * s.work / s.blocks;
+  if (a.batch == 1) return s;
+  // whose stretch it is: requests in rounds of one a thread
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const int64_t own = b < a.batch ? span_of(a, b, rows_per_tile, length, count).work : 0;
+    int64_t sum = own;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int64_t y = __shfl_up_sync(~0u, sum, d);
+      if (lane >= d) sum += y;
+    }
     __syncthreads();
-    const int64_t t = t0 + tid;
-    float s = -INFINITY;
-    int64_t from = -1;
-    if (t < seen) {
-      const int page = a.table[(int64_t)b * a.width + t / a.page];
-      if (page >= 0 && page < a.pages) {
-        from = (((int64_t)page * a.kv_heads + head / group) * (a.page / 16) + t % a.page / 16) * L::kSlice;
-        const uint8_t* slice = a.data + from;
-        const int r = (int)(t % 16);
-        s = 0.f;
-        for (int g = 0; g < L::kGroups; ++g) {
-          const T* par = reinterpret_cast<const T*>(slice + L::k_param(r, g));
-          float dot = 0.f, sum = 0.f;
-          for (int d = g * G; d < (g + 1) * G; d += 8) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(slice + L::k_word(r, d));
-            for (int j = 0; j < 8; ++j) {
-              dot += q[d + j] * (float)(w >> (4 * j) & 15);
-              sum += q[d + j];
+    if (lane == 31) scan[warp] = sum;
+    __syncthreads();
+    int64_t start = before + sum - own;
+    for (int w = 0; w < warp; ++w) start += scan[w];
+    for (int w = 0; w <= kWarps; ++w) before += scan[w];
+    if (s.first >= start && s.first < start + own) {
+      scan[6] = b;
+      scan[7] = start;
+    }
+    if (before > s.first) break;
+  }
+  __syncthreads();
+  s.request = (int)scan[6];
+  s.base = scan[7];
+  return s;
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, int shift, uint32_t magic) { return ((w >> shift) & 0x000f000fu) | magic; }
+// bf16 128 + n, twice, less 136
+__device__ __forceinline__ uint32_t centred(uint32_t w, int shift) {
+  const uint32_t x = nibbles(w, shift, 0x43004300u), m = 0x43084308u;
+  const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&m));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+// step and lowest value of a group
+template <typename T> __device__ __forceinline__ float2 param(uint32_t w);
+template <> __device__ __forceinline__ float2 param<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 param<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+template <int N> struct Words { uint32_t w[N]; };
+template <int N> __device__ __forceinline__ Words<N> lds(const uint8_t* p) {
+  Words<N> r;
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(p);
+  else r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  return r;
+}
+
+// What a warp carries of a unit's rows: operands of q, and per row its reference (log2), sum, output and the share of the output
+// that the groups' middle values give.  Lane 4 r + c: rows of q 8 nt + r as operands, 8 nt + 2 c + {0, 1} as columns.
+template <typename T, int D, int G, int NT>
+struct Rows {
+  static constexpr int NG = D / G, NB = D / 32;
+  uint32_t q[NT][NB][2][2];
+  float q_sum[NT][NG][2];
+  float top[NT][2], sum[NT][2];
+  float out[NT][2 * NB][4];
+  float mid[NT][NG][2];
+  int seen[NT][2];          // keys that a column's row sees
+};
+
+template <typename T, int D, int G, int NT, bool MASKED>
+__device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* slice, int t0, float scale_log2) {
+  using L = Kv4<D, G>;
+  constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
+  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  // ---- scores: rows are the tokens r/2 + 4 (r % 2) and that + 8, which lie in rows r and r + 8 of the keys
+  float x[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+  {
+    const Words<NB> k0 = lds<NB>(slice + r * L::kRow + c * NB * 4), k1 = lds<NB>(slice + (r + 8) * L::kRow + c * NB * 4);
+    const Words<NG> p0 = lds<NG>(slice + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kParams + (r + 8) * NG * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float acc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < BG; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          // bf16: 128 + n.  f16: n 2^-24, a subnormal number
+          constexpr uint32_t magic = kBf16 ? 0x43004300u : 0u;
+          const uint32_t w0 = k0.w[g * BG + i], w1 = k1.w[g * BG + i];
+          const uint32_t a[4] = {nibbles(w0, 8 * k, magic), nibbles(w1, 8 * k, magic), nibbles(w0, 8 * k + 4, magic), nibbles(w1, 8 * k + 4, magic)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
+        }
+      float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
+      if constexpr (kBf16) {
+        u0.y = fmaf(-128.f, u0.x, u0.y);
+        u1.y = fmaf(-128.f, u1.x, u1.y);
+      } else {
+        u0.x *= 16777216.f;
+        u1.x *= 16777216.f;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          x[nt][j] = fmaf(u0.x, acc[nt][j], fmaf(u0.y, s.q_sum[nt][g][j], x[nt][j]));
+          x[nt][2 + j] = fmaf(u1.x, acc[nt][2 + j], fmaf(u1.y, s.q_sum[nt][g][j], x[nt][2 + j]));
+        }
+    }
+  }
+  const int token = t0 + (r >> 1) + 4 * (r & 1);
+  bool rises = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[nt][j] *= scale_log2;
+      if (MASKED && token + 8 * (j >> 1) >= s.seen[nt][j & 1]) x[nt][j] = -INFINITY;
+      rises = rises || x[nt][j] > s.top[nt][j & 1] + kLazy;
+    }
+  // ---- the reference of a row moves seldom: only when a score would make a weight larger than 2^8
+  if (__any_sync(~0u, rises)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float m = fmaxf(x[nt][j], x[nt][2 + j]);
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+        m = fmaxf(m, s.top[nt][j]);
+        const float fade = exp2f(s.top[nt][j] - m);
+        s.top[nt][j] = m;
+        s.sum[nt][j] *= fade;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) s.mid[nt][g][j] *= fade;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+          s.out[nt][i][j] *= fade;
+          s.out[nt][i][2 + j] *= fade;
+        }
+      }
+  }
+  float p[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      p[nt][j] = exp2f(x[nt][j] - s.top[nt][j & 1]);
+      s.sum[nt][j & 1] += p[nt][j];
+    }
+  // ---- outputs: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12); channels 32 b + 4 r + 0..3
+  constexpr int kV = NB / 2;
+  Words<kV> v[4];
+  {
+    const int e = D == 128 ? r ^ ((c >> 1) << 2) : r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = lds<kV>(slice + L::kHalf + (c + 4 * i) * L::kRow + e * NB * 2);
+  }
+  const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
+    const float m0 = fmaf(8.f, u0.x, u0.y), m1 = fmaf(8.f, u1.x, u1.y);
+    uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = p[nt][j] * (j < 2 ? u0.x : u1.x);
+        const float z = p[nt][j] * (j < 2 ? m0 : m1);
+        if (MASKED) {   // what a row does not see may be anything, NaN too
+          const bool hidden = token + 8 * (j >> 1) >= s.seen[nt][j & 1];
+          y[j] = hidden ? 0.f : y[j];
+          s.mid[nt][g][j & 1] += hidden ? 0.f : z;
+        } else {
+          s.mid[nt][g][j & 1] += z;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t h = MmaOp<__nv_bfloat16>::pack(y[2 * i], y[2 * i + 1]);
+        const uint32_t l = MmaOp<__nv_bfloat16>::pack(y[2 * i] - __uint_as_float(h << 16), y[2 * i + 1] - __uint_as_float(h & 0xffff0000u));
+        hi[nt][i] = movmatrix(h);
+        lo[nt][i] = movmatrix(l);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BG; ++i) {
+      const int b = g * BG + i;
+      const uint32_t pick = b & 1 ? 0x7632u : 0x5410u;
+      const uint32_t v0 = __byte_perm(v[0].w[b >> 1], v[1].w[b >> 1], pick), v1 = __byte_perm(v[2].w[b >> 1], v[3].w[b >> 1], pick);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t a[4] = {centred(v0, 8 * h), centred(v0, 8 * h + 4), centred(v1, 8 * h), centred(v1, 8 * h + 4)};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          MmaOp<__nv_bfloat16>::run(s.out[nt][2 * b + h], a, hi[nt]);
+          MmaOp<__nv_bfloat16>::run(s.out[nt][2 * b + h], a, lo[nt]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int D, int G, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ AttnArgs a) {
+  using L = Kv4<D, G>;
+  using S = Shape<D, G, NT>;
+  using R = Rows<T, D, G, NT>;
+  constexpr int NG = L::kGroups, NB = L::kBlocks, kRows = S::kRows, kStages = S::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* out_s = reinterpret_cast<float*>(smem + S::kOut);
+  float* stats_s = reinterpret_cast<float*>(smem + S::kStats);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* empty = full + kStages;
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + S::kMore);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(scan + 8);
+  volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(scan + 9);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      tc::mbar_init(full + i, 1);
+      tc::mbar_init(empty + i, kWarps);
+    }
+    tc::fence_mbar_init();
+    *abort_flag = 0;
+  }
+  const Stretch line = stretch_of(a, kRows, scan);
+  __syncthreads();
+  if (line.first >= line.last) return;
+  const int group = a.heads / a.kv_heads, slices_per_page = a.page / 16;
+  int stage = 0;
+  uint32_t phase = 0;
+  int64_t at = line.first, base = line.base;
+  for (int b = line.request; at < line.last; ++b) {
+    int length, count;
+    const Span span = span_of(a, b, kRows, length, count);
+    const int64_t end = base + span.work;
+    while (at < line.last && at < end) {
+      const int64_t unit = (at - base) / span.tiles;
+      const int tile0 = (int)(at - base - unit * span.tiles);
+      const int tiles = (int)min((int64_t)(span.tiles - tile0), line.last - at);
+      const int head = (int)(unit / span.row_tiles), row0 = (int)(unit - (int64_t)head * span.row_tiles) * kRows;
+      if (warp == kWarps) {
+        // ------------------------------------------------------------ copies: a lane a slice, eight tiles' page numbers at a time
+        const int slices = (length + 15) / 16, first_slice = tile0 * kWarps, last_slice = min(slices, (tile0 + tiles) * kWarps);
+        for (int s0 = first_slice; s0 < last_slice; s0 += 32) {
+          const int s = s0 + lane;
+          int64_t from = -1;
+          if (s < last_slice) {
+            const int page = a.table[(int64_t)b * a.width + s / slices_per_page];
+            if (page >= 0 && page < a.pages) from = (((int64_t)page * a.kv_heads + head) * slices_per_page + s % slices_per_page) * L::kSlice;
+            else *a.status = PSA_ERR_ARG;
+          }
+          const uint32_t good = __ballot_sync(~0u, from >= 0);
+          for (int k = 0; k < 8 && s0 + kWarps * k < last_slice; ++k) {
+            const uint32_t bits = good >> (kWarps * k) & ((1u << kWarps) - 1);
+            const bool ok = !*abort_flag && tc::mbar_wait(empty + stage, phase ^ 1, abort_flag);
+            if (__all_sync(~0u, ok)) {
+              if (lane == 0) {
+                valid[stage] = bits;
+                tc::mbar_arrive_expect_tx(full + stage, __popc(bits) * L::kSlice);
+              }
+              __syncwarp();
+              if (from >= 0 && lane / kWarps == k)
+                tc::bulk_load_a(tc::smem_u32(smem + (stage * kWarps + lane % kWarps) * L::kSlice), a.data + from, L::kSlice, tc::smem_u32(full + stage));
+            }
+            if (++stage == kStages) stage = 0, phase ^= 1;
+          }
+        }
+      } else {
+        // ------------------------------------------------------------ products
+        R s;
+        const int r = lane >> 2, c = lane & 3;
+        const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int row = row0 + 8 * nt + r;
+          const bool in = row < span.rows;
+          const T* from = q + (int64_t)(head * group + row % group) * a.q_stride[1] + (int64_t)(row / group) * a.q_stride[2] + 8 * c;
+          float sums[NG];
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const uint4 w = in ? *reinterpret_cast<const uint4*>(from + 32 * i) : make_uint4(0, 0, 0, 0);
+            s.q[nt][i][0][0] = __byte_perm(w.x, w.z, 0x5410);
+            s.q[nt][i][0][1] = __byte_perm(w.x, w.z, 0x7632);
+            s.q[nt][i][1][0] = __byte_perm(w.y, w.w, 0x5410);
+            s.q[nt][i][1][1] = __byte_perm(w.y, w.w, 0x7632);
+            const float2 e0 = param<T>(w.x), e1 = param<T>(w.y), e2 = param<T>(w.z), e3 = param<T>(w.w);
+            const float sum = ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+            if (i % (G / 32) == 0) sums[i / (G / 32)] = sum;
+            else sums[i / (G / 32)] += sum;
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            sums[g] += __shfl_xor_sync(~0u, sums[g], 1);
+            sums[g] += __shfl_xor_sync(~0u, sums[g], 2);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              s.q_sum[nt][g][j] = __shfl_sync(~0u, sums[g], 4 * (2 * c + j));
+              s.mid[nt][g][j] = 0.f;
             }
           }
-          s += Elem<T>::to_f(par[0]) * dot + Elem<T>::to_f(par[1]) * sum;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = row0 + 8 * nt + 2 * c + j;
+            s.seen[nt][j] = col < span.rows ? length - count + col / group + 1 : 0;
+            s.top[nt][j] = kLowest;
+            s.sum[nt][j] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 2 * NB; ++i) s.out[nt][i][0] = s.out[nt][i][1] = s.out[nt][i][2] = s.out[nt][i][3] = 0.f;
         }
-        s *= a.scale;
-      } else {
-        *a.status = PSA_ERR_ARG;
+        const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
+        for (int i = 0; i < tiles; ++i) {
+          const bool ok = !*abort_flag && tc::mbar_wait(full + stage, phase, abort_flag);
+          if (__all_sync(~0u, ok)) {
+            if (valid[stage] >> warp & 1) {
+              const uint8_t* slice = smem + (stage * kWarps + warp) * L::kSlice;
+              const int t0 = (tile0 + i) * kTile + 16 * warp;
+              if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0, a.scale * 1.4426950408889634f);
+              else take_slice<T, D, G, NT, true>(s, slice, t0, a.scale * 1.4426950408889634f);
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(empty + stage);
+          }
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+        // ------------------------------------------------------------ the four warps' rows into one
+        float* mine = out_s + warp * kRows * S::kOutRow;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float sum = s.sum[nt][j];
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
+            const int row = 8 * nt + 2 * c + j;
+            if (r == 0) {
+              stats_s[(warp * kRows + row) * 2] = s.top[nt][j];
+              stats_s[(warp * kRows + row) * 2 + 1] = sum;
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              float mid = s.mid[nt][g][j];
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) mid += __shfl_xor_sync(~0u, mid, d);
+#pragma unroll
+              for (int i = g * (G / 32); i < (g + 1) * (G / 32); ++i)
+                *reinterpret_cast<float4*>(mine + row * S::kOutRow + 32 * i + 4 * r) =
+                    make_float4(s.out[nt][2 * i][j] + mid, s.out[nt][2 * i][2 + j] + mid, s.out[nt][2 * i + 1][j] + mid, s.out[nt][2 * i + 1][2 + j] + mid);
+            }
+          }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+        const bool starts = tile0 == 0, whole = starts && tiles == span.tiles;
+        float* part = a.parts + ((int64_t)blockIdx.x * 2 + starts) * S::kPart;
+        for (int i = threadIdx.x; i < kRows * D / 4; i += 32 * kWarps) {
+          const int row = i / (D / 4), d = i % (D / 4) * 4;
+          if (row0 + row >= span.rows) break;
+          float top = kLowest, sum = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stats_s[(w * kRows + row) * 2]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float f = exp2f(stats_s[(w * kRows + row) * 2] - top);
+            const float4 y = *reinterpret_cast<const float4*>(out_s + (w * kRows + row) * S::kOutRow + d);
+            sum = fmaf(f, stats_s[(w * kRows + row) * 2 + 1], sum);
+            o.x = fmaf(f, y.x, o.x);
+            o.y = fmaf(f, y.y, o.y);
+            o.z = fmaf(f, y.z, o.z);
+            o.w = fmaf(f, y.w, o.w);
+          }
+          if (whole) {
+            write_row<T>(a, b, head * group + (row0 + row) % group, (row0 + row) / group, d, o, top, sum);
+          } else {
+            *reinterpret_cast<float4*>(part + row * D + d) = o;
+            if (d == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * row) = make_float2(top, sum);
+          }
+        }
+        if (starts && threadIdx.x == 0) {
+          // whose parts the unit is made of: from this block to the one that holds its last tile
+          const int64_t last = at + span.tiles - 1;
+          a.owners[((int64_t)b * a.kv_heads + head) * a.row_tiles + row0 / kRows] =
+              make_int2((int)blockIdx.x, (int)(((last + 1) * line.blocks - 1) / line.work));
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
       }
+      at += tiles;
     }
-    at[tid] = from;
-    float top = s;
-    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    if (tid % 32 == 0) red[tid / 32] = top;
-    __syncthreads();
-    top = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float e = from >= 0 ? expf(s - ref) : 0.f;
-    p[tid] = e;
-    float sum = e;
-    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-    __syncthreads();
-    if (tid % 32 == 0) red[tid / 32] = sum;
-    __syncthreads();
-    const float fade = m == -INFINITY ? 0.f : expf(m - ref);
-    l = l * fade + red[0] + red[1] + red[2] + red[3];
-    m = top;
-    if (tid < D) {
-      acc *= fade;
-      for (int j = 0; j < 128 && t0 + j < seen; ++j) {
-        if (at[j] < 0) continue;
-        const uint8_t* slice = a.data + at[j];
-        const int r = (int)((t0 + j) % 16);
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(slice + L::v_unit(r, tid));
-        const T* par = reinterpret_cast<const T*>(slice + L::v_param(r, tid / G));
-        acc += p[j] * (Elem<T>::to_f(par[1]) + Elem<T>::to_f(par[0]) * (float)(w >> (tid % 4 * 4) & 15));
-      }
-    }
+    base = end;
   }
-  if (tid < D)
-    static_cast<T*>(a.out)[b * a.out_stride[0] + head * a.out_stride[1] + i * a.out_stride[2] + tid] = Elem<T>::from_f(l == 0.f ? 0.f : acc / l);
-  if (a.lse && tid == 0) a.lse[((int64_t)b * a.heads + head) * a.tokens + i] = l == 0.f ? -INFINITY : m + logf(l);
+  if (*abort_flag) {
+    if (threadIdx.x == 0) *a.status = PSA_ERR_TIMEOUT;
+    // copies still in flight must have landed before the block's memory is another's
+    if (warp == kWarps && lane == 0)
+      for (int i = 0; i < kStages; ++i) {
+        int unused = 0;
+        tc::mbar_wait(full + i, i < stage ? phase : phase ^ 1, &unused);
+      }
+  }
+}
+
+// Rows whose tiles lay in several blocks, from their parts in order; rows of nothing.  A block a row, its warps take every fourth part.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ AttnArgs a, int rows_per_tile) {
+  __shared__ float out_s[4][D], stats_s[4][2];
+  const int group = a.heads / a.kv_heads, i = blockIdx.x, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.y;
+  int length, count;
+  const Span span = span_of(a, b, rows_per_tile, length, count);
+  const int row = i * group + head % group;
+  int2 owners = make_int2(0, -1);
+  if (i < count && span.tiles) {
+    owners = a.owners[((int64_t)b * a.kv_heads + head / group) * a.row_tiles + row / rows_per_tile];
+    if (owners.x == owners.y) return;
+  }
+  const int64_t size = (int64_t)rows_per_tile * (D + 2);
+  const int r = row % rows_per_tile;
+  constexpr int kLanes = D / 4;
+  float top = kLowest, sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = owners.x + warp; k <= owners.y; k += 4) {
+    const float* part = a.parts + ((int64_t)k * 2 + (k == owners.x)) * size;
+    const float2 st = *reinterpret_cast<const float2*>(part + rows_per_tile * D + 2 * r);
+    const float4 y = lane < kLanes ? *reinterpret_cast<const float4*>(part + r * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float m = fmaxf(top, st.x), f0 = exp2f(top - m), f1 = exp2f(st.x - m);
+    top = m;
+    sum = sum * f0 + st.y * f1;
+    o.x = o.x * f0 + y.x * f1;
+    o.y = o.y * f0 + y.y * f1;
+    o.z = o.z * f0 + y.z * f1;
+    o.w = o.w * f0 + y.w * f1;
+  }
+  if (lane < kLanes) *reinterpret_cast<float4*>(&out_s[warp][4 * lane]) = o;
+  if (lane == 0) stats_s[warp][0] = top, stats_s[warp][1] = sum;
+  __syncthreads();
+  if (threadIdx.x < kLanes) {
+    const int d = 4 * threadIdx.x;
+    top = fmaxf(fmaxf(stats_s[0][0], stats_s[1][0]), fmaxf(stats_s[2][0], stats_s[3][0]));
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2f(stats_s[w][0] - top);
+      sum += f * stats_s[w][1];
+      o.x += f * out_s[w][d];
+      o.y += f * out_s[w][d + 1];
+      o.z += f * out_s[w][d + 2];
+      o.w += f * out_s[w][d + 3];
+    }
+    write_row<T>(a, b, head, i, d, o, top, sum);
+  }
+}
+
+int sm_count() {   // of the current device; asked once for each
+  static int known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148;
+  if (dev < 64 && known[dev]) return known[dev];
+  int n = 148;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) known[dev] = n;
+  return n;
+}
+
+constexpr int kMostBlocks = 4 * 160;   // of the first kernel: parts of the scratch are laid out for them
+int rows_per_tile(int64_t rows) { return rows <= 8 ? 8 : 16; }
+size_t owners_bytes(int64_t batch, int kv_heads, int64_t row_tiles) { return ((size_t)batch * kv_heads * row_tiles * sizeof(int2) + 255) & ~(size_t)255; }
+
+template <typename T, int D, int G, int NT>
+int launch(const AttnArgs& a, cudaStream_t st) {
+  using S = Shape<D, G, NT>;
+  auto kernel = kv4_attn_kernel<T, D, G, NT>;
+  static thread_local uint64_t ready = 0;   // devices that know the kernel's shared memory, per thread
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !(ready >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
+      set_error("psa_kv4_attention: %d bytes of shared memory: %s", S::kBytes, cudaGetErrorString(cudaGetLastError()));
+      return PSA_ERR_CUDA;
+    }
+    if (dev < 64) ready |= (uint64_t)1 << dev;
+  }
+  int blocks = sm_count() * (NT == 1 ? 3 : 2);
+  if (blocks > kMostBlocks) blocks = kMostBlocks;
+  kernel<<<blocks, kThreads, S::kBytes, st>>>(a);
+  PSA_CHECK_LAUNCH("psa_kv4_attention");
+  const dim3 grid((unsigned)a.tokens, (unsigned)a.heads, (unsigned)a.batch);
+  kv4_join_kernel<T, D><<<grid, 128, 0, st>>>(a, S::kRows);
+  PSA_CHECK_LAUNCH("psa_kv4_attention");
+  return PSA_OK;
 }
 
 }  // namespace
 }  // namespace psa
 
 extern "C" size_t psa_kv4_attention_scratch_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim) {
-  return batch > 0 && tokens > 0 && heads > 0 && kv_heads > 0 && head_dim > 0 ? 16 : 0;
+  using namespace psa;
+  if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  const int64_t rows = tokens * (heads / kv_heads), r = rows_per_tile(rows);
+  return owners_bytes(batch, kv_heads, cdiv64(rows, r)) + (size_t)kMostBlocks * 2 * r * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const void* data, const int32_t* table, const int32_t* lengths,
@@ -123,7 +654,7 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   PSA_REQUIRE((((uintptr_t)data | (uintptr_t)q | (uintptr_t)out) & 15) == 0, PSA_ERR_ARG, "psa_kv4_attention: operands must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     PSA_REQUIRE(q_strides[i] % 8 == 0 && out_strides[i] % 8 == 0, PSA_ERR_ARG, "psa_kv4_attention: strides must be multiples of 8 elements");
-  PSA_REQUIRE(scratch_bytes >= psa_kv4_attention_scratch_bytes(batch, tokens, heads, kv_heads, head_dim), PSA_ERR_ARG,
+  PSA_REQUIRE(((uintptr_t)scratch & 15) == 0 && scratch_bytes >= psa_kv4_attention_scratch_bytes(batch, tokens, heads, kv_heads, head_dim), PSA_ERR_ARG,
               "psa_kv4_attention: scratch of %zu bytes", scratch_bytes);
   AttnArgs a = {};
   a.q = q;
@@ -146,8 +677,12 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   a.width = (int)width;
   a.page = page_size;
   a.scale = sm_scale;
-  const dim3 grid((unsigned)tokens, (unsigned)heads, (unsigned)batch);
-  PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_attn_rows_kernel<T, D, G><<<grid, 128, 0, (cudaStream_t)stream>>>(a));
-  PSA_CHECK_LAUNCH("psa_kv4_attention");
+  const int64_t rows = tokens * (heads / kv_heads);
+  a.least_tiles = 2;
+  a.row_tiles = (int)cdiv64(rows, rows_per_tile(rows));
+  a.owners = static_cast<int2*>(scratch);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + owners_bytes(batch, kv_heads, a.row_tiles));
+  if (rows_per_tile(rows) == 8) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, return (launch<T, D, G, 1>(a, (cudaStream_t)stream)));
+  else PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, return (launch<T, D, G, 2>(a, (cudaStream_t)stream)));
   return PSA_OK;
 }
