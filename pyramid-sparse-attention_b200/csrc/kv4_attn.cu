@@ -7,9 +7,10 @@
 //   o_d    = sum_t (p_t s_t) (n_td - 8) + sum_t p_t (lo_t + 8 s_t)        the first sum is a product of codes with the weights
 //                                                                         times the step, the second a number per row and group
 //
-// Codes are exact in 16 bits.  The weights times the step are split into two bf16 terms (16 bits, and the exponents of 32-bit
-// numbers), so nothing but the output is rounded to the tensors' type; codes less 8 keep the accumulators near zero, where the
-// truncation of the tensor cores' sums does not add up.
+// Codes are exact in f16, and so is q times a power of two per row.  The weights times the step are rounded to f16 (11 bits, whatever the
+// tensors' type); the references of the rows keep them in its range.  Codes less 8 - a second product, with a constant - keep the
+// accumulators near zero: sums of codes from 0 to 15 grow with the context, the tensor cores cut their sums off, and what is cut
+// off adds up (0.1 % of an output of 131072 evenly weighted keys).
 //
 // Work: one tile is 64 tokens of one key head, for up to R = 8 NT query rows (new tokens x query heads of that key head).  All tiles of
 // all requests stand in one line, and every block takes an equal stretch of it, computed from the lengths on the device: requests of
@@ -60,7 +61,12 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int b, int head, in
 
 constexpr int kWarps = 4, kThreads = 32 * (kWarps + 1), kTile = 16 * kWarps;
 constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has seen nothing: exp2(-inf - kLowest) is 0
-constexpr float kLazy = 8.f;                   // a row's reference moves when a score is more than this above it (log2)
+// A weight is 2^(score - reference).  References are set so that the largest score so far, times the largest step of the values so far, gives
+// 2^kHead, and move when a weight times a step could be 2^kLazy times that: f16 has its full precision from 2^-14 to 2^16, so a
+// weight 2^-21 of the largest is still rounded to 11 bits.
+constexpr float kHead = 7.f, kLazy = 8.f;
+constexpr float kLeastCap = 5.9604644775390625e-8f;   // 2^-24
+constexpr float kSumScale = 2.44140625e-4f;           // 2^12 (sums of q are kept 2^-12 of q's operands) 2^-24 (codes)
 
 template <int D, int G, int NT>
 struct Shape {
@@ -157,12 +163,13 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int shift, uint32_t magic) { return ((w >> shift) & 0x000f000fu) | magic; }
-// bf16 128 + n, twice, less 136
-__device__ __forceinline__ uint32_t centred(uint32_t w, int shift) {
-  const uint32_t x = nibbles(w, shift, 0x43004300u), m = 0x43084308u;
-  const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&m));
-  return *reinterpret_cast<const uint32_t*>(&y);
+// Codes of nibbles i and i + 4 as two f16 numbers: n 2^-24 for even i, n 2^-20 for odd ones.  (Subnormal numbers: a nibble is a number
+// where it stands, with no exponent to add and no offset to take off again.)
+__device__ __forceinline__ uint32_t codes(uint32_t w, int i) { return (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // step and lowest value of a group
 template <typename T> __device__ __forceinline__ float2 param(uint32_t w);
@@ -186,23 +193,36 @@ template <typename T, int D, int G, int NT>
 struct Rows {
   static constexpr int NG = D / G, NB = D / 32;
   uint32_t q[NT][NB][2][2];
-  float q_sum[NT][NG][2];
-  float top[NT][2], sum[NT][2];
-  float out[NT][2 * NB][4];
+  uint32_t q_sum[NT][2];    // (0, sum of q over group c) in two terms of the tensors' type
+  float factor[NT][2];      // of a column's scores, to log2
+  float ref[NT][2], sum[NT][2];
+  float out[NT][2 * NB][4]; // of channels 4 i, 4 i + 2: times 2^-24, of the others: times 2^-20
   float mid[NT][NG][2];
+  float cap, limit;         // at least the largest step of the values so far, and the exponent from which a weight is too large
   int seen[NT][2];          // keys that a column's row sees
+  int last;                 // keys of the request
 };
 
 template <typename T, int D, int G, int NT, bool MASKED>
-__device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* slice, int t0, float scale_log2) {
+__device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* slice, int t0) {
   using L = Kv4<D, G>;
   constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
-  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   // ---- scores: rows are the tokens r/2 + 4 (r % 2) and that + 8, which lie in rows r and r + 8 of the keys
   float x[NT][4];
+  {
+    // sum_g lo_g (sum of q over g) is a product too: the parameter words themselves are its operand, a group's step against 0
+    const uint8_t* p = slice + L::kParams + (c < NG ? c : 0) * 4;
+    const uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
+    const uint32_t a[4] = {w0, w1, w0, w1};
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+      MmaOp<T>::run(x[nt], a, s.q_sum[nt]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[nt][j] *= kSumScale;
+    }
+  }
   {
     const Words<NB> k0 = lds<NB>(slice + r * L::kRow + c * NB * 4), k1 = lds<NB>(slice + (r + 8) * L::kRow + c * NB * 4);
     const Words<NG> p0 = lds<NG>(slice + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kParams + (r + 8) * NG * 4);
@@ -215,53 +235,70 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
       for (int i = 0; i < BG; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          // bf16: 128 + n.  f16: n 2^-24, a subnormal number
-          constexpr uint32_t magic = kBf16 ? 0x43004300u : 0u;
           const uint32_t w0 = k0.w[g * BG + i], w1 = k1.w[g * BG + i];
-          const uint32_t a[4] = {nibbles(w0, 8 * k, magic), nibbles(w1, 8 * k, magic), nibbles(w0, 8 * k + 4, magic), nibbles(w1, 8 * k + 4, magic)};
+          const uint32_t a[4] = {codes(w0, 2 * k), codes(w1, 2 * k), codes(w0, 2 * k + 1), codes(w1, 2 * k + 1)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
+          for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
         }
-      float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
-      if constexpr (kBf16) {
-        u0.y = fmaf(-128.f, u0.x, u0.y);
-        u1.y = fmaf(-128.f, u1.x, u1.y);
-      } else {
-        u0.x *= 16777216.f;
-        u1.x *= 16777216.f;
-      }
+      const float s0 = param<T>(p0.w[g]).x, s1 = param<T>(p1.w[g]).x;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          x[nt][j] = fmaf(u0.x, acc[nt][j], fmaf(u0.y, s.q_sum[nt][g][j], x[nt][j]));
-          x[nt][2 + j] = fmaf(u1.x, acc[nt][2 + j], fmaf(u1.y, s.q_sum[nt][g][j], x[nt][2 + j]));
-        }
+        for (int j = 0; j < 4; ++j) x[nt][j] = fmaf(j < 2 ? s0 : s1, acc[nt][j], x[nt][j]);
+    }
+  }
+  // ---- values' parameters
+  float step[NG][2], middle[NG][2], widest = 0.f;
+  {
+    const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
+      step[g][0] = u0.x;
+      step[g][1] = u1.x;
+      middle[g][0] = fmaf(8.f, u0.x, u0.y);
+      middle[g][1] = fmaf(8.f, u1.x, u1.y);
     }
   }
   const int token = t0 + (r >> 1) + 4 * (r & 1);
-  bool rises = false;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    if (MASKED) {   // what lies behind the last key may be anything
+      step[g][0] = token < s.last ? step[g][0] : 0.f;
+      step[g][1] = token + 8 < s.last ? step[g][1] : 0.f;
+    }
+    widest = fmaxf(widest, fmaxf(step[g][0], step[g][1]));
+  }
+  bool rises = widest > s.cap;
+  float e[NT][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[nt][j] *= scale_log2;
-      if (MASKED && token + 8 * (j >> 1) >= s.seen[nt][j & 1]) x[nt][j] = -INFINITY;
-      rises = rises || x[nt][j] > s.top[nt][j & 1] + kLazy;
+      e[nt][j] = fmaf(x[nt][j], s.factor[nt][j & 1], -s.ref[nt][j & 1]);
+      if (MASKED && token + 8 * (j >> 1) >= s.seen[nt][j & 1]) e[nt][j] = -INFINITY;
+      rises = rises || e[nt][j] > s.limit;
     }
-  // ---- the reference of a row moves seldom: only when a score would make a weight larger than 2^8
+  // ---- the references move seldom: when a weight times a step could leave f16
   if (__any_sync(~0u, rises)) {
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
+    const float old = log2f(s.cap);
+    while (s.cap < widest) s.cap *= 2.f;
+    const float up = log2f(s.cap);
+    s.limit = kHead + kLazy - up;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = fmaxf(x[nt][j], x[nt][2 + j]);
+        const bool hide0 = MASKED && token >= s.seen[nt][j], hide1 = MASKED && token + 8 >= s.seen[nt][j];
+        float m = fmaxf(hide0 ? -INFINITY : x[nt][j] * s.factor[nt][j], hide1 ? -INFINITY : x[nt][2 + j] * s.factor[nt][j]);
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-        m = fmaxf(m, s.top[nt][j]);
-        const float fade = exp2f(s.top[nt][j] - m);
-        s.top[nt][j] = m;
+        // largest score so far, or what the reference stood for
+        const float ref = fmaxf(m, s.ref[nt][j] - old + kHead) + (up - kHead), fade = ex2(s.ref[nt][j] - ref);
+        s.ref[nt][j] = ref;
         s.sum[nt][j] *= fade;
 #pragma unroll
         for (int g = 0; g < NG; ++g) s.mid[nt][g][j] *= fade;
@@ -270,38 +307,37 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
           s.out[nt][i][j] *= fade;
           s.out[nt][i][2 + j] *= fade;
         }
+        e[nt][j] = hide0 ? -INFINITY : fmaf(x[nt][j], s.factor[nt][j], -ref);
+        e[nt][2 + j] = hide1 ? -INFINITY : fmaf(x[nt][2 + j], s.factor[nt][j], -ref);
       }
   }
-  float p[NT][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      p[nt][j] = exp2f(x[nt][j] - s.top[nt][j & 1]);
-      s.sum[nt][j & 1] += p[nt][j];
+      e[nt][j] = ex2(e[nt][j]);
+      s.sum[nt][j & 1] += e[nt][j];
     }
   // ---- outputs: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12); channels 32 b + 4 r + 0..3
   constexpr int kV = NB / 2;
   Words<kV> v[4];
   {
-    const int e = D == 128 ? r ^ ((c >> 1) << 2) : r;
+    const int u = D == 128 ? r ^ ((c >> 1) << 2) : r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = lds<kV>(slice + L::kHalf + (c + 4 * i) * L::kRow + e * NB * 2);
+    for (int i = 0; i < 4; ++i) v[i] = lds<kV>(slice + L::kHalf + (c + 4 * i) * L::kRow + u * NB * 2);
   }
-  const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
+  const uint32_t eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};   // -8 in the codes' units
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
-    const float m0 = fmaf(8.f, u0.x, u0.y), m1 = fmaf(8.f, u1.x, u1.y);
-    uint32_t hi[NT][2], lo[NT][2];
+    uint32_t w[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        y[j] = p[nt][j] * (j < 2 ? u0.x : u1.x);
-        const float z = p[nt][j] * (j < 2 ? m0 : m1);
-        if (MASKED) {   // what a row does not see may be anything, NaN too
+        y[j] = e[nt][j] * step[g][j >> 1];
+        const float z = e[nt][j] * middle[g][j >> 1];
+        if (MASKED) {   // nor does what a row does not see count, NaN or not
           const bool hidden = token + 8 * (j >> 1) >= s.seen[nt][j & 1];
           y[j] = hidden ? 0.f : y[j];
           s.mid[nt][g][j & 1] += hidden ? 0.f : z;
@@ -309,13 +345,8 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
           s.mid[nt][g][j & 1] += z;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t h = MmaOp<__nv_bfloat16>::pack(y[2 * i], y[2 * i + 1]);
-        const uint32_t l = MmaOp<__nv_bfloat16>::pack(y[2 * i] - __uint_as_float(h << 16), y[2 * i + 1] - __uint_as_float(h & 0xffff0000u));
-        hi[nt][i] = movmatrix(h);
-        lo[nt][i] = movmatrix(l);
-      }
+      w[nt][0] = movmatrix(MmaOp<__half>::pack(y[0], y[1]));
+      w[nt][1] = movmatrix(MmaOp<__half>::pack(y[2], y[3]));
     }
 #pragma unroll
     for (int i = 0; i < BG; ++i) {
@@ -324,11 +355,11 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
       const uint32_t v0 = __byte_perm(v[0].w[b >> 1], v[1].w[b >> 1], pick), v1 = __byte_perm(v[2].w[b >> 1], v[3].w[b >> 1], pick);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t a[4] = {centred(v0, 8 * h), centred(v0, 8 * h + 4), centred(v1, 8 * h), centred(v1, 8 * h + 4)};
+        const uint32_t a[4] = {codes(v0, 2 * h), codes(v0, 2 * h + 1), codes(v1, 2 * h), codes(v1, 2 * h + 1)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          MmaOp<__nv_bfloat16>::run(s.out[nt][2 * b + h], a, hi[nt]);
-          MmaOp<__nv_bfloat16>::run(s.out[nt][2 * b + h], a, lo[nt]);
+          MmaOp<__half>::run(s.out[nt][2 * b + h], eight, w[nt]);
+          MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[nt]);
         }
       }
     }
@@ -411,39 +442,58 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
           const int row = row0 + 8 * nt + r;
           const bool in = row < span.rows;
           const T* from = q + (int64_t)(head * group + row % group) * a.q_stride[1] + (int64_t)(row / group) * a.q_stride[2] + 8 * c;
-          float sums[NG];
+          // q as f16, times the power of two that brings the row's largest value to 2^14: exact for all that matters to a score.
+          // Channels 4 i + 1 and 4 i + 3 meet codes of 16 times the unit.
+          float2 e[NB][4];
+          float most = 0.f, sums[NG];
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             const uint4 w = in ? *reinterpret_cast<const uint4*>(from + 32 * i) : make_uint4(0, 0, 0, 0);
-            s.q[nt][i][0][0] = __byte_perm(w.x, w.z, 0x5410);
-            s.q[nt][i][0][1] = __byte_perm(w.x, w.z, 0x7632);
-            s.q[nt][i][1][0] = __byte_perm(w.y, w.w, 0x5410);
-            s.q[nt][i][1][1] = __byte_perm(w.y, w.w, 0x7632);
-            const float2 e0 = param<T>(w.x), e1 = param<T>(w.y), e2 = param<T>(w.z), e3 = param<T>(w.w);
-            const float sum = ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+            e[i][0] = param<T>(w.x), e[i][1] = param<T>(w.y), e[i][2] = param<T>(w.z), e[i][3] = param<T>(w.w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(e[i][k].x), fabsf(e[i][k].y)));
+          }
+          most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+          const int up = most > 0.f && isfinite(most) ? min(max(14 - ilogbf(most), -120), 120) : 0;
+          const float grow = __int_as_float((127 + up) << 23);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              s.q[nt][i][k][0] = MmaOp<__half>::pack(e[i][k].x * grow, e[i][k + 2].x * grow);
+              s.q[nt][i][k][1] = MmaOp<__half>::pack(e[i][k].y * (grow * 0.0625f), e[i][k + 2].y * (grow * 0.0625f));
+            }
+            const float sum = ((e[i][0].x + e[i][0].y) + (e[i][1].x + e[i][1].y)) + ((e[i][2].x + e[i][2].y) + (e[i][3].x + e[i][3].y));
             if (i % (G / 32) == 0) sums[i / (G / 32)] = sum;
             else sums[i / (G / 32)] += sum;
           }
+          float sum = 0.f;   // of group c
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             sums[g] += __shfl_xor_sync(~0u, sums[g], 1);
             sums[g] += __shfl_xor_sync(~0u, sums[g], 2);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              s.q_sum[nt][g][j] = __shfl_sync(~0u, sums[g], 4 * (2 * c + j));
-              s.mid[nt][g][j] = 0.f;
-            }
+            sum = c == g ? sums[g] * (grow * 2.44140625e-4f) : sum;
           }
+          const T high = Elem<T>::from_f(sum);
+          s.q_sum[nt][0] = MmaOp<T>::pack(0.f, Elem<T>::to_f(high));
+          s.q_sum[nt][1] = MmaOp<T>::pack(0.f, sum - Elem<T>::to_f(high));
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int col = row0 + 8 * nt + 2 * c + j;
+            s.factor[nt][j] = a.scale * 1.4426950408889634f * 16777216.f / __shfl_sync(~0u, grow, 4 * (2 * c + j));
             s.seen[nt][j] = col < span.rows ? length - count + col / group + 1 : 0;
-            s.top[nt][j] = kLowest;
+            s.ref[nt][j] = kLowest;
             s.sum[nt][j] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) s.mid[nt][g][j] = 0.f;
           }
 #pragma unroll
           for (int i = 0; i < 2 * NB; ++i) s.out[nt][i][0] = s.out[nt][i][1] = s.out[nt][i][2] = s.out[nt][i][3] = 0.f;
         }
+        s.cap = kLeastCap;
+        s.limit = kHead + kLazy + 24.f;
+        s.last = length;
         const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
         for (int i = 0; i < tiles; ++i) {
           const bool ok = !*abort_flag && tc::mbar_wait(full + stage, phase, abort_flag);
@@ -451,8 +501,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
             if (valid[stage] >> warp & 1) {
               const uint8_t* slice = smem + (stage * kWarps + warp) * L::kSlice;
               const int t0 = (tile0 + i) * kTile + 16 * warp;
-              if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0, a.scale * 1.4426950408889634f);
-              else take_slice<T, D, G, NT, true>(s, slice, t0, a.scale * 1.4426950408889634f);
+              if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0);
+              else take_slice<T, D, G, NT, true>(s, slice, t0);
             }
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(empty + stage);
@@ -470,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
             for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
             const int row = 8 * nt + 2 * c + j;
             if (r == 0) {
-              stats_s[(warp * kRows + row) * 2] = s.top[nt][j];
+              stats_s[(warp * kRows + row) * 2] = s.ref[nt][j];
               stats_s[(warp * kRows + row) * 2 + 1] = sum;
             }
 #pragma unroll
@@ -481,7 +531,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
 #pragma unroll
               for (int i = g * (G / 32); i < (g + 1) * (G / 32); ++i)
                 *reinterpret_cast<float4*>(mine + row * S::kOutRow + 32 * i + 4 * r) =
-                    make_float4(s.out[nt][2 * i][j] + mid, s.out[nt][2 * i][2 + j] + mid, s.out[nt][2 * i + 1][j] + mid, s.out[nt][2 * i + 1][2 + j] + mid);
+                    make_float4(fmaf(s.out[nt][2 * i][j], 16777216.f, mid), fmaf(s.out[nt][2 * i][2 + j], 1048576.f, mid),
+                                fmaf(s.out[nt][2 * i + 1][j], 16777216.f, mid), fmaf(s.out[nt][2 * i + 1][2 + j], 1048576.f, mid));
             }
           }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");

@@ -407,12 +407,13 @@ def attention(q, c, counts=None, scale=None):
     out, lse, tol, lse_tol = (torch.zeros(B, H, n, m, dtype=torch.float64, device=DEV) for m in (D, 1, D, 1))
     k, v = stands_for(c.k, c.group), stands_for(c.v, c.group)
     k_step = scales(c.k, c.group)[0].amax()
+    v_step = scales(c.v, c.group)[0].expand(*c.v.shape[:-1], -1, c.group).flatten(-2)
     for b in range(B):
         count = n if counts is None else counts[b]
         at = c.lengths[b] - count + torch.arange(n, device=DEV)
         at = torch.where(torch.arange(n, device=DEV) < count, at, -1)
         L = c.lengths[b]
-        kk, vv = (x[b, :, :L].repeat_interleave(H // Hk, 0) for x in (k, v))
+        kk, vv, step = (x[b, :, :L].repeat_interleave(H // Hk, 0) for x in (k, v, v_step))
         s = q[b].double() @ kk.transpose(-1, -2) * scale
         s = s.masked_fill(torch.arange(L, device=DEV) > at[:, None], -math.inf)
         m = s.amax(-1, keepdim=True) if L else torch.full((H, n, 1), -math.inf, dtype=torch.float64, device=DEV)
@@ -420,11 +421,13 @@ def attention(q, c, counts=None, scale=None):
         total = p.sum(-1, keepdim=True)
         p = p / total.clamp(min=1e-300)
         out[b], lse[b] = p @ vv, m + torch.log(total)
-        # a score is a sum over the channels of q times (128 + code) times a step, in 32 bits: 2^-21 of the terms' sum
-        off = abs(scale) * 2.0 ** -21 * (q[b].double().abs().sum(-1, keepdim=True) * 143 * k_step + (q[b].double().abs() @ kk.abs().amax(1, keepdim=True).transpose(-1, -2) if L else 0))
+        # a score is a sum over the channels of q times a code times a step, in 32 bits - 2^-21 of the terms' sum, where a code and what
+        # is taken off it again come to 143 at most - and of the sum of q, in two terms of 8 bits (2^-17), times a lowest value
+        size = q[b].double().abs().sum(-1, keepdim=True)
+        off = abs(scale) * size * (2.0 ** -21 * 143 * k_step + 2.0 ** -17 * (kk.abs().amax() if L else 0))
         off = off + 2.0 ** -22 * (1 + s.masked_fill(s == -math.inf, 0).abs().amax(-1, keepdim=True) if L else 1)
-        # weights to 2^-17 each (two terms of 8 bits), their products and sums in 32 bits
-        tol[b] = HALF[q.dtype] * 1.01 * out[b].abs() + (2 * off + 2.0 ** -16) * (p @ vv.abs()) + TINY[q.dtype]
+        # a weight times a step is rounded to f16, half a step of which is 2^-11, and meets a code less 8; products and sums in 32 bits
+        tol[b] = HALF[q.dtype] * 1.01 * out[b].abs() + (2 * off + 2.0 ** -16) * (p @ vv.abs()) + 2.0 ** -11 * (p @ (8 * step)) + TINY[q.dtype]
         lse_tol[b] = off + 2.0 ** -17 + 2.0 ** -23 * lse[b].abs().nan_to_num(0, 0, 0)
     return out, lse[..., 0], tol, lse_tol[..., 0]
 
