@@ -4,13 +4,13 @@
 //
 //   q . k  = sum_g  s (sum_d q_d n_d) + lo sum_d q_d                      sum over d in g: one product of q with the codes, on
 //                                                                         the tensor cores, scaled in 32 bits
-//   o_d    = sum_t (p_t s_t) (n_td - 8) + sum_t p_t (lo_t + 8 s_t)        the first sum is a product of codes with the weights
+//   o_d    = sum_t (p_t s_t) n_td + sum_t p_t lo_t                        the first sum is a product of codes with the weights
 //                                                                         times the step, the second a number per row and group
 //
 // Codes are exact in f16, and so is q times a power of two per row.  The weights times the step are rounded to f16 (11 bits, whatever the
-// tensors' type); the references of the rows keep them in its range.  Codes less 8 - a second product, with a constant - keep the
-// accumulators near zero: sums of codes from 0 to 15 grow with the context, the tensor cores cut their sums off, and what is cut
-// off adds up (0.1 % of an output of 131072 evenly weighted keys).
+// tensors' type); the references of the rows keep them in its range.  Half of a slice's tokens enter as hi - s (15 - n): that keeps the
+// accumulators near zero.  Sums of codes alone would grow with the context, the tensor cores cut their sums off, and what is cut off
+// adds up (0.1 % of an output of 131072 evenly weighted keys).
 //
 // Work: one tile is 64 tokens of one key head, for up to R = 8 NT query rows (new tokens x query heads of that key head).  All tiles of
 // all requests stand in one line, and every block takes an equal stretch of it, computed from the lengths on the device: requests of
@@ -39,7 +39,7 @@ struct AttnArgs {
   float* lse;
   int32_t* status;
   int64_t pages;
-  int batch, tokens, heads, kv_heads, width, page;
+  int batch, tokens, heads, kv_heads, group, width, page;   // group: query heads of a key head
   float scale;
   int least_tiles;     // a block takes at least so many
   int row_tiles;       // of a request that brings all `tokens`
@@ -66,7 +66,8 @@ constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has se
 // weight 2^-21 of the largest is still rounded to 11 bits.
 constexpr float kHead = 7.f, kLazy = 8.f;
 constexpr float kLeastCap = 5.9604644775390625e-8f;   // 2^-24
-constexpr float kSumScale = 2.44140625e-4f;           // 2^12 (sums of q are kept 2^-12 of q's operands) 2^-24 (codes)
+// Sums of q are kept in units of scores, 2^-24 of q's operands - in f16, whose numbers end there, 2^12 times that.
+template <typename T> constexpr float kSumScale = std::is_same<T, __half>::value ? 2.44140625e-4f : 1.f;
 
 template <int D, int G, int NT>
 struct Shape {
@@ -84,8 +85,7 @@ struct Shape {
 };
 
 struct Span {   // a request's place in the line of tiles
-  int rows, row_tiles, tiles;
-  int64_t work;
+  int rows, row_tiles, tiles, work;
 };
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_tile, int& length, int& count) {
   length = a.lengths[b];
@@ -97,65 +97,82 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_t
     count = min(max(count, 0), a.tokens);
   }
   Span s;
-  s.rows = count * (a.heads / a.kv_heads);
+  s.rows = count * a.group;
   s.row_tiles = (s.rows + rows_per_tile - 1) / rows_per_tile;
   s.tiles = (length + kTile - 1) / kTile;
-  s.work = (int64_t)s.tiles * s.row_tiles * a.kv_heads;
+  s.work = s.tiles * s.row_tiles * a.kv_heads;   // the entry point sees to it that the sum over all requests fits 32 bits
   return s;
 }
 
-// The block's stretch [first, last) of the line, and the request that `first` lies in with the place where that begins.
-struct Stretch {
-  int64_t first, last, base, work, blocks;
-  int request;
+// The line is shared out in stretches of `each` tiles, the first `longer` of them one longer.
+struct Shares {
+  int blocks, each, longer;
+  __device__ __forceinline__ Shares(int work, int most_blocks, int least) {
+    blocks = min(most_blocks, (work + least - 1) / least);
+    each = blocks ? work / blocks : 0;
+    longer = work - each * blocks;
+  }
+  __device__ __forceinline__ int first(int i) const { return i * each + min(i, longer); }
+  __device__ __forceinline__ int owner(int at) const {
+    const int edge = longer * (each + 1);
+    return at < edge ? at / (each + 1) : longer + (at - edge) / each;
+  }
 };
-__device__ __forceinline__ Stretch stretch_of(const AttnArgs& a, int rows_per_tile, int64_t* scan) {
+
+// The whole line's length, and the request that tile `first(block)` lies in with the place where that begins.  scan: 8 words.
+__device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int* scan, int& request, int& base, Shares& shares) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int length, count;
-  Stretch s;
-  int64_t mine = 0;
+  int length, count, mine = 0;
   for (int b = threadIdx.x; b < a.batch; b += kThreads) mine += span_of(a, b, rows_per_tile, length, count).work;
+  const int own0 = mine;   // of request threadIdx.x, where there are no more than threads
+  int sum = mine;
 #pragma unroll
-  for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(~0u, mine, d);
-  if (lane == 0) scan[warp] = mine;
+  for (int d = 1; d < 32; d *= 2) {
+    const int y = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += y;
+  }
+  if (lane == 31) scan[warp] = sum;
   __syncthreads();
-  s.work = 0;
+  int work = 0;
 #pragma unroll
-  for (int w = 0; w <= kWarps; ++w) s.work += scan[w];
-  s.blocks = min((int64_t)gridDim.x, (s.work + a.least_tiles - 1) / a.least_tiles);
-  s.first = s.last = s.base = 0;
-  s.request = 0;
-  if (blockIdx.x >= s.blocks) return s;
-  s.first = blockIdx.x * s.work / s.blocks;
-  s.last = (blockIdx.x + 1) * s.work / s.blocks;
-  if (a.batch == 1) return s;
-  // whose stretch it is: requests in rounds of one a thread
-  int64_t before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    const int64_t own = b < a.batch ? span_of(a, b, rows_per_tile, length, count).work : 0;
-    int64_t sum = own;
+  for (int w = 0; w <= kWarps; ++w) work += scan[w];
+  shares = Shares(work, gridDim.x, a.least_tiles);
+  request = base = 0;
+  if ((int)blockIdx.x >= shares.blocks || a.batch == 1) return work;
+  // whose tile it is: requests in rounds of one a thread
+  const int first = shares.first(blockIdx.x);
+  int before = 0;
+  for (int b0 = 0;; b0 += kThreads) {
+    int own = own0;
+    if (a.batch > kThreads) {
+      const int b = b0 + threadIdx.x;
+      own = b < a.batch ? span_of(a, b, rows_per_tile, length, count).work : 0;
+      sum = own;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int64_t y = __shfl_up_sync(~0u, sum, d);
-      if (lane >= d) sum += y;
+      for (int d = 1; d < 32; d *= 2) {
+        const int y = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += y;
+      }
+      __syncthreads();
+      if (lane == 31) scan[warp] = sum;
+      __syncthreads();
     }
-    __syncthreads();
-    if (lane == 31) scan[warp] = sum;
-    __syncthreads();
-    int64_t start = before + sum - own;
-    for (int w = 0; w < warp; ++w) start += scan[w];
-    for (int w = 0; w <= kWarps; ++w) before += scan[w];
-    if (s.first >= start && s.first < start + own) {
-      scan[6] = b;
+    int start = before + sum - own;
+#pragma unroll
+    for (int w = 0; w <= kWarps; ++w) {
+      start += w < warp ? scan[w] : 0;
+      before += scan[w];
+    }
+    if (first >= start && first < start + own) {
+      scan[6] = b0 + threadIdx.x;
       scan[7] = start;
     }
-    if (before > s.first) break;
+    if (before > first) break;
   }
   __syncthreads();
-  s.request = (int)scan[6];
-  s.base = scan[7];
-  return s;
+  request = scan[6];
+  base = scan[7];
+  return work;
 }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -166,10 +183,21 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // Codes of nibbles i and i + 4 as two f16 numbers: n 2^-24 for even i, n 2^-20 for odd ones.  (Subnormal numbers: a nibble is a number
 // where it stands, with no exponent to add and no offset to take off again.)
 __device__ __forceinline__ uint32_t codes(uint32_t w, int i) { return (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
+// The same of 15 - n.
+__device__ __forceinline__ uint32_t rest(uint32_t w, int i) { return ~(i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// The same product on an accumulator of zeros.
+template <typename T> __device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 // step and lowest value of a group
 template <typename T> __device__ __forceinline__ float2 param(uint32_t w);
@@ -217,10 +245,11 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
     const uint32_t a[4] = {w0, w1, w0, w1};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
-      MmaOp<T>::run(x[nt], a, s.q_sum[nt]);
+      mma_new<T>(x[nt], a, s.q_sum[nt]);
+      if constexpr (kSumScale<T> != 1.f) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[nt][j] *= kSumScale;
+        for (int j = 0; j < 4; ++j) x[nt][j] *= kSumScale<T>;
+      }
     }
   }
   {
@@ -230,15 +259,16 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
     for (int g = 0; g < NG; ++g) {
       float acc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
       for (int i = 0; i < BG; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const uint32_t w0 = k0.w[g * BG + i], w1 = k1.w[g * BG + i];
           const uint32_t a[4] = {codes(w0, 2 * k), codes(w1, 2 * k), codes(w0, 2 * k + 1), codes(w1, 2 * k + 1)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (i == 0 && k == 0) mma_new<__half>(acc[nt], a, s.q[nt][g * BG][0]);
+            else MmaOp<__half>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
+          }
         }
       const float s0 = param<T>(p0.w[g]).x, s1 = param<T>(p1.w[g]).x;
 #pragma unroll
@@ -247,27 +277,17 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
         for (int j = 0; j < 4; ++j) x[nt][j] = fmaf(j < 2 ? s0 : s1, acc[nt][j], x[nt][j]);
     }
   }
-  // ---- values' parameters
-  float step[NG][2], middle[NG][2], widest = 0.f;
-  {
-    const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
-      step[g][0] = u0.x;
-      step[g][1] = u1.x;
-      middle[g][0] = fmaf(8.f, u0.x, u0.y);
-      middle[g][1] = fmaf(8.f, u1.x, u1.y);
-    }
-  }
+  // ---- the largest step of the values: a lane looks at one group of its two rows
   const int token = t0 + (r >> 1) + 4 * (r & 1);
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
+  float widest;
+  {
+    const uint8_t* p = slice + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
+    float s0 = param<T>(lds<1>(p + r * NG * 4).w[0]).x, s1 = param<T>(lds<1>(p + (r + 8) * NG * 4).w[0]).x;
     if (MASKED) {   // what lies behind the last key may be anything
-      step[g][0] = token < s.last ? step[g][0] : 0.f;
-      step[g][1] = token + 8 < s.last ? step[g][1] : 0.f;
+      s0 = token < s.last ? s0 : 0.f;
+      s1 = token + 8 < s.last ? s1 : 0.f;
     }
-    widest = fmaxf(widest, fmaxf(step[g][0], step[g][1]));
+    widest = fmaxf(s0, s1);
   }
   bool rises = widest > s.cap;
   float e[NT][4];
@@ -326,17 +346,20 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = lds<kV>(slice + L::kHalf + (c + 4 * i) * L::kRow + u * NB * 2);
   }
-  const uint32_t eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};   // -8 in the codes' units
+  const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
+    const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
+    // a slice's first eight tokens: lo + s n; the others: hi - s (15 - n)
+    const float ends[2] = {u0.y, fmaf(15.f, u1.x, u1.y)};
     uint32_t w[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        y[j] = e[nt][j] * step[g][j >> 1];
-        const float z = e[nt][j] * middle[g][j >> 1];
+        y[j] = e[nt][j] * (j < 2 ? u0.x : -u1.x);
+        const float z = e[nt][j] * ends[j >> 1];
         if (MASKED) {   // nor does what a row does not see count, NaN or not
           const bool hidden = token + 8 * (j >> 1) >= s.seen[nt][j & 1];
           y[j] = hidden ? 0.f : y[j];
@@ -355,12 +378,9 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
       const uint32_t v0 = __byte_perm(v[0].w[b >> 1], v[1].w[b >> 1], pick), v1 = __byte_perm(v[2].w[b >> 1], v[3].w[b >> 1], pick);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t a[4] = {codes(v0, 2 * h), codes(v0, 2 * h + 1), codes(v1, 2 * h), codes(v1, 2 * h + 1)};
+        const uint32_t a[4] = {codes(v0, 2 * h), codes(v0, 2 * h + 1), rest(v1, 2 * h), rest(v1, 2 * h + 1)};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          MmaOp<__half>::run(s.out[nt][2 * b + h], eight, w[nt]);
-          MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[nt]);
-        }
+        for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[nt]);
       }
     }
   }
@@ -377,8 +397,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
   float* stats_s = reinterpret_cast<float*>(smem + S::kStats);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* empty = full + kStages;
-  int64_t* scan = reinterpret_cast<int64_t*>(smem + S::kMore);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(scan + 8);
+  int* scan = reinterpret_cast<int*>(smem + S::kMore);
+  volatile int* abort_flag = scan + 8;
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(scan + 9);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -389,22 +409,25 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
     tc::fence_mbar_init();
     *abort_flag = 0;
   }
-  const Stretch line = stretch_of(a, kRows, scan);
+  asm volatile("griddepcontrol.launch_dependents;");
+  int request, base;
+  Shares shares(0, 0, 1);
+  line_of(a, kRows, scan, request, base, shares);
   __syncthreads();
-  if (line.first >= line.last) return;
-  const int group = a.heads / a.kv_heads, slices_per_page = a.page / 16;
+  if ((int)blockIdx.x >= shares.blocks) return;
+  const int group = a.group, slices_per_page = a.page / 16;
   int stage = 0;
   uint32_t phase = 0;
-  int64_t at = line.first, base = line.base;
-  for (int b = line.request; at < line.last; ++b) {
+  int at = shares.first(blockIdx.x);
+  const int last = shares.first(blockIdx.x + 1);
+  for (int b = request; at < last; ++b) {
     int length, count;
     const Span span = span_of(a, b, kRows, length, count);
-    const int64_t end = base + span.work;
-    while (at < line.last && at < end) {
-      const int64_t unit = (at - base) / span.tiles;
-      const int tile0 = (int)(at - base - unit * span.tiles);
-      const int tiles = (int)min((int64_t)(span.tiles - tile0), line.last - at);
-      const int head = (int)(unit / span.row_tiles), row0 = (int)(unit - (int64_t)head * span.row_tiles) * kRows;
+    const int end = base + span.work;
+    while (at < last && at < end) {
+      const int unit = (at - base) / span.tiles, tile0 = at - base - unit * span.tiles;
+      const int tiles = min(span.tiles - tile0, last - at);
+      const int head = unit / span.row_tiles, row0 = (unit - head * span.row_tiles) * kRows;
       if (warp == kWarps) {
         // ------------------------------------------------------------ copies: a lane a slice, eight tiles' page numbers at a time
         const int slices = (length + 15) / 16, first_slice = tile0 * kWarps, last_slice = min(slices, (tile0 + tiles) * kWarps);
@@ -473,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
           for (int g = 0; g < NG; ++g) {
             sums[g] += __shfl_xor_sync(~0u, sums[g], 1);
             sums[g] += __shfl_xor_sync(~0u, sums[g], 2);
-            sum = c == g ? sums[g] * (grow * 2.44140625e-4f) : sum;
+            sum = c == g ? sums[g] * (grow * 5.9604644775390625e-8f / kSumScale<T>) : sum;
           }
           const T high = Elem<T>::from_f(sum);
           s.q_sum[nt][0] = MmaOp<T>::pack(0.f, Elem<T>::to_f(high));
@@ -495,12 +518,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
         s.limit = kHead + kLazy + 24.f;
         s.last = length;
         const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
-        for (int i = 0; i < tiles; ++i) {
-          const bool ok = !*abort_flag && tc::mbar_wait(full + stage, phase, abort_flag);
-          if (__all_sync(~0u, ok)) {
+        int t0 = tile0 * kTile + 16 * warp;
+        for (int i = 0; i < tiles; ++i, t0 += kTile) {
+          bool ok = __all_sync(~0u, tc::mbar_try_wait(full + stage, phase));
+          if (!ok) ok = __all_sync(~0u, tc::mbar_wait(full + stage, phase, abort_flag));
+          if (ok) {
             if (valid[stage] >> warp & 1) {
               const uint8_t* slice = smem + (stage * kWarps + warp) * L::kSlice;
-              const int t0 = (tile0 + i) * kTile + 16 * warp;
               if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0);
               else take_slice<T, D, G, NT, true>(s, slice, t0);
             }
@@ -564,9 +588,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
         }
         if (starts && threadIdx.x == 0) {
           // whose parts the unit is made of: from this block to the one that holds its last tile
-          const int64_t last = at + span.tiles - 1;
-          a.owners[((int64_t)b * a.kv_heads + head) * a.row_tiles + row0 / kRows] =
-              make_int2((int)blockIdx.x, (int)(((last + 1) * line.blocks - 1) / line.work));
+          a.owners[((int64_t)b * a.kv_heads + head) * a.row_tiles + row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(at + span.tiles - 1));
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
       }
@@ -585,55 +607,68 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
   }
 }
 
-// Rows whose tiles lay in several blocks, from their parts in order; rows of nothing.  A block a row, its warps take every fourth part.
+// Rows whose tiles lay in several blocks, from their parts; rows of nothing.  A block a row: its lane groups (a group reads a part's row of
+// channels) take every kGroupsOf-th part, four loads in flight each, and are joined in order.  Launched before the first kernel's
+// blocks are done and held here until they are: what a launch costs is spent while they work.
+constexpr int kJoinThreads = 256;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ AttnArgs a, int rows_per_tile) {
-  __shared__ float out_s[4][D], stats_s[4][2];
-  const int group = a.heads / a.kv_heads, i = blockIdx.x, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.y;
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const __grid_constant__ AttnArgs a, int rows_per_tile) {
+  constexpr int kLanes = D / 4, kGroupsOf = kJoinThreads / kLanes, kInFlight = 4;
+  __shared__ float4 out_s[kGroupsOf][kLanes];
+  __shared__ float2 stats_s[kGroupsOf];
+  const int group = a.group, i = blockIdx.x, head = blockIdx.y, b = blockIdx.z, own = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   int length, count;
   const Span span = span_of(a, b, rows_per_tile, length, count);
-  const int row = i * group + head % group;
+  const int row = i * group + head % group, r = row % rows_per_tile;
   int2 owners = make_int2(0, -1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (i < count && span.tiles) {
     owners = a.owners[((int64_t)b * a.kv_heads + head / group) * a.row_tiles + row / rows_per_tile];
     if (owners.x == owners.y) return;
   }
   const int64_t size = (int64_t)rows_per_tile * (D + 2);
-  const int r = row % rows_per_tile;
-  constexpr int kLanes = D / 4;
   float top = kLowest, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = owners.x + warp; k <= owners.y; k += 4) {
-    const float* part = a.parts + ((int64_t)k * 2 + (k == owners.x)) * size;
-    const float2 st = *reinterpret_cast<const float2*>(part + rows_per_tile * D + 2 * r);
-    const float4 y = lane < kLanes ? *reinterpret_cast<const float4*>(part + r * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-    const float m = fmaxf(top, st.x), f0 = exp2f(top - m), f1 = exp2f(st.x - m);
-    top = m;
-    sum = sum * f0 + st.y * f1;
-    o.x = o.x * f0 + y.x * f1;
-    o.y = o.y * f0 + y.y * f1;
-    o.z = o.z * f0 + y.z * f1;
-    o.w = o.w * f0 + y.w * f1;
+  for (int k0 = owners.x + own; k0 <= owners.y; k0 += kInFlight * kGroupsOf) {
+    float4 y[kInFlight];
+    float2 st[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int k = k0 + u * kGroupsOf;
+      const float* part = a.parts + ((int64_t)min(k, owners.y) * 2 + (k == owners.x)) * size;
+      st[u] = k <= owners.y ? *reinterpret_cast<const float2*>(part + rows_per_tile * D + 2 * r) : make_float2(kLowest, 0.f);
+      y[u] = k <= owners.y ? *reinterpret_cast<const float4*>(part + r * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const float m = fmaxf(top, st[u].x), f0 = exp2f(top - m), f1 = exp2f(st[u].x - m);
+      top = m;
+      sum = sum * f0 + st[u].y * f1;
+      o.x = o.x * f0 + y[u].x * f1;
+      o.y = o.y * f0 + y[u].y * f1;
+      o.z = o.z * f0 + y[u].z * f1;
+      o.w = o.w * f0 + y[u].w * f1;
+    }
   }
-  if (lane < kLanes) *reinterpret_cast<float4*>(&out_s[warp][4 * lane]) = o;
-  if (lane == 0) stats_s[warp][0] = top, stats_s[warp][1] = sum;
+  out_s[own][lane] = o;
+  if (lane == 0) stats_s[own] = make_float2(top, sum);
   __syncthreads();
   if (threadIdx.x < kLanes) {
-    const int d = 4 * threadIdx.x;
-    top = fmaxf(fmaxf(stats_s[0][0], stats_s[1][0]), fmaxf(stats_s[2][0], stats_s[3][0]));
+#pragma unroll
+    for (int w = 1; w < kGroupsOf; ++w) top = fmaxf(top, stats_s[w].x);
     sum = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(stats_s[w][0] - top);
-      sum += f * stats_s[w][1];
-      o.x += f * out_s[w][d];
-      o.y += f * out_s[w][d + 1];
-      o.z += f * out_s[w][d + 2];
-      o.w += f * out_s[w][d + 3];
+    for (int w = 0; w < kGroupsOf; ++w) {
+      const float f = exp2f(stats_s[w].x - top);
+      const float4 y = out_s[w][lane];
+      sum += f * stats_s[w].y;
+      o.x += f * y.x;
+      o.y += f * y.y;
+      o.z += f * y.z;
+      o.w += f * y.w;
     }
-    write_row<T>(a, b, head, i, d, o, top, sum);
+    write_row<T>(a, b, head, i, 4 * lane, o, top, sum);
   }
 }
 
@@ -671,8 +706,17 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   kernel<<<blocks, kThreads, S::kBytes, st>>>(a);
   PSA_CHECK_LAUNCH("psa_kv4_attention");
   const dim3 grid((unsigned)a.tokens, (unsigned)a.heads, (unsigned)a.batch);
-  kv4_join_kernel<T, D><<<grid, 128, 0, st>>>(a, S::kRows);
-  PSA_CHECK_LAUNCH("psa_kv4_attention");
+  cudaLaunchConfig_t how = {};
+  how.gridDim = grid;
+  how.blockDim = dim3(kJoinThreads);
+  how.stream = st;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  how.attrs = &early;
+  how.numAttrs = 1;
+  const cudaError_t rc = cudaLaunchKernelEx(&how, kv4_join_kernel<T, D>, a, (int)S::kRows);
+  PSA_REQUIRE(rc == cudaSuccess, PSA_ERR_CUDA, "psa_kv4_attention: launch failed: %s", cudaGetErrorString(rc));
   return PSA_OK;
 }
 
@@ -725,12 +769,16 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   a.tokens = (int)tokens;
   a.heads = heads;
   a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
   a.width = (int)width;
   a.page = page_size;
   a.scale = sm_scale;
   const int64_t rows = tokens * (heads / kv_heads);
   a.least_tiles = 2;
   a.row_tiles = (int)cdiv64(rows, rows_per_tile(rows));
+  PSA_REQUIRE(rows < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_kv4_attention: %lld rows a key head", (long long)rows);
+  PSA_REQUIRE((double)batch * cdiv64(width * page_size, kTile) * a.row_tiles * kv_heads < 2147483648.0, PSA_ERR_UNSUPPORTED,
+              "psa_kv4_attention: %lld requests of up to %lld tokens: more than 2^31 tiles", (long long)batch, (long long)(width * page_size));
   a.owners = static_cast<int2*>(scratch);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + owners_bytes(batch, kv_heads, a.row_tiles));
   if (rows_per_tile(rows) == 8) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, return (launch<T, D, G, 1>(a, (cudaStream_t)stream)));
