@@ -25,116 +25,125 @@ struct CacheArgs {
 __device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
 __device__ __forceinline__ __nv_bfloat16 cut_off(float x, __nv_bfloat16) { return __float2bfloat16_rz(x); }
 
-template <int D, int G>
-__device__ __forceinline__ uint8_t* slice_of(const CacheArgs& a, int slot, int head) {
-  const int page = slot / a.page, at = slot - page * a.page;
-  return a.data + (((int64_t)page * a.heads + head) * (a.page / 16) + at / 16) * Kv4<D, G>::kSlice;
-}
+constexpr int kHeads = 4;   // heads of a token that a thread takes, their loads in flight together
 
-// A thread holds 8 neighbouring channels of a row of keys (z = 0) or values (z = 1), D/8 threads a row.  Rows run over tokens, then
-// heads, so that a block reads and writes near places whichever way the tensors lie.
+// D/8 threads hold a row, 8 neighbouring channels each, and take kHeads heads of its token; blockIdx.z: keys or values.
 template <int D, int G>
-__device__ __forceinline__ bool place(const CacheArgs& a, int& u, int& head, int64_t& b, int64_t& t, int& slot) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  u = (int)(i % (D / 8));
-  int64_t row = i / (D / 8);
-  head = (int)(row % a.heads);
-  row /= a.heads;
-  if (row >= a.batch * a.tokens) return false;
-  b = row / a.tokens;
-  t = row - b * a.tokens;
-  slot = a.slots[row];
-  return true;
+struct Place {
+  int u, head0, heads, slot;
+  uint32_t row, b, t;
+  uint8_t* slice;        // of head0; further heads lie `apart` bytes on
+  int64_t apart;
+  bool in, good;
+  __device__ __forceinline__ Place(const CacheArgs& a) {
+    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+    u = i % (D / 8);
+    row = blockIdx.x * (256 / (D / 8)) + threadIdx.x / (D / 8);
+    in = row < (uint32_t)a.batch * (uint32_t)a.tokens;
+    head0 = blockIdx.y * kHeads;
+    heads = min(kHeads, a.heads - head0);
+    if (!in) row = 0;
+    b = row / (uint32_t)a.tokens;
+    t = row - b * (uint32_t)a.tokens;
+    slot = a.slots[row];
+    good = in && slot >= 0 && slot < a.slots_total;
+    if (in && !good && slot != -1) *a.status = PSA_ERR_ARG;
+    const int page = good ? slot / a.page : 0, at = good ? slot - page * a.page : 0, slices = a.page / 16;
+    apart = (int64_t)slices * Kv4<D, G>::kSlice;
+    slice = a.data + ((int64_t)page * a.heads + head0) * apart + at / 16 * Kv4<D, G>::kSlice;
+  }
+};
+
+// Values lie in 16-bit units, and the unit that follows one in memory is of the channels 32 further on: the thread four lanes up holds
+// it.  The two swap a unit each, so that both write (or read) 32 bits.  Even 32-channel blocks keep the lower unit's place.
+__device__ __forceinline__ uint32_t swap_units(uint32_t codes, bool odd) {
+  const uint32_t other = __shfl_xor_sync(~0u, odd ? codes & 0xffffu : codes >> 16, 4);
+  return odd ? other | (codes & 0xffff0000u) : (codes & 0xffffu) | other << 16;
 }
 
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
   using L = Kv4<D, G>;
-  const int z = blockIdx.y;
-  int u, head, slot;
-  int64_t b, t;
-  const bool in = place<D, G>(a, u, head, b, t, slot);
-  const bool write = in && slot >= 0 && slot < a.slots_total;
-  if (in && !write && slot != -1) *a.status = PSA_ERR_ARG;
-  float x[8];
-  if (write) {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.src[z]) + b * a.stride[z][0] + head * a.stride[z][1] +
-                                                    t * a.stride[z][2] + u * 8);
-    const T* e = reinterpret_cast<const T*>(&w);
+  const int z = blockIdx.z;
+  const Place<D, G> at(a);
+  uint4 w[kHeads];
+  const T* src = static_cast<const T*>(a.src[z]) + at.b * a.stride[z][0] + at.head0 * a.stride[z][1] + at.t * a.stride[z][2] + at.u * 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = Elem<T>::to_f(e[j]);
-  } else {
+  for (int h = 0; h < kHeads; ++h)
+    w[h] = at.good && h < at.heads ? __ldg(reinterpret_cast<const uint4*>(src + h * a.stride[z][1])) : make_uint4(0, 0, 0, 0);
+  const int r = at.slot & 15, g = at.u * 8 / G;
+  const bool odd = at.u >> 2 & 1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-  }
-  float lo = x[0], hi = x[0];
-  bool finite = true;
+  for (int h = 0; h < kHeads; ++h) {
+    const T* e = reinterpret_cast<const T*>(&w[h]);
+    float x[8], lo, hi;
+    bool finite = true;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    lo = fminf(lo, x[j]);
-    hi = fmaxf(hi, x[j]);
-    finite = finite && isfinite(x[j]);
-  }
+    for (int j = 0; j < 8; ++j) {
+      x[j] = Elem<T>::to_f(e[j]);
+      lo = j ? fminf(lo, x[j]) : x[j];
+      hi = j ? fmaxf(hi, x[j]) : x[j];
+      finite = finite && isfinite(x[j]);
+    }
+    // one that is not finite takes the whole group along: the range of such a group is not finite either
+    lo = finite ? lo : -INFINITY;
+    hi = finite ? hi : INFINITY;
 #pragma unroll
-  for (int d = 1; d < G / 8; d *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
-    finite = __shfl_xor_sync(~0u, (int)finite, d) && finite;
-  }
-  if (!write) return;
-  const float wide = (hi - lo) / 15.f;
-  T step = cut_off(wide, T());
-  T lowest = Elem<T>::from_f(lo);
-  const float s = Elem<T>::to_f(step);
-  uint32_t codes = 0;
-  if (!finite || !isfinite(wide)) {
-    step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));
-  } else if (s > 0.f) {
+    for (int d = 1; d < G / 8; d *= 2) {
+      lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
+      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
+    }
+    const float wide = (hi - lo) / 15.f;
+    T step = cut_off(wide, T());
+    T lowest = Elem<T>::from_f(lo);
+    const float s = Elem<T>::to_f(step);
+    uint32_t codes = 0;
+    if (!isfinite(wide)) {
+      step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));
+    } else if (s > 0.f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) codes |= (uint32_t)fminf(rintf((x[j] - lo) / s), 15.f) << (4 * j);
-  }
-  uint8_t* slice = slice_of<D, G>(a, slot, head);
-  const int r = slot % 16, g = u * 8 / G;
-  if (z == 0) {
-    *reinterpret_cast<uint32_t*>(slice + L::k_word(r, u * 8)) = codes;
-  } else {
-    *reinterpret_cast<uint16_t*>(slice + L::v_unit(r, u * 8)) = (uint16_t)codes;
-    *reinterpret_cast<uint16_t*>(slice + L::v_unit(r, u * 8 + 4)) = (uint16_t)(codes >> 16);
-  }
-  if (u * 8 % G == 0) {
-    T* p = reinterpret_cast<T*>(slice + (z == 0 ? L::k_param(r, g) : L::v_param(r, g)));
-    p[0] = step;
-    p[1] = lowest;
+      for (int j = 0; j < 8; ++j) codes |= (uint32_t)fminf(rintf((x[j] - lo) / s), 15.f) << (4 * j);
+    }
+    if (z) codes = swap_units(codes, odd);
+    if (!at.good || h >= at.heads) continue;
+    uint8_t* slice = at.slice + h * at.apart;
+    // after the swap an even block's thread has the units of channels 8 u and 8 u + 32, an odd one's those of 8 u - 28 and 8 u + 4
+    const int place = z ? L::v_unit(r, odd ? at.u * 8 - 28 : at.u * 8) : L::k_word(r, at.u * 8);
+    *reinterpret_cast<uint32_t*>(slice + place) = codes;
+    if (at.u * 8 % G == 0) {
+      T pair[2] = {step, lowest};
+      *reinterpret_cast<uint32_t*>(slice + (z ? L::v_param(r, g) : L::k_param(r, g))) = *reinterpret_cast<const uint32_t*>(pair);
+    }
   }
 }
 
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const CacheArgs a) {
   using L = Kv4<D, G>;
-  const int z = blockIdx.y;
-  int u, head, slot;
-  int64_t b, t;
-  if (!place<D, G>(a, u, head, b, t, slot)) return;
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (slot >= 0 && slot < a.slots_total) {
-    const uint8_t* slice = slice_of<D, G>(a, slot, head);
-    const int r = slot % 16, g = u * 8 / G;
-    uint32_t codes;
-    if (z == 0) {
-      codes = *reinterpret_cast<const uint32_t*>(slice + L::k_word(r, u * 8));
-    } else {
-      codes = *reinterpret_cast<const uint16_t*>(slice + L::v_unit(r, u * 8)) |
-              (uint32_t)*reinterpret_cast<const uint16_t*>(slice + L::v_unit(r, u * 8 + 4)) << 16;
-    }
-    const T* p = reinterpret_cast<const T*>(slice + (z == 0 ? L::k_param(r, g) : L::v_param(r, g)));
+  const int z = blockIdx.z;
+  const Place<D, G> at(a);
+  const int r = at.slot & 15, g = at.u * 8 / G;
+  const bool odd = at.u >> 2 & 1;
+  uint32_t codes[kHeads], pair[kHeads];
+  const int place = z ? L::v_unit(r, odd ? at.u * 8 - 28 : at.u * 8) : L::k_word(r, at.u * 8), params = z ? L::v_param(r, g) : L::k_param(r, g);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const bool load = at.good && h < at.heads;
+    codes[h] = load ? *reinterpret_cast<const uint32_t*>(at.slice + h * at.apart + place) : 0u;
+    pair[h] = load ? *reinterpret_cast<const uint32_t*>(at.slice + h * at.apart + params) : 0u;
+  }
+  T* dst = static_cast<T*>(a.dst[z]) + at.b * a.stride[z][0] + at.head0 * a.stride[z][1] + at.t * a.stride[z][2] + at.u * 8;
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const uint32_t n = z ? swap_units(codes[h], odd) : codes[h];
+    const T* p = reinterpret_cast<const T*>(&pair[h]);
     const float step = Elem<T>::to_f(p[0]), lowest = Elem<T>::to_f(p[1]);
+    uint4 w;
     T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = Elem<T>::from_f(fmaf((float)(codes >> (4 * j) & 15), step, lowest));
-  } else if (slot != -1) {
-    *a.status = PSA_ERR_ARG;
+    for (int j = 0; j < 8; ++j) e[j] = Elem<T>::from_f(fmaf((float)(n >> (4 * j) & 15), step, lowest));
+    if (at.in && h < at.heads) *reinterpret_cast<uint4*>(dst + h * a.stride[z][1]) = w;
   }
-  *reinterpret_cast<uint4*>(static_cast<T*>(a.dst[z]) + b * a.stride[z][0] + head * a.stride[z][1] + t * a.stride[z][2] + u * 8) = w;
 }
 
 int check(const char* what, const void* data, const void* k, const void* v, const int64_t* strides, const int32_t* slots, int64_t pages,
@@ -144,8 +153,8 @@ int check(const char* what, const void* data, const void* k, const void* v, cons
   PSA_REQUIRE(kv4_sizes_ok(head_dim, group), PSA_ERR_ARG, "%s: head_dim=%d, group=%d (64 or 128, groups of 32, 64 or 128 within it)", what, head_dim, group);
   PSA_REQUIRE(page > 0 && page % 16 == 0 && pages > 0 && pages < ((int64_t)1 << 31) / page && heads > 0 && heads < 65536, PSA_ERR_ARG,
               "%s: %lld pages of %d tokens, %d heads", what, (long long)pages, page, heads);
-  PSA_REQUIRE(batch > 0 && tokens > 0 && batch * tokens < ((int64_t)1 << 31) && cdiv64(batch * tokens * heads * (head_dim / 8), 256) < ((int64_t)1 << 31),
-              PSA_ERR_ARG, "%s: bad shape", what);
+  PSA_REQUIRE(batch > 0 && tokens > 0 && batch < ((int64_t)1 << 31) && tokens < ((int64_t)1 << 31) && batch * tokens < ((int64_t)1 << 31), PSA_ERR_ARG,
+              "%s: bad shape", what);
   PSA_REQUIRE((((uintptr_t)data | (uintptr_t)k | (uintptr_t)v) & 15) == 0, PSA_ERR_ARG, "%s: operands must be 16-byte aligned", what);
   for (int i = 0; i < 6; ++i) PSA_REQUIRE(strides[i] % 8 == 0, PSA_ERR_ARG, "%s: strides must be multiples of 8 elements", what);
   return PSA_OK;
@@ -180,7 +189,7 @@ extern "C" int psa_kv4_append(void* data, const void* k, const void* v, const in
   CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, batch, tokens, status);
   a.src[0] = k;
   a.src[1] = v;
-  const dim3 grid((unsigned)cdiv64(batch * tokens * kv_heads * (head_dim / 8), 256), 2);
+  const dim3 grid((unsigned)cdiv64(batch * tokens, 256 / (head_dim / 8)), (unsigned)cdiv64(kv_heads, kHeads), 2);
   PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_append_kernel<T, D, G><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
   PSA_CHECK_LAUNCH("psa_kv4_append");
   return PSA_OK;
@@ -193,7 +202,7 @@ extern "C" int psa_kv4_read(const void* data, void* k, void* v, const int64_t* s
   CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, batch, tokens, status);
   a.dst[0] = k;
   a.dst[1] = v;
-  const dim3 grid((unsigned)cdiv64(batch * tokens * kv_heads * (head_dim / 8), 256), 2);
+  const dim3 grid((unsigned)cdiv64(batch * tokens, 256 / (head_dim / 8)), (unsigned)cdiv64(kv_heads, kHeads), 2);
   PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_read_kernel<T, D, G><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
   PSA_CHECK_LAUNCH("psa_kv4_read");
   return PSA_OK;

@@ -12,6 +12,7 @@ namespace psa {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int64_t kFewEntries = 1 << 15;   // slots that one block writes about as fast as a second launch starts
 
 // Of each request, for the second kernel: pages held before, pages given, place of the first given page from the top of the
 // pool, tokens given, length before.
@@ -19,7 +20,8 @@ struct Grant {
   int32_t held, given, first, tokens, length;
 };
 
-__device__ __forceinline__ int block_scan(int x, int* warp_sums) {   // inclusive, over kPlanThreads
+template <int THREADS = kPlanThreads>
+__device__ __forceinline__ int block_scan(int x, int* warp_sums) {   // inclusive; warp_sums: 32 words, the last one gets the whole sum
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -29,7 +31,7 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums) {   // inclusiv
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int s = warp_sums[lane];
+    int s = lane < THREADS / 32 ? warp_sums[lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int y = __shfl_up_sync(~0u, s, d);
@@ -43,67 +45,129 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums) {   // inclusiv
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int page) { return (int)((tokens + page - 1) / page); }
 
-// Who gets what, and the new lengths.  One block, requests in rounds of one a thread.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* lengths, const int32_t* counts, const int32_t* free_in,
-                                                            int32_t* lengths_out, int32_t* free_out, Grant* grants, int32_t* free_before,
-                                                            int requests, int width, int pool_size, int page, int tokens,
-                                                            int32_t* status) {
-  __shared__ int warp_sums[32];
-  __shared__ int taken;
-  const int available = min(max(free_in[0], 0), pool_size);
-  if (threadIdx.x == 0) taken = 0;
-  int before = 0;   // needs of the rounds so far
-  for (int b0 = 0; b0 < requests; b0 += kPlanThreads) {
-    const int b = b0 + threadIdx.x;
-    int length = 0, count = 0, held = 0, need = 0;
-    bool bad = false;
-    if (b < requests) {
-      length = lengths[b];
-      count = counts[b];
-      bad = length < 0 || length > (int64_t)width * page || count < 0 || count > tokens || (int64_t)length + count > (int64_t)width * page;
-      if (bad) count = 0;
-      held = pages_of(min(max(length, 0), width * page), page);
-      need = bad ? 0 : pages_of((int64_t)length + count, page) - held;
+struct PlanArgs {
+  const int32_t *table, *lengths, *counts, *pool, *free_in;
+  int32_t *table_out, *lengths_out, *free_out, *slots, *status;
+  Grant* grants;
+  int32_t* free_before;
+  int requests, width, pool_size, page, tokens;
+};
+
+// What a request holds, wants and has a right to want.
+struct Want {
+  int length, count, held, need;
+  bool bad;
+};
+__device__ __forceinline__ Want want_of(const PlanArgs& a, int b) {
+  Want w;
+  w.length = a.lengths[b];
+  w.count = a.counts[b];
+  const int64_t most = (int64_t)a.width * a.page;
+  w.bad = w.length < 0 || w.length > most || w.count < 0 || w.count > a.tokens || (int64_t)w.length + w.count > most;
+  if (w.bad) w.count = 0;
+  w.held = pages_of(min(max(w.length, 0), (int)most), a.page);
+  w.need = w.bad ? 0 : pages_of((int64_t)w.length + w.count, a.page) - w.held;
+  return w;
+}
+__device__ __forceinline__ Grant grant_of(const PlanArgs& a, const Want& w, int total, int available) {
+  const bool served = w.need == 0 || total <= available;
+  if (!served || w.bad) *a.status = PSA_ERR_ARG;
+  return {w.held, served ? w.need : 0, total - w.need, served ? w.count : 0, w.length};
+}
+
+// Entries [from, to) of a request's row of the table and of its slots.
+__device__ __forceinline__ void fill_row(const PlanArgs& a, int b, const Grant& g, int available, int from, int to, int step) {
+  const int top = available - 1 - g.first;
+  const int64_t row = (int64_t)b * a.width;
+  for (int j = from; j < to; j += step) {
+    if (j < a.width) {
+      const bool fresh = j >= g.held && j < g.held + g.given;
+      if (fresh || a.table_out != a.table) a.table_out[row + j] = fresh ? a.pool[top - (j - g.held)] : a.table[row + j];
     }
-    const int total = before + block_scan(need, warp_sums);
-    if (b < requests) {
-      const bool served = need == 0 || total <= available;
-      if (!served || bad) *status = PSA_ERR_ARG;
-      if (!served) count = 0;
-      else if (need) atomicMax(&taken, total);
-      grants[b] = {held, served ? need : 0, total - need, count, length};
-      lengths_out[b] = length + count;
+    if (j < a.tokens) {
+      int slot = -1;
+      if (j < g.tokens) {
+        const int at = g.length + j, k = at / a.page;
+        const int p = k < g.held ? a.table[row + k] : a.pool[top - (k - g.held)];
+        if (p >= 0 && p < 0x7fffffff / a.page) slot = p * a.page + (at - k * a.page);
+      }
+      a.slots[(int64_t)b * a.tokens + j] = slot;
     }
-    before += warp_sums[31];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    *free_before = available;
-    *free_out = available - taken;
   }
 }
 
-// The tables' rows and the slots of the new tokens.
-__global__ void __launch_bounds__(256) fill_kernel(const int32_t* table, const int32_t* pool, const Grant* grants, const int32_t* free_before,
-                                                   int32_t* table_out, int32_t* slots, int width, int page, int tokens) {
-  const int b = blockIdx.y;
-  const Grant g = grants[b];
-  const int top = *free_before - 1 - g.first;
-  for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < max(width, tokens); j += gridDim.x * blockDim.x) {
-    if (j < width) {
-      const bool fresh = j >= g.held && j < g.held + g.given;
-      if (fresh || table_out != table) table_out[(int64_t)b * width + j] = fresh ? pool[top - (j - g.held)] : table[(int64_t)b * width + j];
+// Outputs beside the inputs, up to kPlanThreads requests: a block fills a stretch of a request's row and sums the needs of the requests
+// before it for itself - a few hundred numbers that all blocks find in L2 - which spares a launch that would do nothing else.
+constexpr int kRowThreads = 256, kRowEntries = 2048;
+__global__ void __launch_bounds__(kRowThreads) plan_rows_kernel(const PlanArgs a) {
+  __shared__ int warp_sums[32], taken;
+  const int b = blockIdx.y, available = min(max(a.free_in[0], 0), a.pool_size);
+  int before = 0;
+  for (int i = threadIdx.x; i < b; i += kRowThreads) before += want_of(a, i).need;
+  block_scan<kRowThreads>(before, warp_sums);
+  const Want w = want_of(a, b);
+  const Grant g = grant_of(a, w, warp_sums[31] + w.need, available);
+  fill_row(a, b, g, available, blockIdx.x * kRowEntries + threadIdx.x, min((int)(blockIdx.x + 1) * kRowEntries, max(a.width, a.tokens)), kRowThreads);
+  if (blockIdx.x) return;
+  if (threadIdx.x == 0) a.lengths_out[b] = g.length + g.tokens;
+  if (b) return;
+  // pages taken: the largest running total that fits
+  if (threadIdx.x == 0) taken = 0;
+  int total = 0;
+  for (int b0 = 0; b0 < a.requests; b0 += kRowThreads) {
+    const int i = b0 + threadIdx.x;
+    __syncthreads();
+    const int sum = total + block_scan<kRowThreads>(i < a.requests ? want_of(a, i).need : 0, warp_sums);
+    if (i < a.requests && sum <= available) atomicMax(&taken, sum);
+    total += warp_sums[31];
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) a.free_out[0] = available - taken;
+}
+
+// Outputs that may be the inputs' own memory.  Who gets what, and the new lengths: one block, requests in rounds of one a thread.  It
+// fills the rows too where that is little (FILL); another kernel does where it is much.
+template <bool FILL>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+  __shared__ int warp_sums[32], taken;
+  __shared__ Grant given[FILL ? kPlanThreads : 1];
+  const int available = min(max(a.free_in[0], 0), a.pool_size);
+  if (threadIdx.x == 0) taken = 0;
+  int before = 0;   // needs of the rounds so far
+  for (int b0 = 0; b0 < a.requests; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
+    Want w = {};
+    if (b < a.requests) w = want_of(a, b);
+    const int total = before + block_scan(w.need, warp_sums);
+    if (b < a.requests) {
+      const Grant g = grant_of(a, w, total, available);
+      if (g.given) atomicMax(&taken, total);
+      if (FILL) given[threadIdx.x] = g;
+      else a.grants[b] = g;
+      a.lengths_out[b] = g.length + g.tokens;
     }
-    if (j < tokens) {
-      int slot = -1;
-      if (j < g.tokens) {
-        const int at = g.length + j, k = at / page;
-        const int p = k < g.held ? table[(int64_t)b * width + k] : pool[top - (k - g.held)];
-        if (p >= 0 && p < 0x7fffffff / page) slot = p * page + at % page;
+    before += warp_sums[31];
+    __syncthreads();
+    if (FILL) {
+      const int n = min(kPlanThreads, a.requests - b0);
+      for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {   // a warp a request: its new pages, its slots
+        const Grant g = given[i];
+        const int end = max(a.tokens, a.table_out == a.table ? g.held + g.given : a.width);
+        fill_row(a, b0 + i, g, available, threadIdx.x & 31, end, 32);
       }
-      slots[(int64_t)b * tokens + j] = slot;
+      __syncthreads();
     }
   }
+  if (threadIdx.x == 0) {
+    if (!FILL) *a.free_before = available;
+    a.free_out[0] = available - taken;
+  }
+}
+
+__global__ void __launch_bounds__(kRowThreads) fill_kernel(const PlanArgs a) {
+  const int b = blockIdx.y;
+  fill_row(a, b, a.grants[b], *a.free_before, blockIdx.x * kRowEntries + threadIdx.x,
+           min((int)(blockIdx.x + 1) * kRowEntries, max(a.width, a.tokens)), kRowThreads);
 }
 
 // Pages of the requests marked in `which` go back on top of the pool, the last request's last page first: a request that is given
@@ -162,14 +226,21 @@ extern "C" int psa_plan_pages(const int32_t* table, const int32_t* lengths, cons
   PSA_REQUIRE(tokens > 0 && tokens < ((int64_t)1 << 31) && scratch_bytes >= psa_plan_pages_scratch_bytes(requests), PSA_ERR_ARG,
               "psa_plan_pages: %lld tokens, scratch of %zu bytes", (long long)tokens, scratch_bytes);
   cudaStream_t st = (cudaStream_t)stream;
-  int32_t* free_before = static_cast<int32_t*>(scratch);
-  Grant* grants = reinterpret_cast<Grant*>(static_cast<char*>(scratch) + 16);
-  plan_kernel<<<1, kPlanThreads, 0, st>>>(lengths, counts, free_in, lengths_out, free_out, grants, free_before, (int)requests, (int)width,
-                                          (int)pool_size, page_size, (int)tokens, status);
-  PSA_CHECK_LAUNCH("psa_plan_pages");
+  PlanArgs a = {table, lengths, counts, pool, free_in, table_out, lengths_out, free_out, slots, status,
+                reinterpret_cast<Grant*>(static_cast<char*>(scratch) + 16), static_cast<int32_t*>(scratch), (int)requests, (int)width, (int)pool_size,
+                page_size, (int)tokens};
   const int64_t wide = width > tokens ? width : tokens;
-  const dim3 grid((unsigned)(cdiv64(wide, 256) < 64 ? cdiv64(wide, 256) : 64), (unsigned)requests);
-  fill_kernel<<<grid, 256, 0, st>>>(table, pool, grants, free_before, table_out, slots, (int)width, page_size, (int)tokens);
+  const dim3 rows((unsigned)cdiv64(wide, kRowEntries), (unsigned)requests);
+  const bool apart = lengths_out != lengths && free_out != free_in && table_out != table;
+  if (apart && requests <= kPlanThreads) {
+    plan_rows_kernel<<<rows, kRowThreads, 0, st>>>(a);
+  } else if (requests * (table_out == table ? tokens : wide) <= kFewEntries) {
+    plan_kernel<true><<<1, kPlanThreads, 0, st>>>(a);
+  } else {
+    plan_kernel<false><<<1, kPlanThreads, 0, st>>>(a);
+    PSA_CHECK_LAUNCH("psa_plan_pages");
+    fill_kernel<<<rows, kRowThreads, 0, st>>>(a);
+  }
   PSA_CHECK_LAUNCH("psa_plan_pages");
   return PSA_OK;
 }

@@ -11,7 +11,7 @@
 namespace psa {
 namespace {
 
-constexpr int kMaxPairs = 128, kMaxAxes = 8;
+constexpr int kMaxPairs = 128, kMaxAxes = 8, kInFlight = 4;   // kInFlight: heads whose loads a thread issues at once
 
 struct RotaryArgs {
   const void* src[2];
@@ -60,24 +60,36 @@ __global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant_
   }
   const int first = HALF ? chunk * V : chunk * 2 * V, second = HALF ? first + head_dim / 2 : first + V;
   const int heads = a.heads[0] + a.heads[1];
-  for (int h = blockIdx.y; h < heads; h += parts) {
-    const int z = h >= a.heads[0], hh = z ? h - a.heads[0] : h;
-    const T* src = static_cast<const T*>(a.src[z]) + b * a.src_stride[z][0] + hh * a.src_stride[z][1] + t * a.src_stride[z][2];
-    T* dst = static_cast<T*>(a.dst[z]) + b * a.dst_stride[z][0] + hh * a.dst_stride[z][1] + t * a.dst_stride[z][2];
-    Word w0, w1;
-    w0.u = *reinterpret_cast<const uint4*>(src + first);
-    w1.u = *reinterpret_cast<const uint4*>(src + second);
-    T *e0 = word_of<T>(w0), *e1 = word_of<T>(w1);
+  for (int h0 = blockIdx.y; h0 < heads; h0 += kInFlight * parts) {
+    Word w0[kInFlight], w1[kInFlight];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      T& r0 = HALF ? e0[j] : (j < V / 2 ? e0[2 * j] : e1[2 * j - V]);
-      T& r1 = HALF ? e1[j] : (j < V / 2 ? e0[2 * j + 1] : e1[2 * j + 1 - V]);
-      const float x0 = Elem<T>::to_f(r0), x1 = Elem<T>::to_f(r1);
-      r0 = Elem<T>::from_f(x0 * cs[j] - x1 * sn[j]);
-      r1 = Elem<T>::from_f(x1 * cs[j] + x0 * sn[j]);
+    for (int u = 0; u < kInFlight; ++u) {
+      const int h = h0 + u * parts;
+      if (h < heads) {
+        const int z = h >= a.heads[0], hh = z ? h - a.heads[0] : h;
+        const T* src = static_cast<const T*>(a.src[z]) + b * a.src_stride[z][0] + hh * a.src_stride[z][1] + t * a.src_stride[z][2];
+        w0[u].u = __ldg(reinterpret_cast<const uint4*>(src + first));
+        w1[u].u = __ldg(reinterpret_cast<const uint4*>(src + second));
+      }
     }
-    *reinterpret_cast<uint4*>(dst + first) = w0.u;
-    *reinterpret_cast<uint4*>(dst + second) = w1.u;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int h = h0 + u * parts;
+      if (h >= heads) break;
+      T *e0 = word_of<T>(w0[u]), *e1 = word_of<T>(w1[u]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        T& r0 = HALF ? e0[j] : (j < V / 2 ? e0[2 * j] : e1[2 * j - V]);
+        T& r1 = HALF ? e1[j] : (j < V / 2 ? e0[2 * j + 1] : e1[2 * j + 1 - V]);
+        const float x0 = Elem<T>::to_f(r0), x1 = Elem<T>::to_f(r1);
+        r0 = Elem<T>::from_f(x0 * cs[j] - x1 * sn[j]);
+        r1 = Elem<T>::from_f(x1 * cs[j] + x0 * sn[j]);
+      }
+      const int z = h >= a.heads[0], hh = z ? h - a.heads[0] : h;
+      T* dst = static_cast<T*>(a.dst[z]) + b * a.dst_stride[z][0] + hh * a.dst_stride[z][1] + t * a.dst_stride[z][2];
+      *reinterpret_cast<uint4*>(dst + first) = w0[u].u;
+      *reinterpret_cast<uint4*>(dst + second) = w1[u].u;
+    }
   }
 }
 
@@ -88,7 +100,7 @@ int launch(const RotaryArgs& a, int head_dim, int half, cudaStream_t st) {
   PSA_REQUIRE(blocks < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_rotate_axes: too many tokens");
   const int heads = a.heads[0] + a.heads[1];
   int parts = 1;   // few tokens: the heads are shared out over blocks
-  while (parts < heads && blocks * parts < 148 * 8) parts *= 2;
+  while (parts < heads && blocks * parts < 148 * 16) parts *= 2;
   if (parts > heads) parts = heads;
   const dim3 grid((unsigned)blocks, (unsigned)parts);
   if (half) rotary_axes_kernel<T, true><<<grid, 128, 0, st>>>(a, head_dim, parts);
