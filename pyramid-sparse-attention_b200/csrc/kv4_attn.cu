@@ -84,8 +84,11 @@ struct Shape {
   static constexpr int64_t kPart = (int64_t)kRows * (D + 2);
 };
 
-struct Span {   // a request's place in the line of tiles
-  int rows, row_tiles, tiles, work;
+// A request's part of the line.  A unit - a key head with up to R rows - counts kUnitCells more than it has tiles: what its rows cost before
+// and after the tiles (33 requests of 17 to 16384 tokens, 16 key heads: 110 us without, the blocks with many short ones last).
+constexpr int kUnitCells = 2;
+struct Span {
+  int rows, row_tiles, tiles, cells, work;
 };
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_tile, int& length, int& count) {
   length = a.lengths[b];
@@ -100,11 +103,12 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_t
   s.rows = count * a.group;
   s.row_tiles = (s.rows + rows_per_tile - 1) / rows_per_tile;
   s.tiles = (length + kTile - 1) / kTile;
-  s.work = s.tiles * s.row_tiles * a.kv_heads;   // the entry point sees to it that the sum over all requests fits 32 bits
+  s.cells = s.tiles ? s.tiles + kUnitCells : 0;
+  s.work = s.cells * s.row_tiles * a.kv_heads;   // the entry point sees to it that the sum over all requests fits 32 bits
   return s;
 }
 
-// The line is shared out in stretches of `each` tiles, the first `longer` of them one longer.
+// The line is shared out in stretches of `each` cells, the first `longer` of them one longer.
 struct Shares {
   int blocks, each, longer;
   __device__ __forceinline__ Shares(int work, int most_blocks, int least) {
@@ -119,7 +123,7 @@ struct Shares {
   }
 };
 
-// The whole line's length, and the request that tile `first(block)` lies in with the place where that begins.  scan: 8 words.
+// The whole line's length, and the request that cell `first(block)` lies in with the place where that begins.  scan: 8 words.
 __device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int* scan, int& request, int& base, Shares& shares) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int length, count, mine = 0;
@@ -136,7 +140,7 @@ __device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int
   int work = 0;
 #pragma unroll
   for (int w = 0; w <= kWarps; ++w) work += scan[w];
-  shares = Shares(work, gridDim.x, a.least_tiles);
+  shares = Shares(work, gridDim.x, kUnitCells + a.least_tiles);
   request = base = 0;
   if ((int)blockIdx.x >= shares.blocks || a.batch == 1) return work;
   // whose tile it is: requests in rounds of one a thread
@@ -425,8 +429,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
     const Span span = span_of(a, b, kRows, length, count);
     const int end = base + span.work;
     while (at < last && at < end) {
-      const int unit = (at - base) / span.tiles, tile0 = at - base - unit * span.tiles;
-      const int tiles = min(span.tiles - tile0, last - at);
+      const int unit = (at - base) / span.cells, cell = at - base - unit * span.cells, cells = min(span.cells - cell, last - at);
+      const int tile0 = max(cell - kUnitCells, 0), tiles = max(cell + cells - kUnitCells, 0) - tile0;
+      const int unit_at = at - cell;
+      at += cells;
+      if (tiles == 0) continue;
       const int head = unit / span.row_tiles, row0 = (unit - head * span.row_tiles) * kRows;
       if (warp == kWarps) {
         // ------------------------------------------------------------ copies: a lane a slice, eight tiles' page numbers at a time
@@ -588,11 +595,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
         }
         if (starts && threadIdx.x == 0) {
           // whose parts the unit is made of: from this block to the one that holds its last tile
-          a.owners[((int64_t)b * a.kv_heads + head) * a.row_tiles + row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(at + span.tiles - 1));
+          a.owners[((int64_t)b * a.kv_heads + head) * a.row_tiles + row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(unit_at + span.cells - 1));
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
       }
-      at += tiles;
     }
     base = end;
   }
@@ -777,7 +783,7 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   a.least_tiles = 2;
   a.row_tiles = (int)cdiv64(rows, rows_per_tile(rows));
   PSA_REQUIRE(rows < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_kv4_attention: %lld rows a key head", (long long)rows);
-  PSA_REQUIRE((double)batch * cdiv64(width * page_size, kTile) * a.row_tiles * kv_heads < 2147483648.0, PSA_ERR_UNSUPPORTED,
+  PSA_REQUIRE((double)batch * (cdiv64(width * page_size, kTile) + kUnitCells) * a.row_tiles * kv_heads < 2147483648.0, PSA_ERR_UNSUPPORTED,
               "psa_kv4_attention: %lld requests of up to %lld tokens: more than 2^31 tiles", (long long)batch, (long long)(width * page_size));
   a.owners = static_cast<int2*>(scratch);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + owners_bytes(batch, kv_heads, a.row_tiles));

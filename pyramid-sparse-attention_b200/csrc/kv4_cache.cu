@@ -21,6 +21,11 @@ struct CacheArgs {
   int heads, page;
 };
 
+// A quotient of which only the rounded value counts: the product with the inverse, corrected by its remainder (Markstein, IBM Journal of
+// Research and Development 34, 1990: the quotient rounded to nearest, if the inverse is and nothing leaves the normal range).  With
+// a division for each value their special function units bound the kernel.  The sum with 1.5 * 2^23 rounds to whole numbers.
+constexpr float kTiny = 8.673617379884035e-19f, kRound = 12582912.f;   // 2^-60
+
 // Largest number of the type that is not above x >= 0.
 __device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
 __device__ __forceinline__ __nv_bfloat16 cut_off(float x, __nv_bfloat16) { return __float2bfloat16_rz(x); }
@@ -101,8 +106,13 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
     if (!isfinite(wide)) {
       step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));
     } else if (s > 0.f) {
+      const bool plain = s > kTiny && s < 1.f / kTiny;
+      const float inverse = 1.f / s;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) codes |= (uint32_t)fminf(rintf((x[j] - lo) / s), 15.f) << (4 * j);
+      for (int j = 0; j < 8; ++j) {
+        const float d = x[j] - lo, q0 = d * inverse, q = plain ? fmaf(fmaf(-q0, s, d), inverse, q0) : d / s;
+        codes |= (__float_as_uint(fminf(q, 15.f) + kRound) & 15u) << (4 * j);
+      }
     }
     if (z) codes = swap_units(codes, odd);
     if (!at.good || h >= at.heads) continue;
@@ -141,7 +151,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const CacheArgs a) {
     uint4 w;
     T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = Elem<T>::from_f(fmaf((float)(n >> (4 * j) & 15), step, lowest));
+    for (int j = 0; j < 8; ++j)   // the code behind the point of 2^23 is a number without a conversion
+      e[j] = Elem<T>::from_f(fmaf(__uint_as_float((n >> (4 * j) & 15u) | 0x4b000000u) - 8388608.f, step, lowest));
     if (at.in && h < at.heads) *reinterpret_cast<uint4*>(dst + h * a.stride[z][1]) = w;
   }
 }

@@ -43,7 +43,8 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums) {   // inclusiv
   return x + (warp ? warp_sums[warp - 1] : 0);
 }
 
-__device__ __forceinline__ int pages_of(int64_t tokens, int page) { return (int)((tokens + page - 1) / page); }
+// tokens below 2^31
+__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((uint32_t)tokens + (uint32_t)page - 1u) / (uint32_t)page); }
 
 struct PlanArgs {
   const int32_t *table, *lengths, *counts, *pool, *free_in;
@@ -66,7 +67,7 @@ __device__ __forceinline__ Want want_of(const PlanArgs& a, int b) {
   w.bad = w.length < 0 || w.length > most || w.count < 0 || w.count > a.tokens || (int64_t)w.length + w.count > most;
   if (w.bad) w.count = 0;
   w.held = pages_of(min(max(w.length, 0), (int)most), a.page);
-  w.need = w.bad ? 0 : pages_of((int64_t)w.length + w.count, a.page) - w.held;
+  w.need = w.bad ? 0 : pages_of(w.length + w.count, a.page) - w.held;
   return w;
 }
 __device__ __forceinline__ Grant grant_of(const PlanArgs& a, const Want& w, int total, int available) {
@@ -87,7 +88,7 @@ __device__ __forceinline__ void fill_row(const PlanArgs& a, int b, const Grant& 
     if (j < a.tokens) {
       int slot = -1;
       if (j < g.tokens) {
-        const int at = g.length + j, k = at / a.page;
+        const int at = g.length + j, k = (int)((uint32_t)at / (uint32_t)a.page);
         const int p = k < g.held ? a.table[row + k] : a.pool[top - (k - g.held)];
         if (p >= 0 && p < 0x7fffffff / a.page) slot = p * a.page + (at - k * a.page);
       }
