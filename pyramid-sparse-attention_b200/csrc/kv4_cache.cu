@@ -26,9 +26,24 @@ struct CacheArgs {
 // a division for each value their special function units bound the kernel.  The sum with 1.5 * 2^23 rounds to whole numbers.
 constexpr float kTiny = 8.673617379884035e-19f, kRound = 12582912.f;   // 2^-60
 
-// Largest number of the type that is not above x >= 0.
+// Largest number of the type that is not above x >= 0 (a NaN stays one).
 __device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
 __device__ __forceinline__ __nv_bfloat16 cut_off(float x, __nv_bfloat16) { return __float2bfloat16_rz(x); }
+
+// Two numbers of the type in a word, and the number from which whole numbers up to 15 on are neighbours in it.
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+  using type = __half2;
+  static constexpr uint32_t kBase = 0x64006400u;
+  static __device__ __forceinline__ __half2 make(__half a, __half b) { return __halves2half2(a, b); }
+  static __device__ __forceinline__ __half2 base() { return __float2half2_rn(1024.f); }
+};
+template <> struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static constexpr uint32_t kBase = 0x43004300u;
+  static __device__ __forceinline__ __nv_bfloat162 make(__nv_bfloat16 a, __nv_bfloat16 b) { return __halves2bfloat162(a, b); }
+  static __device__ __forceinline__ __nv_bfloat162 base() { return __float2bfloat162_rn(128.f); }
+};
 
 constexpr int kHeads = 4;   // heads of a token that a thread takes, their loads in flight together
 
@@ -80,39 +95,33 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
   const bool odd = at.u >> 2 & 1;
 #pragma unroll
   for (int h = 0; h < kHeads; ++h) {
-    const T* e = reinterpret_cast<const T*>(&w[h]);
-    float x[8], lo, hi;
-    bool finite = true;
+    using T2 = typename Pair<T>::type;
+    const T2* e = reinterpret_cast<const T2*>(&w[h]);
+    // lowest and negated highest value, two numbers in a word; a NaN stays one
+    T2 low = __hmin2_nan(__hmin2_nan(e[0], e[1]), __hmin2_nan(e[2], e[3])), high = __hmax2_nan(__hmax2_nan(e[0], e[1]), __hmax2_nan(e[2], e[3]));
+    low = Pair<T>::make(__hmin_nan(low.x, low.y), __hneg(__hmax_nan(high.x, high.y)));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = Elem<T>::to_f(e[j]);
-      lo = j ? fminf(lo, x[j]) : x[j];
-      hi = j ? fmaxf(hi, x[j]) : x[j];
-      finite = finite && isfinite(x[j]);
-    }
-    // one that is not finite takes the whole group along: the range of such a group is not finite either
-    lo = finite ? lo : -INFINITY;
-    hi = finite ? hi : INFINITY;
-#pragma unroll
-    for (int d = 1; d < G / 8; d *= 2) {
-      lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
-      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
-    }
-    const float wide = (hi - lo) / 15.f;
+    for (int d = 1; d < G / 8; d *= 2) low = __hmin2_nan(low, __shfl_xor_sync(~0u, low, d));
+    const float lo = Elem<T>::to_f(low.x), wide = (-Elem<T>::to_f(low.y) - lo) / 15.f;
     T step = cut_off(wide, T());
-    T lowest = Elem<T>::from_f(lo);
+    T lowest = low.x;
     const float s = Elem<T>::to_f(step);
     uint32_t codes = 0;
-    if (!isfinite(wide)) {
+    if (!isfinite(wide)) {   // an infinity or a NaN among them, or a range beyond 32 bits
       step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));
-    } else if (s > 0.f) {
-      const bool plain = s > kTiny && s < 1.f / kTiny;
+    } else if (s > kTiny && s < 1.f / kTiny) {
       const float inverse = 1.f / s;
+      // a rounded quotient's bits are those of 1.5 * 2^23 plus the code: their sum with weights 16^j, less what the constant makes
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = x[j] - lo, q0 = d * inverse, q = plain ? fmaf(fmaf(-q0, s, d), inverse, q0) : d / s;
-        codes |= (__float_as_uint(fminf(q, 15.f) + kRound) & 15u) << (4 * j);
+      for (int j = 7; j >= 0; --j) {
+        const float d = Elem<T>::to_f(j & 1 ? e[j / 2].y : e[j / 2].x) - lo, q0 = d * inverse, q = fmaf(fmaf(-q0, s, d), inverse, q0);
+        codes = codes * 16u + __float_as_uint(fminf(q, 15.f) + kRound);
       }
+      codes -= 0x4b400000u * 0x11111111u;
+    } else if (s > 0.f) {
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j)
+        codes |= (__float_as_uint(fminf((Elem<T>::to_f(reinterpret_cast<const T*>(e)[j]) - lo) / s, 15.f) + kRound) & 15u) << (4 * j);
     }
     if (z) codes = swap_units(codes, odd);
     if (!at.good || h >= at.heads) continue;
@@ -146,13 +155,17 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const CacheArgs a) {
 #pragma unroll
   for (int h = 0; h < kHeads; ++h) {
     const uint32_t n = z ? swap_units(codes[h], odd) : codes[h];
-    const T* p = reinterpret_cast<const T*>(&pair[h]);
-    const float step = Elem<T>::to_f(p[0]), lowest = Elem<T>::to_f(p[1]);
-    uint4 w;
-    T* e = reinterpret_cast<T*>(&w);
+    using T2 = typename Pair<T>::type;
+    const T2 p = *reinterpret_cast<const T2*>(&pair[h]), step = Pair<T>::make(p.x, p.x), lowest = Pair<T>::make(p.y, p.y);
+    uint32_t y[4];   // channels i and i + 4: lowest + code * step, rounded once
 #pragma unroll
-    for (int j = 0; j < 8; ++j)   // the code behind the point of 2^23 is a number without a conversion
-      e[j] = Elem<T>::from_f(fmaf(__uint_as_float((n >> (4 * j) & 15u) | 0x4b000000u) - 8388608.f, step, lowest));
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = (n >> (4 * i) & 0x000f000fu) | Pair<T>::kBase;
+      const T2 v = __hfma2(__hsub2(*reinterpret_cast<const T2*>(&c), Pair<T>::base()), step, lowest);
+      y[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const uint4 w = make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                               __byte_perm(y[2], y[3], 0x7632));
     if (at.in && h < at.heads) *reinterpret_cast<uint4*>(dst + h * a.stride[z][1]) = w;
   }
 }

@@ -78,28 +78,31 @@ __device__ __forceinline__ Grant grant_of(const PlanArgs& a, const Want& w, int 
 
 // Entries [from, to) of a request's row of the table and of its slots.
 __device__ __forceinline__ void fill_row(const PlanArgs& a, int b, const Grant& g, int available, int from, int to, int step) {
-  const int top = available - 1 - g.first;
-  const int64_t row = (int64_t)b * a.width;
+  const int top = available - 1 - g.first, shift = a.page & (a.page - 1) ? -1 : 31 - __clz(a.page), most_pages = 0x7fffffff / a.page;
+  const int32_t* table = a.table + (int64_t)b * a.width;
+  int32_t* table_out = a.table_out + (int64_t)b * a.width;
+  int32_t* slots = a.slots + (int64_t)b * a.tokens;
+#pragma unroll 4
   for (int j = from; j < to; j += step) {
     if (j < a.width) {
       const bool fresh = j >= g.held && j < g.held + g.given;
-      if (fresh || a.table_out != a.table) a.table_out[row + j] = fresh ? a.pool[top - (j - g.held)] : a.table[row + j];
+      if (fresh || table_out != table) table_out[j] = fresh ? a.pool[top - (j - g.held)] : table[j];
     }
     if (j < a.tokens) {
       int slot = -1;
       if (j < g.tokens) {
-        const int at = g.length + j, k = (int)((uint32_t)at / (uint32_t)a.page);
-        const int p = k < g.held ? a.table[row + k] : a.pool[top - (k - g.held)];
-        if (p >= 0 && p < 0x7fffffff / a.page) slot = p * a.page + (at - k * a.page);
+        const int at = g.length + j, k = shift >= 0 ? at >> shift : (int)((uint32_t)at / (uint32_t)a.page);
+        const int p = k < g.held ? table[k] : a.pool[top - (k - g.held)];
+        if (p >= 0 && p < most_pages) slot = p * a.page + (at - k * a.page);
       }
-      a.slots[(int64_t)b * a.tokens + j] = slot;
+      slots[j] = slot;
     }
   }
 }
 
 // Outputs beside the inputs, up to kPlanThreads requests: a block fills a stretch of a request's row and sums the needs of the requests
 // before it for itself - a few hundred numbers that all blocks find in L2 - which spares a launch that would do nothing else.
-constexpr int kRowThreads = 256, kRowEntries = 2048;
+constexpr int kRowThreads = 256, kRowEntries = 1024;
 __global__ void __launch_bounds__(kRowThreads) plan_rows_kernel(const PlanArgs a) {
   __shared__ int warp_sums[32], taken;
   const int b = blockIdx.y, available = min(max(a.free_in[0], 0), a.pool_size);

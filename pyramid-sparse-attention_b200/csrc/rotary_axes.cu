@@ -37,8 +37,9 @@ template <> __device__ __forceinline__ float* word_of<float>(Word& w) { return w
 template <> __device__ __forceinline__ __half* word_of<__half>(Word& w) { return w.h; }
 template <> __device__ __forceinline__ __nv_bfloat16* word_of<__nv_bfloat16>(Word& w) { return w.b; }
 
-// A thread owns V pairs of one token - two 16-byte words of a row - computes their sines and cosines once and walks the heads
-// with them.  HALF: pair i is channels (i, i + D/2); otherwise neighbours (2i, 2i + 1).
+// A thread owns V pairs of one token, computes their sines and cosines once and walks the heads with them.  Its two 16-byte words of a
+// row lie half a row apart, so that a warp's words are neighbours, whichever channels make a pair: HALF, channels (i, i + D/2), one of
+// each word; otherwise neighbours (2i, 2i + 1), V/2 pairs in each.
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant__ RotaryArgs a, int head_dim, int parts) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -51,14 +52,14 @@ __global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant_
   float cs[V], sn[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int pair = chunk * V + j;
+    const int pair = HALF ? chunk * V + j : chunk * (V / 2) + j % (V / 2) + (j < V / 2 ? 0 : head_dim / 4);
     const int64_t at = a.axis[pair] * a.pos_stride[0] + b * a.pos_stride[1] + t * a.pos_stride[2];
     const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : static_cast<const int32_t*>(a.pos)[at];
     const int32_t turn = (int32_t)(((uint64_t)p * a.turns[pair]) >> 32);
     sincospif((float)turn * 4.656612873077393e-10f, &sn[j], &cs[j]);   // 2^-31 half turns
     if (a.inverse) sn[j] = -sn[j];
   }
-  const int first = HALF ? chunk * V : chunk * 2 * V, second = HALF ? first + head_dim / 2 : first + V;
+  const int first = chunk * V, second = first + head_dim / 2;
   const int heads = a.heads[0] + a.heads[1];
   for (int h0 = blockIdx.y; h0 < heads; h0 += kInFlight * parts) {
     Word w0[kInFlight], w1[kInFlight];
