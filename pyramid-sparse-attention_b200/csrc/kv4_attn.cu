@@ -67,6 +67,9 @@ constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has se
 constexpr float kHead = 7.f, kLazy = 8.f;
 constexpr float kLeastCap = 5.9604644775390625e-8f;   // 2^-24
 // Sums of q are kept in units of scores, 2^-24 of q's operands - in f16, whose numbers end there, 2^12 times that.
+// A weight times a step in one term of 11 bits is as exact as a bf16 output needs (2^-12 of what the codes add, against its 2^-9); an f16
+// output shows it (0.00041 of the output's norm instead of 0.00021), so there it is two terms: 25 products a slice instead of 17.
+template <typename T> constexpr int kWeightTerms = std::is_same<T, __half>::value ? 2 : 1;
 template <typename T> constexpr float kSumScale = std::is_same<T, __half>::value ? 2.44140625e-4f : 1.f;
 
 template <int D, int G, int NT>
@@ -239,6 +242,7 @@ template <typename T, int D, int G, int NT, bool MASKED>
 __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* slice, int t0) {
   using L = Kv4<D, G>;
   constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
+  constexpr int kTerms = kWeightTerms<T>;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   // ---- scores: rows are the tokens r/2 + 4 (r % 2) and that + 8, which lie in rows r and r + 8 of the keys
   float x[NT][4];
@@ -356,7 +360,7 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
     const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
     // a slice's first eight tokens: lo + s n; the others: hi - s (15 - n)
     const float ends[2] = {u0.y, fmaf(15.f, u1.x, u1.y)};
-    uint32_t w[NT][2];
+    uint32_t w[kTerms][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float y[4];
@@ -372,8 +376,17 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
           s.mid[nt][g][j & 1] += z;
         }
       }
-      w[nt][0] = movmatrix(MmaOp<__half>::pack(y[0], y[1]));
-      w[nt][1] = movmatrix(MmaOp<__half>::pack(y[2], y[3]));
+#pragma unroll
+      for (int k = 0; k < kTerms; ++k) {
+        float first[4];   // 11 bits, cut off where another term follows
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          first[j] = k + 1 < kTerms ? __uint_as_float(__float_as_uint(y[j]) & 0xffffe000u) : y[j];
+          y[j] -= first[j];
+        }
+        w[k][nt][0] = movmatrix(MmaOp<__half>::pack(first[0], first[1]));
+        w[k][nt][1] = movmatrix(MmaOp<__half>::pack(first[2], first[3]));
+      }
     }
 #pragma unroll
     for (int i = 0; i < BG; ++i) {
@@ -384,7 +397,9 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
       for (int h = 0; h < 2; ++h) {
         const uint32_t a[4] = {codes(v0, 2 * h), codes(v0, 2 * h + 1), rest(v1, 2 * h), rest(v1, 2 * h + 1)};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[nt]);
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[k][nt]);
       }
     }
   }
@@ -420,6 +435,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
   __syncthreads();
   if ((int)blockIdx.x >= shares.blocks) return;
   const int group = a.group, slices_per_page = a.page / 16;
+  const bool whole_tiles = a.page % kTile == 0;
   int stage = 0;
   uint32_t phase = 0;
   int at = shares.first(blockIdx.x);
@@ -436,28 +452,41 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
       if (tiles == 0) continue;
       const int head = unit / span.row_tiles, row0 = (unit - head * span.row_tiles) * kRows;
       if (warp == kWarps) {
-        // ------------------------------------------------------------ copies: a lane a slice, eight tiles' page numbers at a time
-        const int slices = (length + 15) / 16, first_slice = tile0 * kWarps, last_slice = min(slices, (tile0 + tiles) * kWarps);
-        for (int s0 = first_slice; s0 < last_slice; s0 += 32) {
-          const int s = s0 + lane;
+        // ------------------------------------------------------------ copies.  A lane looks a page number up for a tile that lies in one piece
+        // (whole: one copy a tile, 32 tiles at a time), or else for a slice (8 tiles at a time)
+        const int slices = (length + 15) / 16, last_slice = min(slices, (tile0 + tiles) * kWarps), stride = whole_tiles ? kWarps : 1;
+        for (int s0 = tile0 * kWarps; s0 < last_slice; s0 += 32 * stride) {
+          const int s = s0 + stride * lane;
           int64_t from = -1;
           if (s < last_slice) {
-            const int page = a.table[(int64_t)b * a.width + s / slices_per_page];
-            if (page >= 0 && page < a.pages) from = (((int64_t)page * a.kv_heads + head) * slices_per_page + s % slices_per_page) * L::kSlice;
+            const int in_page = s / slices_per_page, page = a.table[(int64_t)b * a.width + in_page];
+            if (page >= 0 && page < a.pages) from = (((int64_t)page * a.kv_heads + head) * slices_per_page + s - in_page * slices_per_page) * L::kSlice;
             else *a.status = PSA_ERR_ARG;
           }
           const uint32_t good = __ballot_sync(~0u, from >= 0);
-          for (int k = 0; k < 8 && s0 + kWarps * k < last_slice; ++k) {
-            const uint32_t bits = good >> (kWarps * k) & ((1u << kWarps) - 1);
+          const int n = min(32 * stride, last_slice - s0);
+          for (int k = 0; k < n; k += kWarps) {
             const bool ok = !*abort_flag && tc::mbar_wait(empty + stage, phase ^ 1, abort_flag);
             if (__all_sync(~0u, ok)) {
-              if (lane == 0) {
-                valid[stage] = bits;
-                tc::mbar_arrive_expect_tx(full + stage, __popc(bits) * L::kSlice);
+              const uint32_t in = (1u << min(kWarps, n - k)) - 1;   // the tile's slices
+              uint8_t* to = smem + stage * kWarps * L::kSlice;
+              if (whole_tiles) {
+                if (lane == k / kWarps) {
+                  const int bytes = from >= 0 ? __popc(in) * L::kSlice : 0;
+                  valid[stage] = from >= 0 ? in : 0u;
+                  tc::mbar_arrive_expect_tx(full + stage, bytes);
+                  if (bytes) tc::bulk_load_a(tc::smem_u32(to), a.data + from, bytes, tc::smem_u32(full + stage));
+                }
+              } else {
+                const uint32_t bits = good >> k & in;
+                if (lane == 0) {
+                  valid[stage] = bits;
+                  tc::mbar_arrive_expect_tx(full + stage, __popc(bits) * L::kSlice);
+                }
+                __syncwarp();
+                if (from >= 0 && lane / kWarps == k / kWarps)
+                  tc::bulk_load_a(tc::smem_u32(to + lane % kWarps * L::kSlice), a.data + from, L::kSlice, tc::smem_u32(full + stage));
               }
-              __syncwarp();
-              if (from >= 0 && lane / kWarps == k)
-                tc::bulk_load_a(tc::smem_u32(smem + (stage * kWarps + lane % kWarps) * L::kSlice), a.data + from, L::kSlice, tc::smem_u32(full + stage));
             }
             if (++stage == kStages) stage = 0, phase ^= 1;
           }
