@@ -4,7 +4,8 @@
 
 Each csrc/*.cu is compiled to build/*.o in parallel with
 ``nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and linked into
-psa_b200/libpsa_b200.so.  Objects are reused when they are newer than every source and header.
+psa_b200/libpsa_b200.so; csrc/calls.cpp, the Python entry to some of its calls, is compiled with the host compiler
+against torch's headers and linked with that library into psa_b200/_calls.so.  Objects are reused when they are newer than every source and header.
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +21,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "psa_b200", "libpsa_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CALLS = os.path.join(HERE, "psa_b200", "_calls.so")
+CXX = os.environ.get("CXX", "g++")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
@@ -60,7 +64,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run([NVCC, "-shared", "-o", LIB, *objs], capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_calls(force, hdr_t)
     return LIB
+
+
+def build_calls(force: bool, hdr_t: float) -> None:
+    import torch
+    src = os.path.join(CSRC, "calls.cpp")
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), hdr_t):
+        return
+    at = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(NVCC)) or "/usr/local/cuda"
+    include = [os.path.join(HERE, "..", "include"), os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    abi = f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    r = subprocess.run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", abi, *[f"-I{i}" for i in include], src, "-o", CALLS,
+                        f"-L{os.path.dirname(LIB)}", f"-l:{os.path.basename(LIB)}", "-Wl,-rpath,$ORIGIN", f"-L{os.path.join(at, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"],
+                       capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed on {src}:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

@@ -24,6 +24,10 @@ if not os.path.exists(LIB_PATH):
 
 lib = C.CDLL(LIB_PATH)
 
+import torch  # noqa: E402,F401  (_calls links against its libraries)
+
+from . import _calls  # noqa: E402,F401  (built beside the library: the answering operators' ordinary calls in one step)
+
 _p, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes); mirrors include/psa_b200.h declaration by declaration

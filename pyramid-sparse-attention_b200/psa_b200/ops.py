@@ -11,7 +11,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import PSA_FWD_BLOCKS_MAX, PSA_FWD_LIST_MAX, check, lib
+from ._lib import PSA_FWD_BLOCKS_MAX, PSA_FWD_LIST_MAX, _calls, check, lib
 
 _DT = {torch.float32: _lib.PSA_F32, torch.float16: _lib.PSA_F16, torch.bfloat16: _lib.PSA_BF16}
 
@@ -68,6 +68,7 @@ def status_word(device) -> torch.Tensor:
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     if idx not in _STATUS:
         _STATUS[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        _calls.status(idx, _STATUS[idx].data_ptr())
     return _STATUS[idx]
 
 
@@ -828,19 +829,9 @@ def legacy_backward(q, k, v, mask, o, lse, do, causal: bool, sm_scale: float, py
 # The answering side of the vision-language call site: rotary positions with several axes, a cache in pages that holds keys and
 # values in 4 bits, and the attention of new tokens over it.
 #
-# A step of one token is a dozen calls whose kernels take 2 to 8 us each: the host's share counts.  What a call checks and lays out from
-# shapes, strides, types and devices alone - plain numbers - is done once for each and kept by their values (a plan); a call looks its plan
-# up, allocates and launches.
-_PLANS: Dict[tuple, tuple] = {}
-
-
-def _keep(key: tuple, plan: tuple) -> tuple:
-    if len(_PLANS) >= 1024:
-        _PLANS.clear()
-    _PLANS[key] = plan
-    return plan
-
-
+# A step of one token is a dozen calls whose kernels take 2 to 8 us each: the host's share counts.  An ordinary call - CUDA tensors that a
+# kernel can read as they are - is looked at, given its outputs and launched by one function of _calls; that returns None for any other,
+# which is laid out, or refused with a reason, here.
 def _in_words(x: torch.Tensor) -> bool:
     """Whether the kernels can read rows x [B, H, S, D] word by word (any batch, head and token strides), its address aside."""
     return x.stride(3) == 1 and all(n == 1 or s * x.element_size() % 16 == 0 for n, s in zip(x.shape[:3], x.stride()[:3]))
@@ -882,42 +873,57 @@ _TWO_PI = 2 * Fraction("3.141592653589793238462643383279502884197169399375105820
 def _rotary_plan(head_dim: int, sections: Tuple[int, ...], theta: float, per_axis: bool, inv_freq: Optional[Tuple[float, ...]]):
     """Turns a position (of 2^64) and axis of every channel pair, as psa_rotate_axes takes them: plain numbers, kept by value."""
     pairs = head_dim // 2
-    if inv_freq is None:
-        if per_axis:
-            inv_freq = [theta ** -(j / n) for n in sections for j in range(n)]
-        else:
-            inv_freq = [theta ** -(j / pairs) for j in range(pairs)]
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise ValueError(f"rotate_axes: head_dim {head_dim} (a multiple of 16 up to 256)")
+    if not 1 <= len(sections) <= 8 or any(n < 0 for n in sections) or sum(sections) != pairs:
+        raise ValueError(f"rotate_axes: sections {sections} are not {pairs} channel pairs of 1 to 8 axes")
+    if inv_freq is not None:
+        if len(inv_freq) != pairs or not all(math.isfinite(f) for f in inv_freq):
+            raise ValueError(f"rotate_axes: inv_freq must be {pairs} finite numbers")
+    elif not (math.isfinite(theta) and theta > 0):
+        raise ValueError(f"rotate_axes: theta must be positive, got {theta}")
+    elif per_axis:
+        inv_freq = [theta ** -(j / n) for n in sections for j in range(n)]
+    else:
+        inv_freq = [theta ** -(j / pairs) for j in range(pairs)]
     turns = [round(Fraction(f) * 2 ** 64 / _TWO_PI) % 2 ** 64 for f in inv_freq]
     axis = [a for a, n in enumerate(sections) for _ in range(n)]
     return (C.c_uint64 * pairs)(*turns), (C.c_uint8 * pairs)(*axis)
 
 
 def _rotate(xs, positions: torch.Tensor, plan, half: bool, inverse: bool):
-    """xs: 1 or 2 tensors [B, H, S, D], positions [axes, B or 1, S] -> turned copies."""
+    """xs: 1 or 2 tensors [B, H, S, D], positions [axes, S] or [axes, B or 1, S] -> turned copies."""
     x, n = xs[0], len(xs)
-    key = ("rotate", *[(t.shape, t.stride()) for t in xs], x.dtype, positions.shape, positions.stride(), positions.dtype)
-    call = _PLANS.get(key)
-    if call is None:
-        copy = [not _in_words(t) for t in xs]
-        likes = [_rows_like(_laid_out(t) if c else t) for t, c in zip(xs, copy)]
-        B, _, S, D = x.shape
-        call = _keep(key, (any(copy), copy, _row_strides(*xs), [like for like, _ in likes],
-                           (C.c_int64 * (3 * n))(*[s for _, strides in likes for s in strides]), (C.c_int32 * n)(*[t.shape[1] for t in xs]),
-                           C.c_int(n), C.c_int(8 * positions.element_size()),
-                           (C.c_int64 * 3)(positions.stride(0), positions.stride(1) if positions.shape[1] > 1 else 0, positions.stride(2)),
-                           (C.c_int(positions.shape[0]), C.c_int64(B), C.c_int64(S), C.c_int(D)), C.c_int(_dt(x)), C.c_void_p * n, B * S))
-    any_copy, copy, strides, like, out_strides, heads, count, bits, pos_strides, sizes, dt, pointers, tokens = call
-    at = [t.data_ptr() for t in xs]
-    if any_copy or any(p & 15 for p in at):
-        return _rotate([_laid_out(t) if c or p & 15 else t for t, c, p in zip(xs, copy, at)], positions, plan, half, inverse)
-    outs = [_new_rows(t, k) for t, k in zip(xs, like)]
-    if tokens > 0:
-        index = x.get_device()
-        with _on(x):
-            rc = lib.psa_rotate_axes(pointers(*at), strides, pointers(*[o.data_ptr() for o in outs]), out_strides, heads, count,
-                                     positions.data_ptr(), bits, pos_strides, plan[0], plan[1], *sizes, half, inverse, dt,
-                                     torch._C._cuda_getCurrentRawStream(index))
-        check(rc, "psa_rotate_axes")
+    outs = _calls.rotate(x, xs[1] if n == 2 else None, positions, plan[0], plan[1], half, inverse)
+    if outs is not None:
+        if type(outs) is int:
+            check(outs, "psa_rotate_axes")
+        return outs
+    if any(t.dim() != 4 or (t.shape[0], *t.shape[2:]) != (x.shape[0], *x.shape[2:]) or t.dtype != x.dtype for t in xs):
+        raise ValueError("rotate_axes: q [B, H, S, D] and k [B, Hkv, S, D] of one dtype")
+    _dt(x)
+    B, _, S, D = x.shape
+    axes = max(plan[1]) + 1
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"rotate_axes: positions must be int32 or int64, got {positions.dtype}")
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(1)
+    if positions.dim() != 3 or positions.shape[0] < axes or positions.shape[1] not in (1, B) or positions.shape[2] != S:
+        raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{axes}, {B}, {S}]")
+    _device_of(*xs, positions)
+    xs = [t if _in_words(t) and t.data_ptr() % 16 == 0 else _laid_out(t) for t in xs]
+    likes = [_rows_like(t) for t in xs]
+    outs = tuple(_new_rows(t, like) for t, (like, _) in zip(xs, likes))
+    if B == 0 or S == 0:
+        return outs
+    pointers = C.c_void_p * n
+    with _on(x):
+        rc = lib.psa_rotate_axes(pointers(*[t.data_ptr() for t in xs]), _row_strides(*xs), pointers(*[o.data_ptr() for o in outs]),
+                                 (C.c_int64 * (3 * n))(*[s for _, strides in likes for s in strides]), (C.c_int32 * n)(*[t.shape[1] for t in xs]),
+                                 n, positions.data_ptr(), 8 * positions.element_size(),
+                                 (C.c_int64 * 3)(positions.stride(0), positions.stride(1) if positions.shape[1] > 1 else 0, positions.stride(2)),
+                                 plan[0], plan[1], positions.shape[0], B, S, D, half, inverse, _dt(x), _stream(x))
+    check(rc, "psa_rotate_axes")
     return outs
 
 
@@ -952,48 +958,19 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     leaves a token as it is.  Angles are exact to 2^-24 turns at any position; values are computed in 32 bits and rounded once.
     Returns the turned copies (q, or (q, k)), in the order of dimensions of their inputs; differentiable in q and k."""
     xs = [q] if k is None else [q, k]
-    sections = tuple(sections)
-    inv_freq = None if inv_freq is None else tuple(float(f) for f in inv_freq)
-    key = ("rotary", q.shape, q.dtype, q.get_device(), k is not None and (k.shape, k.dtype, k.get_device()), positions.shape, positions.dtype,
-           positions.get_device(), sections, theta, layout, per_axis, inv_freq)
-    plan = _PLANS.get(key)
-    if plan is None:
-        plan = _keep(key, _check_rotary(xs, positions, sections, theta, layout, bool(per_axis), inv_freq))
-    if positions.dim() == 2:
-        positions = positions.unsqueeze(1)
-    half = layout == "half"
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        outs = _RotateAxes.apply(positions, plan, half, False, *xs)
-    else:
-        outs = _rotate(xs, positions, plan, half, False)
-    return outs[0] if k is None else tuple(outs)
-
-
-def _check_rotary(xs, positions: torch.Tensor, sections, theta: float, layout: str, per_axis: bool, inv_freq):
-    q = xs[0]
-    if any(x.dim() != 4 for x in xs) or any((x.shape[0], *x.shape[2:]) != (q.shape[0], *q.shape[2:]) or x.dtype != q.dtype for x in xs):
+    if q.dim() != 4:
         raise ValueError("rotate_axes: q [B, H, S, D] and k [B, Hkv, S, D] of one dtype")
-    B, _, S, D = q.shape
-    if D % 16 or not 16 <= D <= 256:
-        raise ValueError(f"rotate_axes: head_dim {D} (a multiple of 16 up to 256)")
-    _dt(q)
-    sections = tuple(int(n) for n in sections)
-    if not 1 <= len(sections) <= 8 or any(n < 0 for n in sections) or sum(sections) != D // 2:
-        raise ValueError(f"rotate_axes: sections {sections} are not {D // 2} channel pairs of 1 to 8 axes")
     if layout not in ("half", "pairs"):
         raise ValueError(f"rotate_axes: layout must be 'half' or 'pairs', got {layout!r}")
-    if inv_freq is not None:
-        if len(inv_freq) != D // 2 or not all(math.isfinite(f) for f in inv_freq):
-            raise ValueError(f"rotate_axes: inv_freq must be {D // 2} finite numbers")
-    elif not (math.isfinite(theta) and theta > 0):
-        raise ValueError(f"rotate_axes: theta must be positive, got {theta}")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"rotate_axes: positions must be int32 or int64, got {positions.dtype}")
-    shape = (positions.shape[0], 1, *positions.shape[1:]) if positions.dim() == 2 else tuple(positions.shape)
-    if len(shape) != 3 or shape[0] != len(sections) or shape[1] not in (1, B) or shape[2] != S:
-        raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{len(sections)}, {B}, {S}]")
-    _device_of(*xs, positions)
-    return _rotary_plan(D, sections, float(theta), per_axis, inv_freq)
+    sections = tuple(map(int, sections))
+    if positions.dim() not in (2, 3) or positions.size(0) != len(sections):
+        raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{len(sections)}, {q.size(0)}, {q.size(2)}]")
+    plan = _rotary_plan(q.size(3), sections, float(theta), bool(per_axis), None if inv_freq is None else tuple(map(float, inv_freq)))
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+        outs = _RotateAxes.apply(positions, plan, layout == "half", False, *xs)
+    else:
+        outs = _rotate(xs, positions, plan, layout == "half", False)
+    return outs[0] if k is None else outs
 
 
 def _state32(name: str, t: torch.Tensor, shape) -> None:
@@ -1008,14 +985,6 @@ def _ints32(name: str, t: torch.Tensor, shape) -> torch.Tensor:
     return t.to(torch.int32).contiguous()
 
 
-def _form(t: torch.Tensor) -> tuple:
-    return t.shape, t.dtype, t.is_contiguous(), t.get_device()
-
-
-def _plain32(t: torch.Tensor) -> bool:
-    return t.dtype == torch.int32 and t.is_contiguous()
-
-
 def plan_pages(table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, pool: torch.Tensor, free: torch.Tensor, page_size: int,
                tokens: int, out=None):
     """Room for counts[b] (0 .. tokens) more tokens of every request of a cache in pages, without the host knowing any length.
@@ -1026,32 +995,28 @@ def plan_pages(table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
     check_status() says so.  Returns (table, lengths, free, slots): the state after it, and int32 [requests, tokens] with the
     slot (page * page_size + place) of each new token, -1 behind a request's last one.  out: (table, lengths, free) to write
     into, the inputs themselves for instance; new tensors otherwise."""
-    key = ("pages", _form(table), _form(lengths), counts.shape, counts.dtype, counts.get_device(), _form(pool), _form(free), page_size, tokens,
-           out and tuple(_form(t) for t in out))
-    plan = _PLANS.get(key)
-    if plan is None:
-        if table.dim() != 2 or pool.dim() != 1 or min(table.shape) < 1 or pool.numel() < 1:
-            raise ValueError("plan_pages: table [requests, width] and pool [n] must not be empty")
-        if page_size < 16 or page_size % 16 or tokens < 1:
-            raise ValueError(f"plan_pages: page_size {page_size} (a multiple of 16), tokens {tokens} (1 or more)")
-        n, width = table.shape
-        index = _device_of(table, lengths, counts, pool, free, *(out or ()))
-        for name, t, shape in (("table", table, (n, width)), ("lengths", lengths, (n,)), ("pool", pool, (pool.numel(),)), ("free", free, (1,)),
-                               *(zip(("out table", "out lengths", "out free"), out, ((n, width), (n,), (1,))) if out else ())):
-            _state32(name, t, shape)
-        _ints32("counts", counts, (n,))
-        nbytes = lib.psa_plan_pages_scratch_bytes(n)
-        plan = _keep(key, (n, nbytes, index, (C.c_size_t(nbytes), C.c_int64(n), C.c_int64(width), C.c_int64(pool.numel()), C.c_int(page_size),
-                                              C.c_int64(tokens), C.c_void_p(status_word(table.device).data_ptr()))))
-    n, nbytes, index, sizes = plan
-    counts = counts if _plain32(counts) else counts.to(torch.int32).contiguous()
+    done = _calls.plan_pages(table, lengths, counts, pool, free, page_size, tokens, out)
+    if done is not None:
+        if type(done) is int:
+            check(done, "psa_plan_pages")
+        return done
+    if table.dim() != 2 or pool.dim() != 1 or min(table.shape) < 1 or pool.numel() < 1:
+        raise ValueError("plan_pages: table [requests, width] and pool [n] must not be empty")
+    if page_size < 16 or page_size % 16 or tokens < 1:
+        raise ValueError(f"plan_pages: page_size {page_size} (a multiple of 16), tokens {tokens} (1 or more)")
+    n, width = table.shape
+    _device_of(table, lengths, counts, pool, free, *(out or ()))
+    for name, t, shape in (("table", table, (n, width)), ("lengths", lengths, (n,)), ("pool", pool, (pool.numel(),)), ("free", free, (1,)),
+                           *(zip(("out table", "out lengths", "out free"), out, ((n, width), (n,), (1,))) if out else ())):
+        _state32(name, t, shape)
+    counts = _ints32("counts", counts, (n,))
+    nbytes = lib.psa_plan_pages_scratch_bytes(n)
     with _on(table):
         t_out, l_out, f_out = out if out is not None else (torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(free))
         slots = torch.empty((n, tokens), dtype=torch.int32, device=table.device)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
-        rc = lib.psa_plan_pages(table.data_ptr(), lengths.data_ptr(), counts.data_ptr(), pool.data_ptr(), free.data_ptr(), t_out.data_ptr(),
-                                l_out.data_ptr(), f_out.data_ptr(), slots.data_ptr(), scratch.data_ptr(), *sizes,
-                                torch._C._cuda_getCurrentRawStream(index))
+        rc = lib.psa_plan_pages(_ptr(table), _ptr(lengths), _ptr(counts), _ptr(pool), _ptr(free), _ptr(t_out), _ptr(l_out), _ptr(f_out), _ptr(slots),
+                                _ptr(scratch), nbytes, n, width, pool.numel(), page_size, tokens, _ptr(status_word(table.device)), _stream(table))
     check(rc, "psa_plan_pages")
     return t_out, l_out, f_out, slots
 
@@ -1099,65 +1064,51 @@ def _kv4_data(data: torch.Tensor, head_dim: int, group: int, dtype: torch.dtype)
     return data
 
 
-def _cache_sizes(data: torch.Tensor, B: int, n: int, D: int, group: int, dtype: torch.dtype) -> tuple:
-    return (C.c_int64(data.shape[0]), C.c_int(data.shape[1]), C.c_int(16 * data.shape[2]), C.c_int64(B), C.c_int64(n), C.c_int(D), C.c_int(group),
-            C.c_int(_DT[dtype]), C.c_void_p(status_word(data.device).data_ptr()))
-
-
 def kv4_append(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, group: int) -> None:
     """Quantises rows k, v [B, Hkv, n, D] (float16 or bfloat16, any strides) to 4 bits and writes them into the cache at slots [B, n]
     (page * page_size + place; -1: nowhere), in place.  Of each group of channels: lowest = min, step = (max - min) / 15 cut off to
     the type, code = (x - lowest) / step rounded; a group with an infinity or a NaN reads as NaN.  The slots of a call are
     different ones (as plan_pages gives them).  No gradient."""
-    key = ("append", _form(data), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), slots.shape, slots.dtype,
-           slots.get_device(), group)
-    plan = _PLANS.get(key)
-    if plan is None:
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-            raise ValueError("kv4_append: k and v [B, Hkv, n, D] of one shape and dtype")
-        B, H, n, D = k.shape
-        _kv4_data(data, D, group, k.dtype)
-        if data.shape[1] != H:
-            raise ValueError(f"kv4_append: rows of {H} heads, a cache of {data.shape[1]}")
-        index = _device_of(data, k, v, slots)
-        _ints32("slots", slots, (B, n))
-        plan = _keep(key, (_in_words(k), _in_words(v), _row_strides(k, v), _cache_sizes(data, B, n, D, group, k.dtype), index, B * n))
-    k_fits, v_fits, strides, sizes, index, rows = plan
-    if rows == 0:
+    rc = _calls.append(data, k, v, slots, group)
+    if rc is not None:
+        return check(rc, "psa_kv4_append")
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("kv4_append: k and v [B, Hkv, n, D] of one shape and dtype")
+    B, H, n, D = k.shape
+    _kv4_data(data, D, group, k.dtype)
+    if data.shape[1] != H:
+        raise ValueError(f"kv4_append: rows of {H} heads, a cache of {data.shape[1]}")
+    _device_of(data, k, v, slots)
+    slots = _ints32("slots", slots, (B, n))
+    if slots.numel() == 0:
         return
-    if not (k_fits and v_fits) or (k.data_ptr() | v.data_ptr()) & 15:
-        return kv4_append(data, k if k_fits and k.data_ptr() % 16 == 0 else _laid_out(k), v if v_fits and v.data_ptr() % 16 == 0 else _laid_out(v),
-                          slots, group)
-    slots = slots if _plain32(slots) else slots.to(torch.int32).contiguous()
+    k, v = (x if _in_words(x) and x.data_ptr() % 16 == 0 else _laid_out(x) for x in (k, v))
     with _on(data):
-        rc = lib.psa_kv4_append(data.data_ptr(), k.data_ptr(), v.data_ptr(), strides, slots.data_ptr(), *sizes,
-                                torch._C._cuda_getCurrentRawStream(index))
+        rc = lib.psa_kv4_append(_ptr(data), _ptr(k), _ptr(v), _row_strides(k, v), _ptr(slots), data.shape[0], H, 16 * data.shape[2], B, n, D, group,
+                                _DT[k.dtype], _ptr(status_word(data.device)), _stream(data))
     check(rc, "psa_kv4_append")
 
 
 def kv4_read(data: torch.Tensor, slots: torch.Tensor, head_dim: int, group: int, dtype: torch.dtype):
     """The keys and values that slots [B, n] of the cache hold, as two [B, Hkv, n, D] tensors of dtype (that of the rows which were
     appended); zeros where a slot is -1."""
-    key = ("read", _form(data), slots.shape, slots.dtype, slots.get_device(), head_dim, group, dtype)
-    plan = _PLANS.get(key)
-    if plan is None:
-        _kv4_data(data, head_dim, group, dtype)
-        if slots.dim() != 2:
-            raise ValueError("kv4_read: slots [B, n]")
-        index = _device_of(data, slots)
-        B, n = slots.shape
-        _ints32("slots", slots, (B, n))
-        shape = (B, data.shape[1], n, head_dim)
-        like = torch.empty(shape, dtype=dtype, device="meta")
-        plan = _keep(key, (shape, _row_strides(like, like), _cache_sizes(data, B, n, head_dim, group, dtype), index, B * n))
-    shape, strides, sizes, index, rows = plan
+    got = _calls.read(data, slots, head_dim, group, _DT.get(dtype))
+    if got is not None:
+        if type(got) is int:
+            check(got, "psa_kv4_read")
+        return got
+    _kv4_data(data, head_dim, group, dtype)
+    if slots.dim() != 2:
+        raise ValueError("kv4_read: slots [B, n]")
+    _device_of(data, slots)
+    B, n = slots.shape
+    slots = _ints32("slots", slots, (B, n))
+    k, v = (torch.empty((B, data.shape[1], n, head_dim), dtype=dtype, device=data.device) for _ in range(2))
+    if slots.numel() == 0:
+        return k, v
     with _on(data):
-        k, v = torch.empty(shape, dtype=dtype, device=data.device), torch.empty(shape, dtype=dtype, device=data.device)
-        if rows == 0:
-            return k, v
-        slots = slots if _plain32(slots) else slots.to(torch.int32).contiguous()
-        rc = lib.psa_kv4_read(data.data_ptr(), k.data_ptr(), v.data_ptr(), strides, slots.data_ptr(), *sizes,
-                              torch._C._cuda_getCurrentRawStream(index))
+        rc = lib.psa_kv4_read(_ptr(data), _ptr(k), _ptr(v), _row_strides(k, v), _ptr(slots), data.shape[0], data.shape[1], 16 * data.shape[2], B, n,
+                              head_dim, group, _DT[dtype], _ptr(status_word(data.device)), _stream(data))
     check(rc, "psa_kv4_read")
     return k, v
 
@@ -1173,41 +1124,33 @@ def kv4_attention(q: torch.Tensor, data: torch.Tensor, table: torch.Tensor, leng
     Returns [B, H, n, D] in q's order of dimensions, with return_lse also the logarithms of the sums, float32 [B, H, n] (-inf for a
     row of nothing).  No gradient."""
     sm_scale = sm_scale if sm_scale is None else float(sm_scale)
-    key = ("attend", q.shape, q.stride(), q.dtype, q.get_device(), _form(data), _form(table), _form(lengths),
-           counts is not None and (counts.shape, counts.dtype, counts.get_device()), group, sm_scale)
-    plan = _PLANS.get(key)
-    if plan is None:
-        if q.dim() != 4:
-            raise ValueError("kv4_attention: q [B, H, n, D]")
-        B, H, n, D = q.shape
-        _kv4_data(data, D, group, q.dtype)
-        if H < 1 or H % data.shape[1]:
-            raise ValueError(f"kv4_attention: {H} query heads on {data.shape[1]} key heads")
-        if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1:
-            raise ValueError(f"kv4_attention: table [{B}, width]")
-        index = _device_of(q, data, table, lengths, counts)
-        _state32("table", table, table.shape), _state32("lengths", lengths, (B,))
-        if counts is not None:
-            _ints32("counts", counts, (B,))
-        fits = _in_words(q)
-        like, out_strides = _rows_like(q if fits else _laid_out(q))
-        nbytes = lib.psa_kv4_attention_scratch_bytes(B, n, H, data.shape[1], D)
-        plan = _keep(key, (fits, _row_strides(q), like, out_strides, (B, H, n), nbytes, index,
-                           (C.c_size_t(nbytes), C.c_int64(data.shape[0]), C.c_int(16 * data.shape[2]), C.c_int64(table.shape[1]), C.c_int64(B),
-                            C.c_int64(n), C.c_int(H), C.c_int(data.shape[1]), C.c_int(D), C.c_int(group),
-                            C.c_float(D ** -0.5 if sm_scale is None else sm_scale), C.c_int(_DT[q.dtype]),
-                            C.c_void_p(status_word(q.device).data_ptr()))))
-    fits, strides, like, out_strides, shape, nbytes, index, sizes = plan
-    if not fits or q.data_ptr() & 15:
-        return kv4_attention(_laid_out(q), data, table, lengths, group, counts, sm_scale, return_lse)
+    done = _calls.attend(q, data, table, lengths, group, counts, sm_scale, bool(return_lse))
+    if done is not None:
+        if type(done) is int:
+            check(done, "psa_kv4_attention")
+        return done if return_lse else done[0]
+    if q.dim() != 4:
+        raise ValueError("kv4_attention: q [B, H, n, D]")
+    B, H, n, D = q.shape
+    _kv4_data(data, D, group, q.dtype)
+    if H < 1 or H % data.shape[1]:
+        raise ValueError(f"kv4_attention: {H} query heads on {data.shape[1]} key heads")
+    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1:
+        raise ValueError(f"kv4_attention: table [{B}, width]")
+    _device_of(q, data, table, lengths, counts)
+    _state32("table", table, table.shape), _state32("lengths", lengths, (B,))
+    counts = None if counts is None else _ints32("counts", counts, (B,))
+    if not _in_words(q) or q.data_ptr() % 16:
+        q = _laid_out(q)
+    like, out_strides = _rows_like(q)
+    nbytes = lib.psa_kv4_attention_scratch_bytes(B, n, H, data.shape[1], D)
     with _on(q):
         out = _new_rows(q, like)
-        lse = torch.empty(shape, dtype=torch.float32, device=q.device) if return_lse else None
+        lse = torch.empty((B, H, n), dtype=torch.float32, device=q.device) if return_lse else None
         if nbytes:
-            if counts is not None and not _plain32(counts):
-                counts = counts.to(torch.int32).contiguous()
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            rc = lib.psa_kv4_attention(q.data_ptr(), strides, data.data_ptr(), table.data_ptr(), lengths.data_ptr(), _ptr(counts), out.data_ptr(),
-                                       out_strides, _ptr(lse), scratch.data_ptr(), *sizes, torch._C._cuda_getCurrentRawStream(index))
+            rc = lib.psa_kv4_attention(_ptr(q), _row_strides(q), _ptr(data), _ptr(table), _ptr(lengths), _ptr(counts), _ptr(out), out_strides, _ptr(lse),
+                                       _ptr(scratch), nbytes, data.shape[0], 16 * data.shape[2], table.shape[1], B, n, H, data.shape[1], D, group,
+                                       D ** -0.5 if sm_scale is None else sm_scale, _DT[q.dtype], _ptr(status_word(q.device)), _stream(q))
             check(rc, "psa_kv4_attention")
     return (out, lse) if return_lse else out
