@@ -21,10 +21,15 @@ struct CacheArgs {
   int heads, page;
 };
 
-// A quotient of which only the rounded value counts: the product with the inverse, corrected by its remainder (Markstein, IBM Journal of
-// Research and Development 34, 1990: the quotient rounded to nearest, if the inverse is and nothing leaves the normal range).  With
-// a division for each value their special function units bound the kernel.  The sum with 1.5 * 2^23 rounds to whole numbers.
-constexpr float kTiny = 8.673617379884035e-19f, kRound = 12582912.f;   // 2^-60
+// A quotient of which only the rounded value counts, as a product with the inverse.  The inverse is off by 2^-24 of itself at most, the
+// product by less than 2^-20; the sum with 24 rounds that to steps of 2^-19 or 2^-18, so that a tie is one again, and the sum with
+// 1.5 * 2^23 rounds to whole numbers, ties to even.  (What lies within 2^-19 of a tie counts as one; value - lowest in 32 bits is
+// off by 2^-21 already.)  With a division for each value their special function units bound the kernel: 77 us for what takes 24.
+constexpr float kTies = 24.f, kRound = 12582912.f;
+// Steps for which that holds, and which the type cuts off by less than 1/30 of themselves: 15 is the largest code by itself.
+template <typename T> constexpr float kLeastStep = 8.673617379884035e-19f;   // 2^-60
+template <> constexpr float kLeastStep<__half> = 6.103515625e-05f;           // 2^-14
+constexpr float kMostStep = 1.152921504606847e18f;                           // 2^60
 
 // Largest number of the type that is not above x >= 0 (a NaN stays one).
 __device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
@@ -45,33 +50,56 @@ template <> struct Pair<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat162 base() { return __float2bfloat162_rn(128.f); }
 };
 
-constexpr int kHeads = 4;   // heads of a token that a thread takes, their loads in flight together
+constexpr int kRows = 4;   // rows that a thread takes, their loads in flight together
 
-// D/8 threads hold a row, 8 neighbouring channels each, and take kHeads heads of its token; blockIdx.z: keys or values.
-template <int D, int G>
-struct Place {
-  int u, head0, heads, slot;
-  uint32_t row, b, t;
-  uint8_t* slice;        // of head0; further heads lie `apart` bytes on
-  int64_t apart;
+// D/8 threads hold a row, 8 neighbouring channels each; blockIdx.z: keys or values.  A thread's rows are four heads of a token (HS 2), or,
+// where there are fewer heads, both heads of two tokens (1) or the one head of four (0).
+struct Slot {
+  int place;         // in its slice
+  int64_t slice;     // byte offset of head 0's slice
   bool in, good;
-  __device__ __forceinline__ Place(const CacheArgs& a) {
-    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
-    u = i % (D / 8);
-    row = blockIdx.x * (256 / (D / 8)) + threadIdx.x / (D / 8);
+  __device__ __forceinline__ Slot(const CacheArgs& a, uint32_t row, int slice_bytes) {
     in = row < (uint32_t)a.batch * (uint32_t)a.tokens;
-    head0 = blockIdx.y * kHeads;
-    heads = min(kHeads, a.heads - head0);
-    if (!in) row = 0;
-    b = row / (uint32_t)a.tokens;
-    t = row - b * (uint32_t)a.tokens;
-    slot = a.slots[row];
+    const int slot = a.slots[in ? row : 0];
     good = in && slot >= 0 && slot < a.slots_total;
     if (in && !good && slot != -1) *a.status = PSA_ERR_ARG;
-    const int page = good ? slot / a.page : 0, at = good ? slot - page * a.page : 0, slices = a.page / 16;
-    apart = (int64_t)slices * Kv4<D, G>::kSlice;
-    slice = a.data + ((int64_t)page * a.heads + head0) * apart + at / 16 * Kv4<D, G>::kSlice;
+    const int page = good ? slot / a.page : 0, at = good ? slot - page * a.page : 0;
+    slice = ((int64_t)page * a.heads * (a.page / 16) + at / 16) * slice_bytes;
+    place = at & 15;
   }
+};
+template <int D, int G, int HS>
+struct Rows {
+  static constexpr int kHeads = 1 << HS, kTokens = kRows >> HS;
+  int u, head0;
+  int64_t apart, stride, slice_[kTokens], at_[kTokens];
+  int place_[kTokens], heads;
+  bool in_[kTokens], good_[kTokens];
+  __device__ __forceinline__ Rows(const CacheArgs& a) {
+    const int64_t* strides = a.stride[blockIdx.z];
+    u = threadIdx.x % (D / 8);
+    head0 = blockIdx.y * kHeads;
+    heads = a.heads - head0;
+    apart = (int64_t)(a.page / 16) * Kv4<D, G>::kSlice;
+    stride = strides[1];
+    const uint32_t row = (blockIdx.x * (256 / (D / 8)) + threadIdx.x / (D / 8)) * kTokens;
+    uint32_t b = row / (uint32_t)a.tokens, t = row - b * (uint32_t)a.tokens;
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const Slot s(a, row + k, Kv4<D, G>::kSlice);
+      place_[k] = s.place;
+      in_[k] = s.in;
+      good_[k] = s.good;
+      slice_[k] = s.slice + head0 * apart;
+      at_[k] = b * strides[0] + t * strides[2] + head0 * stride + u * 8;
+      if (++t == (uint32_t)a.tokens) t = 0, ++b;
+    }
+  }
+  __device__ __forceinline__ bool in(int j) const { return in_[j >> HS] && j % kHeads < heads; }
+  __device__ __forceinline__ bool good(int j) const { return good_[j >> HS] && j % kHeads < heads; }
+  __device__ __forceinline__ int place(int j) const { return place_[j >> HS]; }
+  __device__ __forceinline__ int64_t slice(int j) const { return slice_[j >> HS] + j % kHeads * apart; }
+  __device__ __forceinline__ int64_t at(int j) const { return at_[j >> HS] + j % kHeads * stride; }
 };
 
 // Values lie in 16-bit units, and the unit that follows one in memory is of the channels 32 further on: the thread four lanes up holds
@@ -81,82 +109,108 @@ __device__ __forceinline__ uint32_t swap_units(uint32_t codes, bool odd) {
   return odd ? other | (codes & 0xffff0000u) : (codes & 0xffffu) | other << 16;
 }
 
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const CacheArgs a) {
+template <typename T, int D, int G, int HS>
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(const CacheArgs a) {
   using L = Kv4<D, G>;
+  using T2 = typename Pair<T>::type;
   const int z = blockIdx.z;
-  const Place<D, G> at(a);
-  uint4 w[kHeads];
-  const T* src = static_cast<const T*>(a.src[z]) + at.b * a.stride[z][0] + at.head0 * a.stride[z][1] + at.t * a.stride[z][2] + at.u * 8;
+  const Rows<D, G, HS> to(a);
+  uint4 w[kRows];
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h)
-    w[h] = at.good && h < at.heads ? __ldg(reinterpret_cast<const uint4*>(src + h * a.stride[z][1])) : make_uint4(0, 0, 0, 0);
-  const int r = at.slot & 15, g = at.u * 8 / G;
-  const bool odd = at.u >> 2 & 1;
+  for (int j = 0; j < kRows; ++j)
+    w[j] = to.good(j) ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.src[z]) + to.at(j))) : make_uint4(0, 0, 0, 0);
+  // lowest and negated highest value of a group, two numbers in a word; a NaN stays one
+  uint32_t ends[kRows];
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    using T2 = typename Pair<T>::type;
-    const T2* e = reinterpret_cast<const T2*>(&w[h]);
-    // lowest and negated highest value, two numbers in a word; a NaN stays one
+  for (int j = 0; j < kRows; ++j) {
+    const T2* e = reinterpret_cast<const T2*>(&w[j]);
     T2 low = __hmin2_nan(__hmin2_nan(e[0], e[1]), __hmin2_nan(e[2], e[3])), high = __hmax2_nan(__hmax2_nan(e[0], e[1]), __hmax2_nan(e[2], e[3]));
     low = Pair<T>::make(__hmin_nan(low.x, low.y), __hneg(__hmax_nan(high.x, high.y)));
 #pragma unroll
     for (int d = 1; d < G / 8; d *= 2) low = __hmin2_nan(low, __shfl_xor_sync(~0u, low, d));
-    const float lo = Elem<T>::to_f(low.x), wide = (-Elem<T>::to_f(low.y) - lo) / 15.f;
-    T step = cut_off(wide, T());
+    ends[j] = *reinterpret_cast<const uint32_t*>(&low);
+  }
+  // Every lane of a group knows them by now: of four neighbours each does one row's divisions.
+  const int lane = threadIdx.x & 31, own = lane & 3;
+  uint32_t pair;
+  float inverse;   // 0: not for the product with it
+  {
+    const uint32_t x = own & 2 ? (own & 1 ? ends[3] : ends[2]) : (own & 1 ? ends[1] : ends[0]);
+    const bool skip = !(own & 2 ? (own & 1 ? to.good(3) : to.good(2)) : (own & 1 ? to.good(1) : to.good(0)));
+    const T2 low = *reinterpret_cast<const T2*>(&x);
     T lowest = low.x;
+    const float wide = (-Elem<T>::to_f(low.y) - Elem<T>::to_f(lowest)) / 15.f;
+    T step = cut_off(wide, T());
     const float s = Elem<T>::to_f(step);
-    uint32_t codes = 0;
-    if (!isfinite(wide)) {   // an infinity or a NaN among them, or a range beyond 32 bits
-      step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));
-    } else if (s > kTiny && s < 1.f / kTiny) {
-      const float inverse = 1.f / s;
-      // a rounded quotient's bits are those of 1.5 * 2^23 plus the code: their sum with weights 16^j, less what the constant makes
+    if (!isfinite(wide)) step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));   // an infinity or a NaN among them, or a range beyond 32 bits
+    inverse = skip ? 1.f : s >= kLeastStep<T> && s < kMostStep && isfinite(wide) ? __frcp_rn(s) : 0.f;
+    const T2 both = Pair<T>::make(step, lowest);
+    pair = *reinterpret_cast<const uint32_t*>(&both);
+  }
+  uint32_t pairs[kRows], codes[kRows];
+  bool plain = true;
 #pragma unroll
-      for (int j = 7; j >= 0; --j) {
-        const float d = Elem<T>::to_f(j & 1 ? e[j / 2].y : e[j / 2].x) - lo, q0 = d * inverse, q = fmaf(fmaf(-q0, s, d), inverse, q0);
-        codes = codes * 16u + __float_as_uint(fminf(q, 15.f) + kRound);
+  for (int j = 0; j < kRows; ++j) {
+    pairs[j] = __shfl_sync(~0u, pair, (lane & ~3) | j);
+    const float inv = __shfl_sync(~0u, inverse, (lane & ~3) | j);
+    plain = plain && inv != 0.f;
+    const T2* e = reinterpret_cast<const T2*>(&w[j]);
+    const float lo = Elem<T>::to_f(reinterpret_cast<const T2*>(&pairs[j])->y);
+    // a rounded quotient's bits are those of 1.5 * 2^23 plus the code: their sum with weights 16^i, less what the constant makes
+    codes[j] = 0u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = Elem<T>::to_f(i & 1 ? e[i / 2].y : e[i / 2].x) - lo;
+      codes[j] += __float_as_uint(fmaf(x, inv, kTies) + (kRound - kTies)) << (4 * i);
+    }
+  }
+  if (!plain) {   // some group's step is none, or nearly none, or far beyond any that counts
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const T2 p = *reinterpret_cast<const T2*>(&pairs[j]);
+      const T* e = reinterpret_cast<const T*>(&w[j]);
+      const float s = Elem<T>::to_f(p.x), lo = Elem<T>::to_f(p.y);
+      codes[j] = 0;
+      if (s > 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) codes[j] |= (__float_as_uint(fminf((Elem<T>::to_f(e[i]) - lo) / s, 15.f) + kRound) & 15u) << (4 * i);
       }
-      codes -= 0x4b400000u * 0x11111111u;
-    } else if (s > 0.f) {
-#pragma unroll 1
-      for (int j = 0; j < 8; ++j)
-        codes |= (__float_as_uint(fminf((Elem<T>::to_f(reinterpret_cast<const T*>(e)[j]) - lo) / s, 15.f) + kRound) & 15u) << (4 * j);
     }
-    if (z) codes = swap_units(codes, odd);
-    if (!at.good || h >= at.heads) continue;
-    uint8_t* slice = at.slice + h * at.apart;
+  }
+  const int g = to.u * 8 / G;
+  const bool odd = to.u >> 2 & 1;
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) {
+    if (z) codes[j] = swap_units(codes[j], odd);
+    if (!to.good(j)) continue;
     // after the swap an even block's thread has the units of channels 8 u and 8 u + 32, an odd one's those of 8 u - 28 and 8 u + 4
-    const int place = z ? L::v_unit(r, odd ? at.u * 8 - 28 : at.u * 8) : L::k_word(r, at.u * 8);
-    *reinterpret_cast<uint32_t*>(slice + place) = codes;
-    if (at.u * 8 % G == 0) {
-      T pair[2] = {step, lowest};
-      *reinterpret_cast<uint32_t*>(slice + (z ? L::v_param(r, g) : L::k_param(r, g))) = *reinterpret_cast<const uint32_t*>(pair);
-    }
+    const int place = z ? L::v_unit(to.place(j), odd ? to.u * 8 - 28 : to.u * 8) : L::k_word(to.place(j), to.u * 8);
+    uint8_t* slice = a.data + to.slice(j);
+    *reinterpret_cast<uint32_t*>(slice + place) = codes[j];
+    if (to.u * 8 % G == 0) *reinterpret_cast<uint32_t*>(slice + (z ? L::v_param(to.place(j), g) : L::k_param(to.place(j), g))) = pairs[j];
   }
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, int HS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const CacheArgs a) {
   using L = Kv4<D, G>;
   const int z = blockIdx.z;
-  const Place<D, G> at(a);
-  const int r = at.slot & 15, g = at.u * 8 / G;
-  const bool odd = at.u >> 2 & 1;
-  uint32_t codes[kHeads], pair[kHeads];
-  const int place = z ? L::v_unit(r, odd ? at.u * 8 - 28 : at.u * 8) : L::k_word(r, at.u * 8), params = z ? L::v_param(r, g) : L::k_param(r, g);
+  const Rows<D, G, HS> from(a);
+  const int g = from.u * 8 / G;
+  const bool odd = from.u >> 2 & 1;
+  uint32_t codes[kRows], pair[kRows];
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    const bool load = at.good && h < at.heads;
-    codes[h] = load ? *reinterpret_cast<const uint32_t*>(at.slice + h * at.apart + place) : 0u;
-    pair[h] = load ? *reinterpret_cast<const uint32_t*>(at.slice + h * at.apart + params) : 0u;
+  for (int j = 0; j < kRows; ++j) {
+    const int r = from.place(j), place = z ? L::v_unit(r, odd ? from.u * 8 - 28 : from.u * 8) : L::k_word(r, from.u * 8);
+    const uint8_t* slice = a.data + from.slice(j);
+    codes[j] = from.good(j) ? *reinterpret_cast<const uint32_t*>(slice + place) : 0u;
+    pair[j] = from.good(j) ? *reinterpret_cast<const uint32_t*>(slice + (z ? L::v_param(r, g) : L::k_param(r, g))) : 0u;
   }
-  T* dst = static_cast<T*>(a.dst[z]) + at.b * a.stride[z][0] + at.head0 * a.stride[z][1] + at.t * a.stride[z][2] + at.u * 8;
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    const uint32_t n = z ? swap_units(codes[h], odd) : codes[h];
+  for (int j = 0; j < kRows; ++j) {
+    const uint32_t n = z ? swap_units(codes[j], odd) : codes[j];
     using T2 = typename Pair<T>::type;
-    const T2 p = *reinterpret_cast<const T2*>(&pair[h]), step = Pair<T>::make(p.x, p.x), lowest = Pair<T>::make(p.y, p.y);
+    const T2 p = *reinterpret_cast<const T2*>(&pair[j]), step = Pair<T>::make(p.x, p.x), lowest = Pair<T>::make(p.y, p.y);
     uint32_t y[4];   // channels i and i + 4: lowest + code * step, rounded once
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -166,7 +220,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const CacheArgs a) {
     }
     const uint4 w = make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
                                __byte_perm(y[2], y[3], 0x7632));
-    if (at.in && h < at.heads) *reinterpret_cast<uint4*>(dst + h * a.stride[z][1]) = w;
+    if (from.in(j)) *reinterpret_cast<uint4*>(static_cast<T*>(a.dst[z]) + from.at(j)) = w;
   }
 }
 
@@ -183,6 +237,8 @@ int check(const char* what, const void* data, const void* k, const void* v, cons
   for (int i = 0; i < 6; ++i) PSA_REQUIRE(strides[i] % 8 == 0, PSA_ERR_ARG, "%s: strides must be multiples of 8 elements", what);
   return PSA_OK;
 }
+
+int heads_shift(int heads) { return heads >= 3 ? 2 : heads - 1; }
 
 CacheArgs arguments(const void* data, const int64_t* strides, const int32_t* slots, int64_t pages, int heads, int page, int64_t batch,
                     int64_t tokens, int32_t* status) {
@@ -213,8 +269,11 @@ extern "C" int psa_kv4_append(void* data, const void* k, const void* v, const in
   CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, batch, tokens, status);
   a.src[0] = k;
   a.src[1] = v;
-  const dim3 grid((unsigned)cdiv64(batch * tokens, 256 / (head_dim / 8)), (unsigned)cdiv64(kv_heads, kHeads), 2);
-  PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_append_kernel<T, D, G><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
+  const int hs = heads_shift(kv_heads);
+  const dim3 grid((unsigned)cdiv64(batch * tokens, (256 / (head_dim / 8)) << (2 - hs)), (unsigned)cdiv64(kv_heads, 1 << hs), 2);
+  if (hs == 2) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_append_kernel<T, D, G, 2><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
+  else if (hs == 1) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_append_kernel<T, D, G, 1><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
+  else PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_append_kernel<T, D, G, 0><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
   PSA_CHECK_LAUNCH("psa_kv4_append");
   return PSA_OK;
 }
@@ -226,8 +285,11 @@ extern "C" int psa_kv4_read(const void* data, void* k, void* v, const int64_t* s
   CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, batch, tokens, status);
   a.dst[0] = k;
   a.dst[1] = v;
-  const dim3 grid((unsigned)cdiv64(batch * tokens, 256 / (head_dim / 8)), (unsigned)cdiv64(kv_heads, kHeads), 2);
-  PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_read_kernel<T, D, G><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
+  const int hs = heads_shift(kv_heads);
+  const dim3 grid((unsigned)cdiv64(batch * tokens, (256 / (head_dim / 8)) << (2 - hs)), (unsigned)cdiv64(kv_heads, 1 << hs), 2);
+  if (hs == 2) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_read_kernel<T, D, G, 2><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
+  else if (hs == 1) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_read_kernel<T, D, G, 1><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
+  else PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, kv4_read_kernel<T, D, G, 0><<<grid, 256, 0, (cudaStream_t)stream>>>(a));
   PSA_CHECK_LAUNCH("psa_kv4_read");
   return PSA_OK;
 }

@@ -3,9 +3,9 @@
 //
 // Channel pair i of token (b, t) is turned by the angle pos[axis(i)][b][t] * freq(i).  The angle is kept in turns as a 64-bit
 // fraction: turns(i) = freq(i) / 2 pi * 2^64 comes from the host, the product with the position is taken modulo 2^64 - whole turns
-// drop out of an integer product by themselves - and its upper half, as a signed number of 2^-32 turns, goes through sincospif.
-// The error is |pos| * 2^-65 turns plus the rounding of that number to 24 bits (2^-25 half turns), at any position a model reaches;
-// pos * freq in 32 bits is off by 2^-25 * pos radians (0.004 at position 131072).
+// drop out of an integer product by themselves - and its upper half, a signed number of 2^-32 turns, gives the nearest quarter turn
+// and what is left of it, at most an eighth.  The error is |pos| * 2^-65 turns plus a few roundings of sine and cosine, at any position
+// a model reaches; pos * freq in 32 bits is off by 2^-25 * pos radians (0.004 at position 131072).
 #include "psa_common.cuh"
 
 namespace psa {
@@ -37,35 +37,60 @@ template <> __device__ __forceinline__ float* word_of<float>(Word& w) { return w
 template <> __device__ __forceinline__ __half* word_of<__half>(Word& w) { return w.h; }
 template <> __device__ __forceinline__ __nv_bfloat16* word_of<__nv_bfloat16>(Word& w) { return w.b; }
 
+// Sine and cosine of turn * 2^-32 turns.  Taylor's series at |r| <= pi / 4: what follows the last terms is below r^11 / 11! (2 10^-9) and
+// r^10 / 10! (2.5 10^-8, half a rounding of a cosine that is above 0.7).
+__device__ __forceinline__ void sine_cosine(int32_t turn, float& sine, float& cosine) {
+  const uint32_t quarter = ((uint32_t)turn + (1u << 29)) >> 30;
+  const float r = (float)(int32_t)((uint32_t)turn - (quarter << 30)) * 1.4629180792671596e-09f;   // 2 pi / 2^32
+  const float x = r * r;
+  const float s = fmaf(r * x, fmaf(x, fmaf(x, fmaf(x, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), r);
+  const float c = fmaf(x, fmaf(x, fmaf(x, fmaf(x, 1.f / 40320, -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const float u = quarter & 1 ? c : s, v = quarter & 1 ? s : c;
+  sine = __uint_as_float(__float_as_uint(u) ^ (quarter & 2) << 30);
+  cosine = __uint_as_float(__float_as_uint(v) ^ ((quarter + 1) & 2) << 30);
+}
+
 // A thread owns V pairs of one token, computes their sines and cosines once and walks the heads with them.  Its two 16-byte words of a
 // row lie half a row apart, so that a warp's words are neighbours, whichever channels make a pair: HALF, channels (i, i + D/2), one of
 // each word; otherwise neighbours (2i, 2i + 1), V/2 pairs in each.
 template <typename T, bool HALF>
-__global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant__ RotaryArgs a, int head_dim, int parts) {
+__global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant__ RotaryArgs a, int head_dim, int heads_each) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int chunks = head_dim / 2 / V;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int chunk = (int)(i % chunks);
-  const int64_t token = i / chunks;
-  if (token >= a.batch * a.seq) return;
-  const int64_t b = token / a.seq, t = token - b * a.seq;
+  // turns and axes to shared memory: lanes that read the kernel's arguments at different places wait for one another
+  __shared__ uint64_t turns_s[kMaxPairs];
+  __shared__ uint8_t axis_s[kMaxPairs];
+  for (int i = threadIdx.x; i < head_dim / 2; i += blockDim.x) {
+    turns_s[i] = a.turns[i];
+    axis_s[i] = a.axis[i];
+  }
+  __syncthreads();
+  const int chunks = head_dim / 2 / V, each = blockDim.x / chunks;   // tokens of a block
+  const int own = threadIdx.x / chunks, chunk = threadIdx.x - own * chunks;
+  const int64_t tokens = a.batch * a.seq, token = (int64_t)blockIdx.x * each + own;
+  if (own >= each || token >= tokens) return;
+  const int64_t b = tokens <= 0xffffffffll ? (uint32_t)token / (uint32_t)a.seq : token / a.seq, t = token - b * a.seq;
+  const int64_t pos_at = b * a.pos_stride[1] + t * a.pos_stride[2];
   float cs[V], sn[V];
+  int64_t p = 0;
+  int axis = -1;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int pair = HALF ? chunk * V + j : chunk * (V / 2) + j % (V / 2) + (j < V / 2 ? 0 : head_dim / 4);
-    const int64_t at = a.axis[pair] * a.pos_stride[0] + b * a.pos_stride[1] + t * a.pos_stride[2];
-    const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : static_cast<const int32_t*>(a.pos)[at];
-    const int32_t turn = (int32_t)(((uint64_t)p * a.turns[pair]) >> 32);
-    sincospif((float)turn * 4.656612873077393e-10f, &sn[j], &cs[j]);   // 2^-31 half turns
+    if (axis_s[pair] != axis) {
+      axis = axis_s[pair];
+      const int64_t at = axis * a.pos_stride[0] + pos_at;
+      p = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : static_cast<const int32_t*>(a.pos)[at];
+    }
+    sine_cosine((int32_t)(((uint64_t)p * turns_s[pair]) >> 32), sn[j], cs[j]);
     if (a.inverse) sn[j] = -sn[j];
   }
   const int first = chunk * V, second = first + head_dim / 2;
-  const int heads = a.heads[0] + a.heads[1];
-  for (int h0 = blockIdx.y; h0 < heads; h0 += kInFlight * parts) {
+  const int heads = min(a.heads[0] + a.heads[1], (int)(blockIdx.y + 1) * heads_each);
+  for (int h0 = blockIdx.y * heads_each; h0 < heads; h0 += kInFlight) {
     Word w0[kInFlight], w1[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const int h = h0 + u * parts;
+      const int h = h0 + u;
       if (h < heads) {
         const int z = h >= a.heads[0], hh = z ? h - a.heads[0] : h;
         const T* src = static_cast<const T*>(a.src[z]) + b * a.src_stride[z][0] + hh * a.src_stride[z][1] + t * a.src_stride[z][2];
@@ -75,7 +100,7 @@ __global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant_
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const int h = h0 + u * parts;
+      const int h = h0 + u;
       if (h >= heads) break;
       T *e0 = word_of<T>(w0[u]), *e1 = word_of<T>(w1[u]);
 #pragma unroll
@@ -96,16 +121,18 @@ __global__ void __launch_bounds__(128) rotary_axes_kernel(const __grid_constant_
 
 template <typename T>
 int launch(const RotaryArgs& a, int head_dim, int half, cudaStream_t st) {
-  const int64_t threads = a.batch * a.seq * (head_dim / 2 / (16 / (int)sizeof(T)));
-  const int64_t blocks = cdiv64(threads, 128);
+  const int64_t blocks = cdiv64(a.batch * a.seq, 128 / (head_dim / 2 / (16 / (int)sizeof(T))));
   PSA_REQUIRE(blocks < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_rotate_axes: too many tokens");
   const int heads = a.heads[0] + a.heads[1];
-  int parts = 1;   // few tokens: the heads are shared out over blocks
-  while (parts < heads && blocks * parts < 148 * 16) parts *= 2;
-  if (parts > heads) parts = heads;
-  const dim3 grid((unsigned)blocks, (unsigned)parts);
-  if (half) rotary_axes_kernel<T, true><<<grid, 128, 0, st>>>(a, head_dim, parts);
-  else rotary_axes_kernel<T, false><<<grid, 128, 0, st>>>(a, head_dim, parts);
+  // A block's heads are neighbours: in token-major tensors their rows are, too.  Few tokens: the heads are shared out over blocks, down
+  // to what a thread loads at once - fewer cost more sines than they hide latency (16 heads of 2536 tokens: 5.2 us by fours, 7.2 one by
+  // one) - or to one, where the GPU would be empty otherwise.
+  int each = heads;
+  while (each > kInFlight && blocks * cdiv64(heads, each) < 148 * 16) each = each > 2 * kInFlight ? (each + 1) / 2 : kInFlight;
+  while (each > 1 && blocks * cdiv64(heads, each) < 148) each = (each + 1) / 2;
+  const dim3 grid((unsigned)blocks, (unsigned)cdiv64(heads, each));
+  if (half) rotary_axes_kernel<T, true><<<grid, 128, 0, st>>>(a, head_dim, each);
+  else rotary_axes_kernel<T, false><<<grid, 128, 0, st>>>(a, head_dim, each);
   PSA_CHECK_LAUNCH("psa_rotate_axes");
   return PSA_OK;
 }
