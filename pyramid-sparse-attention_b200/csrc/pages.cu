@@ -43,15 +43,20 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sums) {   // inclusiv
   return x + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// tokens below 2^31
-__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((uint32_t)tokens + (uint32_t)page - 1u) / (uint32_t)page); }
+// Tokens below 2^31.  Pages of a power of two (shift >= 0) need no division.
+__device__ __forceinline__ int page_of(int token, int page, int shift) { return shift >= 0 ? token >> shift : (int)((uint32_t)token / (uint32_t)page); }
+__device__ __forceinline__ int pages_of(int tokens, int page, int shift) {
+  const uint32_t up = (uint32_t)tokens + (uint32_t)page - 1u;
+  return (int)(shift >= 0 ? up >> shift : up / (uint32_t)page);
+}
 
 struct PlanArgs {
   const int32_t *table, *lengths, *counts, *pool, *free_in;
   int32_t *table_out, *lengths_out, *free_out, *slots, *status;
   Grant* grants;
   int32_t* free_before;
-  int requests, width, pool_size, page, tokens;
+  int requests, width, pool_size, page, tokens, shift;
+  bool fours;   // rows of the table and of the slots are whole 16-byte words
 };
 
 // What a request holds, wants and has a right to want.
@@ -66,8 +71,8 @@ __device__ __forceinline__ Want want_of(const PlanArgs& a, int b) {
   const int64_t most = (int64_t)a.width * a.page;
   w.bad = w.length < 0 || w.length > most || w.count < 0 || w.count > a.tokens || (int64_t)w.length + w.count > most;
   if (w.bad) w.count = 0;
-  w.held = pages_of(min(max(w.length, 0), (int)most), a.page);
-  w.need = w.bad ? 0 : pages_of(w.length + w.count, a.page) - w.held;
+  w.held = pages_of(min(max(w.length, 0), (int)most), a.page, a.shift);
+  w.need = w.bad ? 0 : pages_of(w.length + w.count, a.page, a.shift) - w.held;
   return w;
 }
 __device__ __forceinline__ Grant grant_of(const PlanArgs& a, const Want& w, int total, int available) {
@@ -76,33 +81,46 @@ __device__ __forceinline__ Grant grant_of(const PlanArgs& a, const Want& w, int 
   return {w.held, served ? w.need : 0, total - w.need, served ? w.count : 0, w.length};
 }
 
-// Entries [from, to) of a request's row of the table and of its slots.
-__device__ __forceinline__ void fill_row(const PlanArgs& a, int b, const Grant& g, int available, int from, int to, int step) {
-  const int top = available - 1 - g.first, shift = a.page & (a.page - 1) ? -1 : 31 - __clz(a.page), most_pages = 0x7fffffff / a.page;
-  const int32_t* table = a.table + (int64_t)b * a.width;
-  int32_t* table_out = a.table_out + (int64_t)b * a.width;
-  int32_t* slots = a.slots + (int64_t)b * a.tokens;
-#pragma unroll 4
-  for (int j = from; j < to; j += step) {
-    if (j < a.width) {
-      const bool fresh = j >= g.held && j < g.held + g.given;
-      if (fresh || table_out != table) table_out[j] = fresh ? a.pool[top - (j - g.held)] : table[j];
-    }
-    if (j < a.tokens) {
-      int slot = -1;
-      if (j < g.tokens) {
-        const int at = g.length + j, k = shift >= 0 ? at >> shift : (int)((uint32_t)at / (uint32_t)a.page);
-        const int p = k < g.held ? table[k] : a.pool[top - (k - g.held)];
-        if (p >= 0 && p < most_pages) slot = p * a.page + (at - k * a.page);
-      }
-      slots[j] = slot;
+// Entries [from, to) of a row, four neighbours a thread (`own` of `threads`), as `value` gives them.
+template <typename F>
+__device__ __forceinline__ void fill(int32_t* row, bool fours, int from, int to, int own, int threads, F value) {
+  for (int j = (from & ~3) + 4 * own; j < to; j += 4 * threads) {
+    int x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = j + i >= from && j + i < to ? value(j + i) : 0;
+    if (fours && j >= from && j + 3 < to) {
+      *reinterpret_cast<int4*>(row + j) = make_int4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i >= from && j + i < to) row[j + i] = x[i];
     }
   }
 }
 
+// Part [from, to) of a request's row of the table - in place, of its new pages only - and of its slots.
+__device__ __forceinline__ void fill_row(const PlanArgs& a, int b, const Grant& g, int available, int from, int to, int own, int threads) {
+  const int top = available - 1 - g.first, most_pages = 0x7fffffff / a.page;
+  const int32_t* table = a.table + (int64_t)b * a.width;
+  int32_t* table_out = a.table_out + (int64_t)b * a.width;
+  const bool in_place = table_out == table;
+  fill(table_out, a.fours, in_place ? max(from, g.held) : from, min(to, in_place ? g.held + g.given : a.width), own, threads,
+       [&](int j) { return j >= g.held && j < g.held + g.given ? a.pool[top - (j - g.held)] : table[j]; });
+  int last = -1, page = -1;   // the page looked up before
+  fill(a.slots + (int64_t)b * a.tokens, a.fours, from, min(to, a.tokens), own, threads, [&](int j) {
+    if (j >= g.tokens) return -1;
+    const int at = g.length + j, k = page_of(at, a.page, a.shift);
+    if (k != last) {
+      last = k;
+      page = k < g.held ? table[k] : a.pool[top - (k - g.held)];
+    }
+    return page >= 0 && page < most_pages ? page * a.page + (at - k * a.page) : -1;
+  });
+}
+
 // Outputs beside the inputs, up to kPlanThreads requests: a block fills a stretch of a request's row and sums the needs of the requests
 // before it for itself - a few hundred numbers that all blocks find in L2 - which spares a launch that would do nothing else.
-constexpr int kRowThreads = 256, kRowEntries = 1024;
+constexpr int kRowThreads = 256, kRowEntries = 4096;
 __global__ void __launch_bounds__(kRowThreads) plan_rows_kernel(const PlanArgs a) {
   __shared__ int warp_sums[32], taken;
   const int b = blockIdx.y, available = min(max(a.free_in[0], 0), a.pool_size);
@@ -111,7 +129,7 @@ __global__ void __launch_bounds__(kRowThreads) plan_rows_kernel(const PlanArgs a
   block_scan<kRowThreads>(before, warp_sums);
   const Want w = want_of(a, b);
   const Grant g = grant_of(a, w, warp_sums[31] + w.need, available);
-  fill_row(a, b, g, available, blockIdx.x * kRowEntries + threadIdx.x, min((int)(blockIdx.x + 1) * kRowEntries, max(a.width, a.tokens)), kRowThreads);
+  fill_row(a, b, g, available, blockIdx.x * kRowEntries, (blockIdx.x + 1) * kRowEntries, threadIdx.x, kRowThreads);
   if (blockIdx.x) return;
   if (threadIdx.x == 0) a.lengths_out[b] = g.length + g.tokens;
   if (b) return;
@@ -156,8 +174,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       const int n = min(kPlanThreads, a.requests - b0);
       for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {   // a warp a request: its new pages, its slots
         const Grant g = given[i];
-        const int end = max(a.tokens, a.table_out == a.table ? g.held + g.given : a.width);
-        fill_row(a, b0 + i, g, available, threadIdx.x & 31, end, 32);
+        fill_row(a, b0 + i, g, available, 0, max(a.tokens, a.width), threadIdx.x & 31, 32);
       }
       __syncthreads();
     }
@@ -170,8 +187,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
 
 __global__ void __launch_bounds__(kRowThreads) fill_kernel(const PlanArgs a) {
   const int b = blockIdx.y;
-  fill_row(a, b, a.grants[b], *a.free_before, blockIdx.x * kRowEntries + threadIdx.x,
-           min((int)(blockIdx.x + 1) * kRowEntries, max(a.width, a.tokens)), kRowThreads);
+  fill_row(a, b, a.grants[b], *a.free_before, blockIdx.x * kRowEntries, (blockIdx.x + 1) * kRowEntries, threadIdx.x, kRowThreads);
 }
 
 // Pages of the requests marked in `which` go back on top of the pool, the last request's last page first: a request that is given
@@ -185,7 +201,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_kernel(const int32_t* ta
   for (int b0 = 0; b0 < requests; b0 += kPlanThreads) {
     const int b = requests - 1 - (b0 + (int)threadIdx.x);
     int held = 0;
-    if (b >= 0 && which[b]) held = pages_of(min(max(lengths[b], 0), width * page), page);
+    if (b >= 0 && which[b]) held = pages_of(min(max(lengths[b], 0), width * page), page, -1);
     held_of[threadIdx.x] = held;
     end_of[threadIdx.x] = before + block_scan(held, warp_sums);
     if (held) lengths[b] = 0;
@@ -227,12 +243,15 @@ extern "C" int psa_plan_pages(const int32_t* table, const int32_t* lengths, cons
   PSA_REQUIRE(table && lengths && counts && pool && free_in && table_out && lengths_out && free_out && slots && scratch && status, PSA_ERR_ARG,
               "psa_plan_pages: null pointer");
   if (int rc = check_sizes("psa_plan_pages", requests, width, pool_size, page_size)) return rc;
-  PSA_REQUIRE(tokens > 0 && tokens < ((int64_t)1 << 31) && scratch_bytes >= psa_plan_pages_scratch_bytes(requests), PSA_ERR_ARG,
+  PSA_REQUIRE(tokens > 0 && tokens <= ((int64_t)1 << 30) && scratch_bytes >= psa_plan_pages_scratch_bytes(requests), PSA_ERR_ARG,
               "psa_plan_pages: %lld tokens, scratch of %zu bytes", (long long)tokens, scratch_bytes);
   cudaStream_t st = (cudaStream_t)stream;
   PlanArgs a = {table, lengths, counts, pool, free_in, table_out, lengths_out, free_out, slots, status,
                 reinterpret_cast<Grant*>(static_cast<char*>(scratch) + 16), static_cast<int32_t*>(scratch), (int)requests, (int)width, (int)pool_size,
-                page_size, (int)tokens};
+                page_size, (int)tokens, -1, false};
+  if ((page_size & (page_size - 1)) == 0)
+    for (a.shift = 0; 1 << a.shift < page_size;) ++a.shift;
+  a.fours = ((((uintptr_t)table_out | (uintptr_t)slots) & 15) | (uintptr_t)(width & 3) | (uintptr_t)(tokens & 3)) == 0;
   const int64_t wide = width > tokens ? width : tokens;
   const dim3 rows((unsigned)cdiv64(wide, kRowEntries), (unsigned)requests);
   const bool apart = lengths_out != lengths && free_out != free_in && table_out != table;

@@ -134,7 +134,7 @@ def test_pages_entries_refuse():
     def call(requests=2, width=4, pool=8, page=16, tokens=1, scratch=10 ** 6, table=P):
         return lib.psa_plan_pages(table, P, P, P, P, P, P, P, P, P, scratch, requests, width, pool, page, tokens, P, None)
     for kw in (dict(requests=0), dict(requests=65536), dict(width=0), dict(width=2 ** 28), dict(pool=0), dict(pool=2 ** 27), dict(page=8), dict(page=0),
-               dict(tokens=0), dict(scratch=8), dict(table=None)):
+               dict(tokens=0), dict(tokens=2 ** 30 + 1), dict(scratch=8), dict(table=None)):
         refused(call(**kw), "psa_plan_pages")
     refused(lib.psa_release_pages(P, P, None, P, P, 2, 4, 8, 16, P, None), "null")
     refused(lib.psa_release_pages(P, P, P, P, P, 2, 4, 8, 17, P, None), "page size 17")
