@@ -21,56 +21,12 @@
 //
 // The bound is the cache's bytes (160 a token and key head at head_dim 128, groups of 32).  mma.sync and not tcgen05: 8 query rows
 // against 128 rows of a tcgen05 tile, and operands that are made in registers; the products take a fifth of a warp's issue slots.
-#include <type_traits>
-
-#include "kv4.cuh"
-#include "mma_sync.cuh"
-#include "tc_common.cuh"
+#include "kv4_attn.cuh"
 
 namespace psa {
 namespace {
 
-struct AttnArgs {
-  const void* q;
-  int64_t q_stride[3], out_stride[3];   // batch, head, token; in elements
-  const uint8_t* data;
-  const int32_t *table, *lengths, *counts;
-  void* out;
-  float* lse;
-  int32_t* status;
-  int64_t pages;
-  int batch, tokens, heads, kv_heads, group, width, page;   // group: query heads of a key head
-  float scale;
-  int least_tiles;     // a block takes at least so many
-  int row_tiles;       // of a request that brings all `tokens`
-  int2* owners;        // [batch][kv_heads][row_tiles]: first and last block of a unit (rows of a tile x a key head)
-  float* parts;        // [blocks][2]: what a block has of a unit that began before it, and of one that goes on behind it
-};
-
-template <typename T>
-__device__ __forceinline__ void write_row(const AttnArgs& a, int b, int head, int i, int d, float4 o, float top, float sum) {
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
-  T* to = static_cast<T*>(a.out) + b * a.out_stride[0] + head * a.out_stride[1] + i * a.out_stride[2] + d;
-  uint2 w;
-  w.x = MmaOp<T>::pack(o.x * f, o.y * f);
-  w.y = MmaOp<T>::pack(o.z * f, o.w * f);
-  *reinterpret_cast<uint2*>(to) = w;
-  if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + head) * a.tokens + i] = sum == 0.f ? -INFINITY : 0.6931471805599453f * (top + log2f(sum));
-}
-
-
-constexpr int kWarps = 4, kThreads = 32 * (kWarps + 1), kTile = 16 * kWarps;
-constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has seen nothing: exp2(-inf - kLowest) is 0
-// A weight is 2^(score - reference).  References are set so that the largest score so far, times the largest step of the values so far, gives
-// 2^kHead, and move when a weight times a step could be 2^kLazy times that: f16 has its full precision from 2^-14 to 2^16, so a
-// weight 2^-21 of the largest is still rounded to 11 bits.
-constexpr float kHead = 7.f, kLazy = 8.f;
-constexpr float kLeastCap = 5.9604644775390625e-8f;   // 2^-24
-// Sums of q are kept in units of scores, 2^-24 of q's operands - in f16, whose numbers end there, 2^12 times that.
-// A weight times a step in one term of 11 bits is as exact as a bf16 output needs (2^-12 of what the codes add, against its 2^-9); an f16
-// output shows it (0.00041 of the output's norm instead of 0.00021), so there it is two terms: 25 products a slice instead of 17.
-template <typename T> constexpr int kWeightTerms = std::is_same<T, __half>::value ? 2 : 1;
-template <typename T> constexpr float kSumScale = std::is_same<T, __half>::value ? 2.44140625e-4f : 1.f;
+constexpr int kThreads = 32 * (kWarps + 1);
 
 template <int D, int G, int NT>
 struct Shape {
@@ -87,141 +43,11 @@ struct Shape {
   static constexpr int64_t kPart = (int64_t)kRows * (D + 2);
 };
 
-// A request's part of the line.  A unit - a key head with up to R rows - counts kUnitCells more than it has tiles: what its rows cost before
-// and after the tiles (33 requests of 17 to 16384 tokens, 16 key heads: 110 us without, the blocks with many short ones last).
-constexpr int kUnitCells = 2;
-struct Span {
-  int rows, row_tiles, tiles, cells, work;
-};
-__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_tile, int& length, int& count) {
-  length = a.lengths[b];
-  count = a.counts ? a.counts[b] : a.tokens;
-  const int most = a.width * a.page;
-  if (length < 0 || length > most || count < 0 || count > a.tokens) {
-    *a.status = PSA_ERR_ARG;
-    length = min(max(length, 0), most);
-    count = min(max(count, 0), a.tokens);
-  }
-  Span s;
-  s.rows = count * a.group;
-  s.row_tiles = (s.rows + rows_per_tile - 1) / rows_per_tile;
-  s.tiles = (length + kTile - 1) / kTile;
-  s.cells = s.tiles ? s.tiles + kUnitCells : 0;
-  s.work = s.cells * s.row_tiles * a.kv_heads;   // the entry point sees to it that the sum over all requests fits 32 bits
-  return s;
-}
-
-// The line is shared out in stretches of `each` cells, the first `longer` of them one longer.
-struct Shares {
-  int blocks, each, longer;
-  __device__ __forceinline__ Shares(int work, int most_blocks, int least) {
-    blocks = min(most_blocks, (work + least - 1) / least);
-    each = blocks ? work / blocks : 0;
-    longer = work - each * blocks;
-  }
-  __device__ __forceinline__ int first(int i) const { return i * each + min(i, longer); }
-  __device__ __forceinline__ int owner(int at) const {
-    const int edge = longer * (each + 1);
-    return at < edge ? at / (each + 1) : longer + (at - edge) / each;
-  }
-};
-
-// The whole line's length, and the request that cell `first(block)` lies in with the place where that begins.  scan: 8 words.
-__device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int* scan, int& request, int& base, Shares& shares) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int length, count, mine = 0;
-  for (int b = threadIdx.x; b < a.batch; b += kThreads) mine += span_of(a, b, rows_per_tile, length, count).work;
-  const int own0 = mine;   // of request threadIdx.x, where there are no more than threads
-  int sum = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int y = __shfl_up_sync(~0u, sum, d);
-    if (lane >= d) sum += y;
-  }
-  if (lane == 31) scan[warp] = sum;
-  __syncthreads();
-  int work = 0;
-#pragma unroll
-  for (int w = 0; w <= kWarps; ++w) work += scan[w];
-  shares = Shares(work, gridDim.x, kUnitCells + a.least_tiles);
-  request = base = 0;
-  if ((int)blockIdx.x >= shares.blocks || a.batch == 1) return work;
-  // whose tile it is: requests in rounds of one a thread
-  const int first = shares.first(blockIdx.x);
-  int before = 0;
-  for (int b0 = 0;; b0 += kThreads) {
-    int own = own0;
-    if (a.batch > kThreads) {
-      const int b = b0 + threadIdx.x;
-      own = b < a.batch ? span_of(a, b, rows_per_tile, length, count).work : 0;
-      sum = own;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int y = __shfl_up_sync(~0u, sum, d);
-        if (lane >= d) sum += y;
-      }
-      __syncthreads();
-      if (lane == 31) scan[warp] = sum;
-      __syncthreads();
-    }
-    int start = before + sum - own;
-#pragma unroll
-    for (int w = 0; w <= kWarps; ++w) {
-      start += w < warp ? scan[w] : 0;
-      before += scan[w];
-    }
-    if (first >= start && first < start + own) {
-      scan[6] = b0 + threadIdx.x;
-      scan[7] = start;
-    }
-    if (before > first) break;
-  }
-  __syncthreads();
-  request = scan[6];
-  base = scan[7];
-  return work;
-}
-
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Codes of nibbles i and i + 4 as two f16 numbers: n 2^-24 for even i, n 2^-20 for odd ones.  (Subnormal numbers: a nibble is a number
-// where it stands, with no exponent to add and no offset to take off again.)
-__device__ __forceinline__ uint32_t codes(uint32_t w, int i) { return (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
-// The same of 15 - n.
-__device__ __forceinline__ uint32_t rest(uint32_t w, int i) { return ~(i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// The same product on an accumulator of zeros.
-template <typename T> __device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
-}
-// step and lowest value of a group
-template <typename T> __device__ __forceinline__ float2 param(uint32_t w);
-template <> __device__ __forceinline__ float2 param<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <> __device__ __forceinline__ float2 param<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-
-template <int N> struct Words { uint32_t w[N]; };
-template <int N> __device__ __forceinline__ Words<N> lds(const uint8_t* p) {
-  Words<N> r;
-  if constexpr (N == 4) *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p);
-  else if constexpr (N == 2) *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(p);
-  else r.w[0] = *reinterpret_cast<const uint32_t*>(p);
-  return r;
-}
-
 // What a warp carries of a unit's rows: operands of q, and per row its reference (log2), sum, output and the share of the output
 // that the groups' middle values give.  Lane 4 r + c: rows of q 8 nt + r as operands, 8 nt + 2 c + {0, 1} as columns.
 template <typename T, int D, int G, int NT>
@@ -406,7 +232,7 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
 }
 
 template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(const __grid_constant__ AttnArgs a) {
   using L = Kv4<D, G>;
   using S = Shape<D, G, NT>;
   using R = Rows<T, D, G, NT>;
@@ -431,117 +257,42 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
   asm volatile("griddepcontrol.launch_dependents;");
   int request, base;
   Shares shares(0, 0, 1);
-  line_of(a, kRows, scan, request, base, shares);
+  line_of<kThreads>(a, kRows, scan, request, base, shares);
   __syncthreads();
   if ((int)blockIdx.x >= shares.blocks) return;
-  const int group = a.group, slices_per_page = a.page / 16;
+  const int group = a.group;
   const bool whole_tiles = a.page % kTile == 0;
   int stage = 0;
   uint32_t phase = 0;
-  int at = shares.first(blockIdx.x);
-  const int last = shares.first(blockIdx.x + 1);
-  for (int b = request; at < last; ++b) {
-    int length, count;
-    const Span span = span_of(a, b, kRows, length, count);
-    const int end = base + span.work;
-    while (at < last && at < end) {
-      const int unit = (at - base) / span.cells, cell = at - base - unit * span.cells, cells = min(span.cells - cell, last - at);
-      const int tile0 = max(cell - kUnitCells, 0), tiles = max(cell + cells - kUnitCells, 0) - tile0;
-      const int unit_at = at - cell;
-      at += cells;
-      if (tiles == 0) continue;
-      const int head = unit / span.row_tiles, row0 = (unit - head * span.row_tiles) * kRows;
+  bool dead = false;   // a wait ran out: nothing is waited for any more, and what is computed does not count
+  Walk walk = {request, base, shares.first(blockIdx.x), shares.first(blockIdx.x + 1)};
+  Piece p;
+  while (walk.next(a, kRows, p)) {
       if (warp == kWarps) {
-        // ------------------------------------------------------------ copies.  A lane looks a page number up for a tile that lies in one piece
-        // (whole: one copy a tile, 32 tiles at a time), or else for a slice (8 tiles at a time)
-        const int slices = (length + 15) / 16, last_slice = min(slices, (tile0 + tiles) * kWarps), stride = whole_tiles ? kWarps : 1;
-        for (int s0 = tile0 * kWarps; s0 < last_slice; s0 += 32 * stride) {
-          const int s = s0 + stride * lane;
-          int64_t from = -1;
-          if (s < last_slice) {
-            const int in_page = s / slices_per_page, page = a.table[(int64_t)b * a.width + in_page];
-            if (page >= 0 && page < a.pages) from = (((int64_t)page * a.kv_heads + head) * slices_per_page + s - in_page * slices_per_page) * L::kSlice;
-            else *a.status = PSA_ERR_ARG;
-          }
-          const uint32_t good = __ballot_sync(~0u, from >= 0);
-          const int n = min(32 * stride, last_slice - s0);
-          for (int k = 0; k < n; k += kWarps) {
-            const bool ok = !*abort_flag && tc::mbar_wait(empty + stage, phase ^ 1, abort_flag);
-            if (__all_sync(~0u, ok)) {
-              const uint32_t in = (1u << min(kWarps, n - k)) - 1;   // the tile's slices
-              uint8_t* to = smem + stage * kWarps * L::kSlice;
-              if (whole_tiles) {
-                if (lane == k / kWarps) {
-                  const int bytes = from >= 0 ? __popc(in) * L::kSlice : 0;
-                  valid[stage] = from >= 0 ? in : 0u;
-                  tc::mbar_arrive_expect_tx(full + stage, bytes);
-                  if (bytes) tc::bulk_load_a(tc::smem_u32(to), a.data + from, bytes, tc::smem_u32(full + stage));
-                }
-              } else {
-                const uint32_t bits = good >> k & in;
-                if (lane == 0) {
-                  valid[stage] = bits;
-                  tc::mbar_arrive_expect_tx(full + stage, __popc(bits) * L::kSlice);
-                }
-                __syncwarp();
-                if (from >= 0 && lane / kWarps == k / kWarps)
-                  tc::bulk_load_a(tc::smem_u32(to + lane % kWarps * L::kSlice), a.data + from, L::kSlice, tc::smem_u32(full + stage));
-              }
-            }
-            if (++stage == kStages) stage = 0, phase ^= 1;
-          }
+        // ------------------------------------------------------------ copies: one a tile where pages hold whole ones, else one a slice
+        const int last_slice = min((p.length + 15) / 16, (p.tile0 + p.tiles) * kWarps);
+        Lookup found;
+        for (int i = 0; i < p.tiles; ++i) {
+          if ((i & (whole_tiles ? 31 : 7)) == 0) found.look(a, p, i, whole_tiles, last_slice);
+          if (!dead && !__all_sync(~0u, tc::mbar_wait(empty + stage, phase ^ 1, abort_flag))) dead = true;
+          if (!dead) found.copy<L::kSlice>(a, i, whole_tiles, last_slice - (p.tile0 + i) * kWarps, smem + stage * kWarps * L::kSlice, full + stage, valid + stage);
+          if (++stage == kStages) stage = 0, phase ^= 1;
         }
       } else {
         // ------------------------------------------------------------ products
         R s;
-        const int r = lane >> 2, c = lane & 3;
-        const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0];
+        const int r = lane >> 2, c = lane & 3, length = p.length, count = p.count, row0 = p.row0;
+        const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + 8 * c;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int row = row0 + 8 * nt + r;
-          const bool in = row < span.rows;
-          const T* from = q + (int64_t)(head * group + row % group) * a.q_stride[1] + (int64_t)(row / group) * a.q_stride[2] + 8 * c;
-          // q as f16, times the power of two that brings the row's largest value to 2^14: exact for all that matters to a score.
-          // Channels 4 i + 1 and 4 i + 3 meet codes of 16 times the unit.
-          float2 e[NB][4];
-          float most = 0.f, sums[NG];
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const uint4 w = in ? *reinterpret_cast<const uint4*>(from + 32 * i) : make_uint4(0, 0, 0, 0);
-            e[i][0] = param<T>(w.x), e[i][1] = param<T>(w.y), e[i][2] = param<T>(w.z), e[i][3] = param<T>(w.w);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) most = fmaxf(most, fmaxf(fabsf(e[i][k].x), fabsf(e[i][k].y)));
-          }
-          most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-          const int up = most > 0.f && isfinite(most) ? min(max(14 - ilogbf(most), -120), 120) : 0;
-          const float grow = __int_as_float((127 + up) << 23);
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              s.q[nt][i][k][0] = MmaOp<__half>::pack(e[i][k].x * grow, e[i][k + 2].x * grow);
-              s.q[nt][i][k][1] = MmaOp<__half>::pack(e[i][k].y * (grow * 0.0625f), e[i][k + 2].y * (grow * 0.0625f));
-            }
-            const float sum = ((e[i][0].x + e[i][0].y) + (e[i][1].x + e[i][1].y)) + ((e[i][2].x + e[i][2].y) + (e[i][3].x + e[i][3].y));
-            if (i % (G / 32) == 0) sums[i / (G / 32)] = sum;
-            else sums[i / (G / 32)] += sum;
-          }
-          float sum = 0.f;   // of group c
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            sums[g] += __shfl_xor_sync(~0u, sums[g], 1);
-            sums[g] += __shfl_xor_sync(~0u, sums[g], 2);
-            sum = c == g ? sums[g] * (grow * 5.9604644775390625e-8f / kSumScale<T>) : sum;
-          }
-          const T high = Elem<T>::from_f(sum);
-          s.q_sum[nt][0] = MmaOp<T>::pack(0.f, Elem<T>::to_f(high));
-          s.q_sum[nt][1] = MmaOp<T>::pack(0.f, sum - Elem<T>::to_f(high));
+          const float grow = row_operands<T, D, G>(q + (int64_t)(p.head * group + row % group) * a.q_stride[1] + (int64_t)(row / group) * a.q_stride[2],
+                                                   row < p.rows, s.q[nt], s.q_sum[nt]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int col = row0 + 8 * nt + 2 * c + j;
             s.factor[nt][j] = a.scale * 1.4426950408889634f * 16777216.f / __shfl_sync(~0u, grow, 4 * (2 * c + j));
-            s.seen[nt][j] = col < span.rows ? length - count + col / group + 1 : 0;
+            s.seen[nt][j] = col < p.rows ? length - count + col / group + 1 : 0;
             s.ref[nt][j] = kLowest;
             s.sum[nt][j] = 0.f;
 #pragma unroll
@@ -554,19 +305,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
         s.limit = kHead + kLazy + 24.f;
         s.last = length;
         const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
-        int t0 = tile0 * kTile + 16 * warp;
-        for (int i = 0; i < tiles; ++i, t0 += kTile) {
-          bool ok = __all_sync(~0u, tc::mbar_try_wait(full + stage, phase));
-          if (!ok) ok = __all_sync(~0u, tc::mbar_wait(full + stage, phase, abort_flag));
-          if (ok) {
-            if (valid[stage] >> warp & 1) {
-              const uint8_t* slice = smem + (stage * kWarps + warp) * L::kSlice;
-              if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0);
-              else take_slice<T, D, G, NT, true>(s, slice, t0);
-            }
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(empty + stage);
+        int t0 = p.tile0 * kTile + 16 * warp;
+        for (int i = 0; i < p.tiles; ++i, t0 += kTile) {
+          if (!dead && !__all_sync(~0u, tc::mbar_try_wait(full + stage, phase))) dead = !__all_sync(~0u, tc::mbar_wait(full + stage, phase, abort_flag));
+          if (!dead && (valid[stage] >> warp & 1)) {
+            const uint8_t* slice = smem + (stage * kWarps + warp) * L::kSlice;
+            if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0);
+            else take_slice<T, D, G, NT, true>(s, slice, t0);
           }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(empty + stage);
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
         // ------------------------------------------------------------ the four warps' rows into one
@@ -596,11 +344,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
             }
           }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
-        const bool starts = tile0 == 0, whole = starts && tiles == span.tiles;
+        const bool starts = p.tile0 == 0, whole = starts && p.tiles == p.all_tiles;
         float* part = a.parts + ((int64_t)blockIdx.x * 2 + starts) * S::kPart;
         for (int i = threadIdx.x; i < kRows * D / 4; i += 32 * kWarps) {
           const int row = i / (D / 4), d = i % (D / 4) * 4;
-          if (row0 + row >= span.rows) break;
+          if (row0 + row >= p.rows) break;
           float top = kLowest, sum = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -616,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
             o.w = fmaf(f, y.w, o.w);
           }
           if (whole) {
-            write_row<T>(a, b, head * group + (row0 + row) % group, (row0 + row) / group, d, o, top, sum);
+            write_row<T>(a, p.b, p.head * group + (row0 + row) % group, (row0 + row) / group, d, o, top, sum);
           } else {
             *reinterpret_cast<float4*>(part + row * D + d) = o;
             if (d == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * row) = make_float2(top, sum);
@@ -624,12 +372,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) kv4_attn_kernel(con
         }
         if (starts && threadIdx.x == 0) {
           // whose parts the unit is made of: from this block to the one that holds its last tile
-          a.owners[((int64_t)b * a.kv_heads + head) * a.row_tiles + row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(unit_at + span.cells - 1));
+          a.owners[((int64_t)p.b * a.kv_heads + p.head) * a.row_tiles + row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(p.end - 1));
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
       }
-    }
-    base = end;
   }
   if (*abort_flag) {
     if (threadIdx.x == 0) *a.status = PSA_ERR_TIMEOUT;
@@ -718,12 +464,21 @@ int sm_count() {   // of the current device; asked once for each
   return n;
 }
 
-constexpr int kMostBlocks = 4 * 160;   // of the first kernel: parts of the scratch are laid out for them
-int rows_per_tile(int64_t rows) { return rows <= 8 ? 8 : 16; }
+constexpr int kMostSms = 160;   // parts of the scratch are laid out for them
+// Rows of a unit: as few units as 48 rows each make, and no more rows than they need.
+int rows_per_tile(int64_t rows) {
+  const int64_t most = cdiv64(rows, cdiv64(rows, 48));
+  return most <= 8 ? 8 : most <= 16 ? 16 : most <= 32 ? 32 : 48;
+}
+// What a unit's beginning and end cost, in tiles (33 requests of 17 to 16384 tokens, 16 key heads of 64 channels: 87 us with 1, 62 with 2, 46
+// with 4, 41 with 8, 45 with 12; 4 key heads of 128 with 5 tokens: 74 us with 2, 64 with 3, 63 with 4).
+int unit_cells(int head_dim, int rows) { return rows > 16 ? 4 : head_dim == 64 ? 8 : 6; }
+// The least cells of a block: few, which leaves a small call's tiles to many blocks (500 tokens, 4 key heads: 8.2 us with 2, 11.7 with 10).
+int least_cells(int rows) { return rows > 16 ? 1 : 2; }
 size_t owners_bytes(int64_t batch, int kv_heads, int64_t row_tiles) { return ((size_t)batch * kv_heads * row_tiles * sizeof(int2) + 255) & ~(size_t)255; }
 
 template <typename T, int D, int G, int NT>
-int launch(const AttnArgs& a, cudaStream_t st) {
+int launch_few(const AttnArgs& a, int sms, cudaStream_t st) {
   using S = Shape<D, G, NT>;
   auto kernel = kv4_attn_kernel<T, D, G, NT>;
   static thread_local uint64_t ready = 0;   // devices that know the kernel's shared memory, per thread
@@ -736,10 +491,15 @@ int launch(const AttnArgs& a, cudaStream_t st) {
     }
     if (dev < 64) ready |= (uint64_t)1 << dev;
   }
-  int blocks = sm_count() * (NT == 1 ? 3 : 2);
-  if (blocks > kMostBlocks) blocks = kMostBlocks;
-  kernel<<<blocks, kThreads, S::kBytes, st>>>(a);
+  kernel<<<sms * blocks_of(S::kRows), kThreads, S::kBytes, st>>>(a);
   PSA_CHECK_LAUNCH("psa_kv4_attention");
+  return PSA_OK;
+}
+template <typename T, int D, int G>
+int launch(const AttnArgs& a, int rows, cudaStream_t st) {
+  const int sms = sm_count() < kMostSms ? sm_count() : kMostSms;
+  const int first = rows == 8 ? launch_few<T, D, G, 1>(a, sms, st) : rows == 16 ? launch_few<T, D, G, 2>(a, sms, st) : launch_rows<T, D, G>(a, sms, rows, st);
+  if (first != PSA_OK) return first;
   const dim3 grid((unsigned)a.tokens, (unsigned)a.heads, (unsigned)a.batch);
   cudaLaunchConfig_t how = {};
   how.gridDim = grid;
@@ -750,7 +510,7 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   early.val.programmaticStreamSerializationAllowed = 1;
   how.attrs = &early;
   how.numAttrs = 1;
-  const cudaError_t rc = cudaLaunchKernelEx(&how, kv4_join_kernel<T, D>, a, (int)S::kRows);
+  const cudaError_t rc = cudaLaunchKernelEx(&how, kv4_join_kernel<T, D>, a, rows);
   PSA_REQUIRE(rc == cudaSuccess, PSA_ERR_CUDA, "psa_kv4_attention: launch failed: %s", cudaGetErrorString(rc));
   return PSA_OK;
 }
@@ -762,7 +522,7 @@ extern "C" size_t psa_kv4_attention_scratch_bytes(int64_t batch, int64_t tokens,
   using namespace psa;
   if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
   const int64_t rows = tokens * (heads / kv_heads), r = rows_per_tile(rows);
-  return owners_bytes(batch, kv_heads, cdiv64(rows, r)) + (size_t)kMostBlocks * 2 * r * (head_dim + 2) * sizeof(float);
+  return owners_bytes(batch, kv_heads, cdiv64(rows, r)) + (size_t)kMostSms * blocks_of((int)r) * 2 * r * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const void* data, const int32_t* table, const int32_t* lengths,
@@ -777,7 +537,9 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   PSA_REQUIRE(page_size > 0 && page_size % 16 == 0 && pages > 0 && pages < ((int64_t)1 << 31) / page_size && width > 0 &&
                   width < ((int64_t)1 << 31) / page_size, PSA_ERR_ARG, "psa_kv4_attention: %lld pages of %d tokens, %lld a request", (long long)pages,
               page_size, (long long)width);
-  PSA_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < 65536, PSA_ERR_ARG, "psa_kv4_attention: %d heads on %d key heads", heads,
+  PSA_REQUIRE(kv_heads > 0 && (double)pages * (page_size / 16) * kv_heads < 2147483648.0, PSA_ERR_ARG,
+              "psa_kv4_attention: %lld pages of %d tokens, %d key heads", (long long)pages, page_size, kv_heads);
+  PSA_REQUIRE(heads > 0 && heads % kv_heads == 0 && heads < 65536, PSA_ERR_ARG, "psa_kv4_attention: %d heads on %d key heads", heads,
               kv_heads);
   PSA_REQUIRE(batch > 0 && batch < 65536 && tokens > 0 && tokens < 65536, PSA_ERR_ARG, "psa_kv4_attention: %lld requests, %lld tokens",
               (long long)batch, (long long)tokens);
@@ -809,14 +571,14 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   a.page = page_size;
   a.scale = sm_scale;
   const int64_t rows = tokens * (heads / kv_heads);
-  a.least_tiles = 2;
+  a.unit_cells = unit_cells(head_dim, rows_per_tile(rows));
+  a.least_cells = least_cells(rows_per_tile(rows));
   a.row_tiles = (int)cdiv64(rows, rows_per_tile(rows));
   PSA_REQUIRE(rows < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_kv4_attention: %lld rows a key head", (long long)rows);
-  PSA_REQUIRE((double)batch * (cdiv64(width * page_size, kTile) + kUnitCells) * a.row_tiles * kv_heads < 2147483648.0, PSA_ERR_UNSUPPORTED,
+  PSA_REQUIRE((double)batch * (cdiv64(width * page_size, kTile) + a.unit_cells) * a.row_tiles * kv_heads < 2147483648.0, PSA_ERR_UNSUPPORTED,
               "psa_kv4_attention: %lld requests of up to %lld tokens: more than 2^31 tiles", (long long)batch, (long long)(width * page_size));
   a.owners = static_cast<int2*>(scratch);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + owners_bytes(batch, kv_heads, a.row_tiles));
-  if (rows_per_tile(rows) == 8) PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, return (launch<T, D, G, 1>(a, (cudaStream_t)stream)));
-  else PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, return (launch<T, D, G, 2>(a, (cudaStream_t)stream)));
+  PSA_DISPATCH_KV4(dtype, head_dim, group, T, D, G, return (launch<T, D, G>(a, rows_per_tile(rows), (cudaStream_t)stream)));
   return PSA_OK;
 }
