@@ -28,7 +28,7 @@ struct Shape {
   static constexpr int kArea = kBuffers * kWeights > kOuts + kTotals ? kBuffers * kWeights : kOuts + kTotals;
   static constexpr int kQ = kStages * kTileBytes + kArea;                          // [kTiles][blocks][lanes] operands of q, 16 bytes
   static constexpr int kQSum = kQ + kTiles * L::kBlocks * 512;                     // [kTiles][lanes] operands of its sums, 8 bytes
-  static constexpr int kColumns = kQSum + kTiles * 256;                            // [rows] {factor to log2, keys that the row sees}
+  static constexpr int kColumns = kQSum + kTiles * 256;                            // [row pairs] {factors to log2, keys that the rows see}
   static constexpr int kRise = kColumns + kRows * 8;                               // [slices][rows] scores that ask for a higher reference
   static constexpr int kWide = kRise + kWarps * kRows * 4;                         // [warps] steps that do
   static constexpr int kBars = kWide + kWarps * kHalves * 4;                       // full
@@ -52,13 +52,34 @@ __device__ __forceinline__ void get2(uint32_t at, uint32_t& a, uint32_t& b) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(at) : "memory");
 }
 
+// Two 32-bit operations in one instruction: the scheduler's slots are what these kernels run out of.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // What a warp carries of its rows.  Lane 4 r + c has rows 8 nt + 2 c + {0, 1} of the warp's: of the scores of its tokens, and of the outputs of
 // its channels.
 template <typename T, int D, int G, int NT>
 struct Rows {
-  float ref[NT][2];             // log2
-  float sum[NT][2];
-  float mid[NT][D / G][2];      // the share of the output that the groups' middle values give
+  float2 ref[NT];               // log2, negated
+  float2 sum[NT];
+  float2 mid[NT][D / G];        // the share of the output that the groups' middle values give
   float out[NT][2][4];          // of channels 4 i, 4 i + 2 (first) and 4 i + 1, 4 i + 3: times 2^-24 and 2^-20
   float cap, limit;             // at least the largest step of the values so far, and the exponent from which a weight is too large
 };
@@ -96,19 +117,22 @@ __device__ __forceinline__ void score(float (&x)[NT][4], int tile0, const uint8_
       const uint32_t w0 = k0.w[b], w1 = k1.w[b];
       const uint32_t a0[4] = {codes(w0, 0), codes(w1, 0), codes(w0, 1), codes(w1, 1)}, a1[4] = {codes(w0, 2), codes(w1, 2), codes(w0, 3), codes(w1, 3)};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const Words<4> q = lds<4>(smem + S::kQ + (((tile0 + nt) * NB + b) * 32 + lane) * 16);
-        const uint32_t b0[2] = {q.w[0], q.w[1]}, b1[2] = {q.w[2], q.w[3]};
-        if (i == 0) mma_new<__half>(acc[nt], a0, b0);
-        else MmaOp<__half>::run(acc[nt], a0, b0);
-        MmaOp<__half>::run(acc[nt], a1, b1);
-      }
+      for (int k = 0; k < 2; ++k)   // one product of every row tile after the other: none waits for the one before it
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const Words<2> q = lds<2>(smem + S::kQ + (((tile0 + nt) * NB + b) * 32 + lane) * 16 + k * 8);
+          if (i == 0 && k == 0) mma_new<__half>(acc[nt], a0, q.w);
+          else MmaOp<__half>::run(acc[nt], k ? a1 : a0, q.w);
+        }
     }
     const float s0 = param<T>(p0.w[g]).x, s1 = param<T>(p1.w[g]).x;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[nt][j] = fmaf(j < 2 ? s0 : s1, acc[nt][j], x[nt][j]);
+      for (int j = 0; j < 4; j += 2) {
+        const float2 y = fma2(both(j ? s1 : s0), make_float2(acc[nt][j], acc[nt][j + 1]), make_float2(x[nt][j], x[nt][j + 1]));
+        x[nt][j] = y.x, x[nt][j + 1] = y.y;
+      }
   }
 }
 
@@ -128,14 +152,12 @@ __device__ __forceinline__ void weigh(Rows<T, D, G, NT>& s, const float (&e)[NT]
     for (int nt = 0; nt < NT; ++nt) {
       const float4 w = columns[4 * nt];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) hidden[nt] |= token + 8 * (j >> 1) >= __float_as_int(j & 1 ? w.w : w.y) ? 1u << j : 0u;
+      for (int j = 0; j < 4; ++j) hidden[nt] |= token + 8 * (j >> 1) >= __float_as_int(j & 1 ? w.w : w.z) ? 1u << j : 0u;
     }
   }
   if (count) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s.sum[nt][j & 1] += e[nt][j];
+    for (int nt = 0; nt < NT; ++nt) s.sum[nt] = add2(add2(s.sum[nt], make_float2(e[nt][0], e[nt][1])), make_float2(e[nt][2], e[nt][3]));
   }
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
@@ -145,12 +167,18 @@ __device__ __forceinline__ void weigh(Rows<T, D, G, NT>& s, const float (&e)[NT]
     uint32_t w[kTerms][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float y[4];
+      const float2 e0 = make_float2(e[nt][0], e[nt][1]), e1 = make_float2(e[nt][2], e[nt][3]);
+      const float2 y0 = mul2(e0, both(u0.x)), y1 = mul2(e1, both(-u1.x));
+      float y[4] = {y0.x, y0.y, y1.x, y1.y};
+      if constexpr (MASKED) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[j] = e[nt][j] * (j < 2 ? u0.x : -u1.x);
-        if (MASKED && (hidden[nt] >> j & 1)) y[j] = 0.f;
-        else if (count) s.mid[nt][g][j & 1] = fmaf(e[nt][j], ends[j >> 1], s.mid[nt][g][j & 1]);
+        for (int j = 0; j < 4; ++j) {
+          float& mid = j & 1 ? s.mid[nt][g].y : s.mid[nt][g].x;
+          if (hidden[nt] >> j & 1) y[j] = 0.f;
+          else if (count) mid = fmaf(e[nt][j], ends[j >> 1], mid);
+        }
+      } else {
+        s.mid[nt][g] = fma2(e1, both(ends[1]), fma2(e0, both(ends[0]), s.mid[nt][g]));
       }
 #pragma unroll
       for (int k = 0; k < kTerms; ++k) {
@@ -196,18 +224,26 @@ __device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4
     }
     widest = fmaxf(s0, s1);
   }
+  float t[NT][4];   // to the references
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const float4 w = columns[4 * nt];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      e[nt][j] *= j & 1 ? w.z : w.x;
-      if (MASKED && token + 8 * (j >> 1) >= __float_as_int(j & 1 ? w.w : w.y)) e[nt][j] = -INFINITY;
-      most = fmaxf(most, e[nt][j] - s.ref[nt][j & 1]);
+    for (int j = 0; j < 4; j += 2) {
+      const float2 y = fma2(make_float2(e[nt][j], e[nt][j + 1]), make_float2(w.x, w.y), s.ref[nt]);
+      t[nt][j] = MASKED && token + 4 * j >= __float_as_int(w.z) ? -INFINITY : y.x;
+      t[nt][j + 1] = MASKED && token + 4 * j >= __float_as_int(w.w) ? -INFINITY : y.y;
+      most = fmaxf(most, fmaxf(t[nt][j], t[nt][j + 1]));
     }
   }
   const bool rises = __any_sync(~0u, widest > s.cap || most > s.limit);
   if (rises) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float4 w = columns[4 * nt];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[nt][j] = MASKED && token + 8 * (j >> 1) >= __float_as_int(j & 1 ? w.w : w.z) ? -INFINITY : e[nt][j] * (j & 1 ? w.y : w.x);
+    }
     float* rise = reinterpret_cast<float*>(smem + S::kRise) + warp % kWarps * S::kRows + 8 * tile0;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
@@ -225,7 +261,7 @@ __device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[nt][j] = ex2(e[nt][j] - s.ref[nt][j & 1]);
+      for (int j = 0; j < 4; ++j) e[nt][j] = ex2(t[nt][j]);
     weigh<T, D, G, NT, MASKED>(s, e, true, columns, slice, token, to);
   }
   return rises;
@@ -255,11 +291,12 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, rise[w * S::kRows + 8 * nt + 2 * c + j]);
       // largest score so far, or what the reference stood for
-      const float ref = fmaxf(m, s.ref[nt][j] - old + kHead) + (up - kHead), fade = ex2(s.ref[nt][j] - ref);
-      s.ref[nt][j] = ref;
-      s.sum[nt][j] *= fade;
+      float& was = j ? s.ref[nt].y : s.ref[nt].x;
+      const float ref = fmaxf(m, kHead - was - old) + (up - kHead), fade = ex2(-was - ref);
+      was = -ref;
+      (j ? s.sum[nt].y : s.sum[nt].x) *= fade;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) s.mid[nt][g][j] *= fade;
+      for (int g = 0; g < NG; ++g) (j ? s.mid[nt][g].y : s.mid[nt][g].x) *= fade;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         s.out[nt][h][j] *= fade;
@@ -395,21 +432,22 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT * kHalves)) kv4_att
       for (int i = 0; i < NB; ++i)
         *reinterpret_cast<uint4*>(smem + S::kQ + ((nt * NB + i) * 32 + lane) * 16) = make_uint4(w[i][0][0], w[i][0][1], w[i][1][0], w[i][1][1]);
       *reinterpret_cast<uint2*>(smem + S::kQSum + (nt * 32 + lane) * 8) = make_uint2(sum[0], sum[1]);
-      if (c == 0)
-        *reinterpret_cast<float2*>(smem + S::kColumns + (8 * nt + r) * 8) =
-            make_float2(a.scale * 1.4426950408889634f * 16777216.f / grow, __int_as_float(in ? max(p.length - p.count + row / group + 1, 0) : 0));
+      if (c == 0) {
+        float* column = reinterpret_cast<float*>(smem + S::kColumns) + (8 * nt + (r & ~1)) * 2 + (r & 1);
+        column[0] = a.scale * 1.4426950408889634f * 16777216.f / grow;
+        column[2] = __int_as_float(in ? max(p.length - p.count + row / group + 1, 0) : 0);
+      }
     }
     Rows<T, D, G, NT> s;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      s.ref[nt] = both(-kLowest);
+      s.sum[nt] = both(0.f);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s.ref[nt][j] = kLowest;
-        s.sum[nt][j] = 0.f;
+      for (int g = 0; g < NG; ++g) s.mid[nt][g] = both(0.f);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) s.mid[nt][g][j] = 0.f;
-        s.out[nt][j][0] = s.out[nt][j][1] = s.out[nt][j][2] = s.out[nt][j][3] = 0.f;
-      }
+      for (int j = 0; j < 8; ++j) s.out[nt][j / 4][j % 4] = 0.f;
+    }
     s.cap = kLeastCap;
     s.limit = kHead + kLazy + 24.f;
     __syncthreads();
@@ -446,12 +484,13 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT * kHalves)) kv4_att
         const int row = 8 * (tile0 + nt) + 2 * c + j;
 #pragma unroll
         for (int g = 0; g <= NG; ++g) {
-          float x = g < NG ? s.mid[nt][g < NG ? g : 0][j] : s.sum[nt][j];
+          const float2 pair = g < NG ? s.mid[nt][g < NG ? g : 0] : s.sum[nt];
+          float x = j ? pair.y : pair.x;
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(~0u, x, d);
           if (r == 0) totals[(own * (NG + 1) + g) * kRows + row] = x;
         }
-        if (r == 0 && own == 0) refs[row] = s.ref[nt][j];
+        if (r == 0 && own == 0) refs[row] = j ? -s.ref[nt].y : -s.ref[nt].x;
         *reinterpret_cast<float4*>(outs + (own / NB * kRows + row) * S::kOutRow + 32 * (own % NB) + 4 * r) =
             make_float4(s.out[nt][0][j] * 16777216.f, s.out[nt][0][2 + j] * 1048576.f, s.out[nt][1][j] * 16777216.f, s.out[nt][1][2 + j] * 1048576.f);
       }
