@@ -243,6 +243,12 @@ extern "C" int psa_plan_pages(const int32_t* table, const int32_t* lengths, cons
   PSA_REQUIRE(table && lengths && counts && pool && free_in && table_out && lengths_out && free_out && slots && scratch && status, PSA_ERR_ARG,
               "psa_plan_pages: null pointer");
   if (int rc = check_sizes("psa_plan_pages", requests, width, pool_size, page_size)) return rc;
+  // blocks read counts and pool while others write: an output may be its own input's memory, not another's
+  for (const int32_t* out : {(const int32_t*)table_out, (const int32_t*)lengths_out, (const int32_t*)free_out, (const int32_t*)slots})
+    PSA_REQUIRE(out != counts && out != pool && (out == table_out || out != table) && (out == lengths_out || out != lengths) &&
+                    (out == free_out || out != free_in), PSA_ERR_ARG, "psa_plan_pages: an output in another input's memory");
+  PSA_REQUIRE(table_out != lengths_out && table_out != free_out && table_out != slots && lengths_out != free_out && lengths_out != slots &&
+                  free_out != slots, PSA_ERR_ARG, "psa_plan_pages: two outputs in the same memory");
   PSA_REQUIRE(tokens > 0 && tokens <= ((int64_t)1 << 30) && scratch_bytes >= psa_plan_pages_scratch_bytes(requests), PSA_ERR_ARG,
               "psa_plan_pages: %lld tokens, scratch of %zu bytes", (long long)tokens, scratch_bytes);
   cudaStream_t st = (cudaStream_t)stream;

@@ -136,6 +136,17 @@ def test_pages_entries_refuse():
     for kw in (dict(requests=0), dict(requests=65536), dict(width=0), dict(width=2 ** 28), dict(pool=0), dict(pool=2 ** 27), dict(page=8), dict(page=0),
                dict(tokens=0), dict(tokens=2 ** 30 + 1), dict(scratch=8), dict(table=None)):
         refused(call(**kw), "psa_plan_pages")
+
+    def apart(**same):
+        names = ("table", "lengths", "counts", "pool", "free", "table_out", "lengths_out", "free_out", "slots")
+        at = {n: P * (i + 1) for i, n in enumerate(names)}
+        at.update({a: at[b] for a, b in same.items()})
+        return lib.psa_plan_pages(*[at[n] for n in names], P * 20, 10 ** 6, 2, 4, 8, 16, 2 ** 30 + 1, P * 21, None)
+    refused(apart(table_out="table", lengths_out="lengths", free_out="free"), "tokens")          # in place: only the number of tokens is wrong
+    for same in (dict(lengths_out="counts"), dict(table_out="pool"), dict(free_out="lengths"), dict(slots="table"), dict(free_out="counts")):
+        refused(apart(**same), "another input")
+    for same in (dict(lengths_out="free_out"), dict(slots="table_out")):
+        refused(apart(**same), "two outputs")
     refused(lib.psa_release_pages(P, P, None, P, P, 2, 4, 8, 16, P, None), "null")
     refused(lib.psa_release_pages(P, P, P, P, P, 2, 4, 8, 17, P, None), "page size 17")
     assert lib.psa_plan_pages_scratch_bytes(0) == 0
@@ -167,6 +178,21 @@ def test_cache_entries_refuse():
         refused(attend(**kw), word)
     assert lib.psa_kv4_slice_bytes(128, 32) == 16 * 160 and lib.psa_kv4_slice_bytes(128, 16) == 0
     assert lib.psa_kv4_attention_scratch_bytes(0, 1, 1, 1, 64) == 0
+
+
+def test_calls_leave_what_is_out_of_the_ordinary_to_their_wrappers(ops):
+    """CPU tensors, numbers that are none, wrong counts of arguments: None, and nothing is launched."""
+    from psa_b200 import _calls
+    i, data = torch.zeros(2, dtype=torch.int32), ops.kv4_empty(2, 1, 16, 64, 32, "cpu")
+    turns, axis = ops._rotary_plan(64, (32,), 1e4, False, None)
+    assert _calls.rotate(x(2, 1, 1, 64), None, i.view(1, 2), turns, axis, True, False) is None
+    assert _calls.rotate(3, None, i, turns, axis, True, False) is None and _calls.rotate() is None
+    assert _calls.plan_pages(i.view(2, 1), i, i, i, i[:1], 16, 1, None) is None and _calls.plan_pages(None) is None
+    assert _calls.append(data, x(1, 1, 2, 64), x(1, 1, 2, 64), i[None], 32) is None and _calls.append(data, 1, 2, 3, 4) is None
+    assert _calls.read(data, i[None], 64, 32, 2) is None and _calls.read(data, i[None], 64, 2 ** 70, None) is None
+    assert _calls.attend(x(2, 1, 1, 64), data, i.view(2, 1), i, 32, None, None, False) is None and _calls.attend(*[None] * 8) is None
+    with pytest.raises(TypeError):
+        _calls.status("cuda", 0)
 
 
 def test_rotary_plan_counts_turns_to_the_last_bit(ops):

@@ -598,3 +598,260 @@ def test_cache_offsets_beyond_32_bits(ops):
     want = torch.softmax(q[0].double() @ kk.transpose(-1, -2) * 128 ** -0.5, -1) @ vv
     assert float((got[0].double() - want).abs().max()) < 0.02
     ops.check_status()
+
+
+# ---------------------------------------------------------------- more than 16 rows a key head
+MANY = [(10, 2, 5, [5, 70, 3000]), (4, 1, 8, [9, 64, 65, 8]), (6, 1, 8, [1000, 8]), (28, 4, 6, [4000, 77]), (8, 8, 20, [20, 500, 33]), (7, 1, 64, [64, 900])]
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+@pytest.mark.parametrize("D,group", SIZES)
+@pytest.mark.parametrize("H,Hk,n,lengths", MANY)
+def test_attention_of_many_rows(ops, dtype, D, group, H, Hk, n, lengths):
+    g = gen(2 * D + group + H + n)
+    c = Filled(ops, g, lengths, Hk, D, group, dtype, 64 if n % 2 else 128)
+    check_attention(ops, randn(g, len(lengths), n, H, D, dtype=dtype).transpose(1, 2), c)
+
+
+@pytest.mark.parametrize("page", [16, 48, 272])
+@pytest.mark.parametrize("n", [4, 8])
+def test_attention_of_many_rows_pages_of_other_sizes(ops, page, n):
+    """Pages that do not hold whole tiles, a copy a slice; more than 8 tiles of them, and lengths at their borders."""
+    g = gen(page + n)
+    lengths = [max(page - 1, n), page + n, 3 * page + 17, n, 1500, 700]
+    c = Filled(ops, g, lengths, 2, 128, 32, torch.float16, page)
+    check_attention(ops, randn(g, 6, 14, n, 128, dtype=torch.float16), c)
+
+
+@pytest.mark.parametrize("n", [3, 6])
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(6.0, 2.0, 1.0), (1.0, 1.0, 200.0), (0.02, 0.02, 1e-3), (20.0, 3.0, 0.1)])
+def test_attention_of_many_rows_sharp_flat_large_and_small(ops, n, q_scale, k_scale, v_scale):
+    g = gen(33)
+    c = Filled(ops, g, [3000, 64, 6], 2, 128, 64, torch.bfloat16, 64, k_scale=k_scale, v_scale=v_scale)
+    check_attention(ops, randn(g, 3, 16, n, 128).mul_(q_scale).to(torch.bfloat16), c)
+
+
+def test_attention_of_many_rows_maximum_that_rises_late_and_falls(ops):
+    """The references of all warps move together: keys that line up with some rows' queries more and more, with others' less and less."""
+    g = gen(34)
+    c = Filled(ops, g, [2000, 2000], 1, 128, 32, torch.bfloat16, 64)
+    u = randn(g, 128, dtype=torch.bfloat16)
+    ramp = torch.linspace(-3, 3, 2000, device=DEV)[:, None].to(torch.bfloat16)
+    c.k[0, 0], c.k[1, 0] = u * ramp, u * -ramp
+    ops.kv4_append(c.data, c.k, c.v, c.slots, 32)
+    sign = torch.where(torch.arange(12, device=DEV) % 3 == 0, -1.0, 1.0).to(torch.bfloat16)[None, :, None, None]
+    check_attention(ops, (u * 1.5 * sign).expand(2, 12, 3, 128).clone(), c)
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+def test_attention_of_many_rows_counts_and_scales(ops, dtype):
+    """Requests with fewer new tokens than rows, none, and more than they have tokens; scales of either sign and none."""
+    g = gen(35)
+    c = Filled(ops, g, [200, 64, 5, 0, 1, 90], 2, 64, 32, dtype, 32)
+    q = randn(g, 6, 6, 11, 64, dtype=dtype)
+    for scale in (None, 0.0, -0.3):
+        got = check_attention(ops, q, c, counts=[3, 11, 11, 11, 1, 0], scale=scale)
+    assert not bool(got[0, :, 3:].any()) and not bool(got[3].any()) and not bool(got[5].any()) and not bool(got[2, :, :6].any())
+
+
+# ---------------------------------------------------------------- all of it together
+class Layer:
+    """One attention layer of a decoder: rotary positions with three axes, the new keys and values into the cache, attention over it."""
+
+    def __init__(self, table, Hk, D, dtype, group):
+        from psa_b200.cache import KV4Cache
+        self.cache = KV4Cache(table, Hk, D, dtype, group)
+        self.k, self.v = [], []                                   # what every request holds, as it was appended
+
+    def step(self, ops, q, k, v, positions, slots, counts):
+        q, k = ops.rotate_axes(q, k, positions, (8, 12, 12) if q.shape[-1] == 64 else (16, 24, 24), theta=1e6)
+        self.cache.append(k, v, slots)
+        return q, k, self.cache.attend(q, counts)
+
+
+def token_major(g, B, n, H, D, dtype):
+    return randn(g, B, n, H, D, dtype=dtype).transpose(1, 2)
+
+
+@pytest.mark.parametrize("dtype,D,group,H,Hk", [(torch.bfloat16, 128, 32, 28, 4), (torch.float16, 64, 64, 6, 6)], **names)
+def test_answering_prompts_and_tokens(ops, dtype, D, group, H, Hk):
+    """Prompts of different lengths in one padded batch, single tokens, drafted tokens, a request that ends and another in its place:
+    every output against plain attention in 64 bits over what the cache stands for."""
+    from psa_b200.cache import PageTable
+    g = gen(40)
+    B = 4
+    table = PageTable(B, 400, 40, 32, DEV)
+    layers = [Layer(table, Hk, D, dtype, group) for _ in range(2)]
+    held = [[(torch.zeros(Hk, 0, D, dtype=dtype, device=DEV),) * 2 for _ in range(B)] for _ in layers]
+    for counts in ([150, 3, 77, 0], [1, 1, 1, 0], [1, 1, 1, 31], [5, 0, 2, 5], "end 1", [1, 40, 1, 1], [1, 1, 1, 1]):
+        if counts == "end 1":
+            table.release(torch.tensor([False, True, False, False], device=DEV))
+            for h in held:
+                h[1] = (torch.zeros(Hk, 0, D, dtype=dtype, device=DEV),) * 2
+            continue
+        n = max(counts)
+        count = torch.tensor(counts, device=DEV)
+        start = table.lengths.clone()
+        slots = table.reserve(count, n)
+        pos = (start[:, None] + torch.arange(n, device=DEV)).expand(3, B, n)
+        for layer, h in zip(layers, held):
+            q, k, v = (token_major(g, B, n, heads, D, dtype) for heads in (H, Hk, Hk))
+            q, k, out = layer.step(ops, q, k, v, pos, slots, count)
+            for b, m in enumerate(counts):
+                h[b] = tuple(torch.cat([old, new[b, :, :m]], 1) for old, new in zip(h[b], (k, v)))
+            longest = max(x[0].shape[1] for x in h)
+
+            class Held:
+                pass
+            c = Held()
+            c.group, c.lengths = group, [x[0].shape[1] for x in h]
+            c.k, c.v = (torch.stack([torch.nn.functional.pad(x[i], (0, 0, 0, longest - x[i].shape[1])) for x in h]) for i in (0, 1))
+            assert table.lengths.tolist() == c.lengths
+            want, _, tol, _ = attention(q, c, counts)
+            assert bool(((out.double() - want).abs() <= tol).all())
+    ops.check_status()
+
+
+def test_answering_step_captured_and_replayed(ops):
+    """One step of two layers as a CUDA graph, replayed with other tokens, against the same steps launched one by one; a second graph of the
+    same state between them."""
+    from psa_b200.cache import PageTable
+    g = gen(41)
+    B, H, Hk, D, dtype = 3, 8, 2, 64, torch.bfloat16
+
+    def state():
+        table = PageTable(B, 300, 60, 16, DEV)
+        return table, [Layer(table, Hk, D, dtype, 32) for _ in range(2)]
+    eager, replayed = state(), state()
+    inputs = [token_major(g, B, 1, heads, D, dtype) for heads in (H, Hk, Hk)]
+    drafted = [token_major(g, B, 4, heads, D, dtype) for heads in (4 * H, Hk, Hk)]
+    ones, four = torch.ones(B, dtype=torch.int32, device=DEV), torch.tensor([4, 0, 3], dtype=torch.int32, device=DEV)
+
+    def step(s, xs, counts):
+        table, layers = s
+        n = xs[0].shape[2]
+        start = table.lengths.clone()
+        slots = table.reserve(counts, n)
+        pos = (start[:, None] + torch.arange(n, device=DEV, dtype=torch.int32)).expand(3, B, n)
+        return [layer.step(ops, *xs, pos, slots, counts)[2] for layer in layers]
+    for s in (eager, replayed):                                    # a start, and every kernel's first launch outside the captures
+        step(s, [x.expand(-1, -1, 90, -1).contiguous() if x.shape[2] == 1 else x for x in inputs], torch.tensor([90, 17, 64], device=DEV))
+        step(s, drafted, four)
+    graphs, outs = [], []
+    for xs, counts in ((inputs, ones), (drafted, four)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(replayed, xs, counts))
+        graphs.append(graph)
+    for which in (0, 0, 1, 0, 1, 1, 0):
+        for x in (inputs, drafted)[which]:
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV).to(dtype))
+        want = step(eager, (inputs, drafted)[which], (ones, four)[which])
+        graphs[which].replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs[which], want))
+    assert torch.equal(eager[0].lengths, replayed[0].lengths) and torch.equal(eager[0].table, replayed[0].table)
+    ops.check_status()
+
+
+def test_rotary_backward_captured(ops):
+    """Forward and gradients in a captured graph, replayed with other values.  (No eager graph of the same leaves is alive while it is
+    captured: PyTorch's engine would make its stream wait for the capturing one, whatever the operator, and the capture would fail.)"""
+    g = gen(42)
+    q, k = (token_major(g, 1, 33, h, 64, torch.bfloat16).requires_grad_() for h in (4, 2))
+    pos = torch.arange(33, dtype=torch.int32, device=DEV)[None]
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+
+    def both():
+        outs = ops.rotate_axes(q, k, pos, (32,))
+        return [x.detach() for x in outs], torch.autograd.grad(outs, (q, k), (dq, dk))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs, grads = both()
+    for _ in range(2):
+        dq.copy_(torch.randn_like(dq)), dk.copy_(torch.randn_like(dk))
+        with torch.no_grad():
+            q.copy_(torch.randn_like(q)), k.copy_(torch.randn_like(k))
+        graph.replay()
+        want_outs, want = both()
+        assert all(torch.equal(a, b) for a, b in zip((*outs, *grads), (*want_outs, *want)))
+
+
+def test_answering_on_other_streams_and_threads(ops):
+    """Calls on a stream of their own, and from several host threads at once, give what they give one after another."""
+    import threading
+    g = gen(43)
+    cases = []
+    for i in range(4):
+        c = Filled(ops, g, [300 + 100 * i, 40, 1000], 2, 64 if i % 2 else 128, 32, TYPES[i // 2], 64)
+        q = randn(g, 3, 2 * (1, 4, 9, 20)[i], 1, c.D, dtype=c.dtype)
+        pos = torch.arange(len(c.lengths), device=DEV).view(1, 3, 1).int()
+        cases.append((c, q, pos))
+
+    def call(c, q, pos):
+        turned = ops.rotate_axes(q, None, pos, (c.D // 2,))
+        return ops.kv4_attention(turned, c.data, c.table, c.len, c.group), *ops.kv4_read(c.data, c.slots, c.D, c.group, c.dtype)
+    want = [call(*x) for x in cases]
+    torch.cuda.synchronize()
+    got, failed = [None] * len(cases), []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = call(*cases[i])
+            stream.synchronize()
+        except Exception as e:          # noqa: BLE001  (reported by the main thread)
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    ops.check_status()
+
+
+@pytest.mark.parametrize("H", [1, 2, 3, 6])
+@pytest.mark.parametrize("dtype", TYPES, **names)
+def test_cache_of_few_heads(ops, H, dtype):
+    """A thread's four rows are of one, two or four tokens, over the ends of batch elements; some slots are none."""
+    g = gen(44 + H)
+    B, n, D = 3, 7, 64
+    k, v = token_major(g, B, n, H, D, dtype), randn(g, B, H, n, D, dtype=dtype)
+    data = ops.kv4_empty(3, H, 16, D, 32, DEV)
+    slots = some_slots(g, B, n, 3, 16)
+    slots[1, 3] = slots[2, 6] = -1
+    ops.kv4_append(data, k, v, slots, 32)
+    for x, y in zip((k, v), ops.kv4_read(data, slots, D, 32, dtype)):
+        want = stands_for(x, 32) * (slots >= 0)[:, None, :, None]
+        assert bool(((y.double() - want).abs() <= HALF[dtype] * 1.001 * want.abs() + TINY[dtype]).all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+def test_cache_ties_go_to_the_even_code(ops, dtype):
+    """Values exactly between two codes, for steps whose inverse is rounded: lowest 0, step s, values (i + 1/2) s."""
+    steps = [1.0, 3.0, 5.0, 7.0, 11.0, 13.0, 0.375, 49.0]
+    x = torch.zeros(1, 1, len(steps), 64, device=DEV)
+    for t, s in enumerate(steps):
+        x[0, 0, t, :15] = (torch.arange(15, device=DEV) + 0.5) * s
+        x[0, 0, t, 16], x[0, 0, t, 32:48] = 15 * s, torch.arange(16, device=DEV) * s
+    x = x.to(dtype)
+    exact = (x.double()[..., :15] == ((torch.arange(15, device=DEV) + 0.5) * torch.tensor(steps, device=DEV)[:, None]).double()).all(-1)[0, 0]
+    # (2 i + 1) s / 2 up to 29 s / 2: whole numbers of s's last place up to 29 s, which bf16 (8 bits) holds up to s = 7 (and 3 / 8), f16 all
+    assert int(exact.sum()) == (5 if dtype == torch.bfloat16 else 8)
+    data = ops.kv4_empty(1, 1, 16, 64, 64, DEV)
+    slots = torch.arange(len(steps), device=DEV)[None]
+    ops.kv4_append(data, x, x, slots, 64)
+    k, v = ops.kv4_read(data, slots, 64, 64, dtype)
+    want = stands_for(x, 64)
+    for y in (k, v):
+        assert bool(((y.double() - want).abs() <= HALF[dtype] * 1.001 * want.abs()).all())
