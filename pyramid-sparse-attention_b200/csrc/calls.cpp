@@ -113,10 +113,11 @@ struct Buffer {   // of a ctypes array
   }
 };
 
-// rotate(q, k or None, positions [axes, (B or 1,) S], turns, axis of pairs, half, inverse) -> tuple
+// rotate(q, k or None, positions [axes, (B or 1,) S], turns, axis of pairs, half, inverse, axes) -> tuple
 PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 7) return none();
+  int64_t axes;
+  if (n != 8 || !integer(args[7], axes)) return none();
   const at::Tensor* q = plain(args[0]);
   if (!q) return none();
   const int index = q->get_device();
@@ -137,7 +138,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     heads[i] = (int32_t)x.size(1);
   }
   const int dims = (int)pos->dim();
-  if ((dims != 2 && dims != 3) || pos->size(dims - 1) != q->size(2) || (dims == 3 && pos->size(1) != q->size(0) && pos->size(1) != 1)) return none();
+  if ((dims != 2 && dims != 3) || pos->size(0) != axes || pos->size(dims - 1) != q->size(2) || (dims == 3 && pos->size(1) != q->size(0) && pos->size(1) != 1)) return none();
   const int64_t pos_strides[3] = {pos->stride(0), dims == 3 && pos->size(1) > 1 ? pos->stride(1) : 0, pos->stride(dims - 1)};
   Buffer turns(args[3]), axis(args[4]);
   const int64_t dim = q->size(3);
@@ -193,13 +194,13 @@ PyObject* plan_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (args[7] == Py_None)
     for (int i = 0; i < 3; ++i) out[i] = made((i == 0 ? table : i == 1 ? lengths : free)->sizes(), at::kInt, table->device());
   const at::Tensor slots = made({requests, tokens}, at::kInt, table->device());
-  const size_t bytes = psa_plan_pages_scratch_bytes(requests);
-  const at::Tensor scratch = made({(int64_t)bytes}, at::kByte, table->device());
+  const size_t bytes = args[7] == Py_None && requests <= 1024 ? 0 : psa_plan_pages_scratch_bytes(requests);
+  const at::Tensor scratch = bytes ? made({(int64_t)bytes}, at::kByte, table->device()) : at::Tensor();
   void* stream = c10::cuda::getCurrentCUDAStream(index).stream();
   const int rc = called([&] {
     return psa_plan_pages(table->const_data_ptr<int32_t>(), lengths->const_data_ptr<int32_t>(), counts->const_data_ptr<int32_t>(),
                           pool->const_data_ptr<int32_t>(), free->const_data_ptr<int32_t>(), out[0].data_ptr<int32_t>(), out[1].data_ptr<int32_t>(),
-                          out[2].data_ptr<int32_t>(), slots.data_ptr<int32_t>(), scratch.data_ptr(), bytes, requests, width, pool->size(0), (int)page,
+                          out[2].data_ptr<int32_t>(), slots.data_ptr<int32_t>(), bytes ? scratch.data_ptr() : nullptr, bytes, requests, width, pool->size(0), (int)page,
                           tokens, status_words[index], stream);
   });
   if (rc) return PyLong_FromLong(rc);

@@ -240,7 +240,7 @@ extern "C" int psa_plan_pages(const int32_t* table, const int32_t* lengths, cons
                               int32_t* table_out, int32_t* lengths_out, int32_t* free_out, int32_t* slots, void* scratch, size_t scratch_bytes,
                               int64_t requests, int64_t width, int64_t pool_size, int page_size, int64_t tokens, int32_t* status, void* stream) {
   using namespace psa;
-  PSA_REQUIRE(table && lengths && counts && pool && free_in && table_out && lengths_out && free_out && slots && scratch && status, PSA_ERR_ARG,
+  PSA_REQUIRE(table && lengths && counts && pool && free_in && table_out && lengths_out && free_out && slots && status, PSA_ERR_ARG,
               "psa_plan_pages: null pointer");
   if (int rc = check_sizes("psa_plan_pages", requests, width, pool_size, page_size)) return rc;
   // blocks read counts and pool while others write: an output may be its own input's memory, not another's
@@ -249,8 +249,12 @@ extern "C" int psa_plan_pages(const int32_t* table, const int32_t* lengths, cons
                     (out == free_out || out != free_in), PSA_ERR_ARG, "psa_plan_pages: an output in another input's memory");
   PSA_REQUIRE(table_out != lengths_out && table_out != free_out && table_out != slots && lengths_out != free_out && lengths_out != slots &&
                   free_out != slots, PSA_ERR_ARG, "psa_plan_pages: two outputs in the same memory");
-  PSA_REQUIRE(tokens > 0 && tokens <= ((int64_t)1 << 30) && scratch_bytes >= psa_plan_pages_scratch_bytes(requests), PSA_ERR_ARG,
-              "psa_plan_pages: %lld tokens, scratch of %zu bytes", (long long)tokens, scratch_bytes);
+  PSA_REQUIRE(tokens > 0 && tokens <= ((int64_t)1 << 30), PSA_ERR_ARG, "psa_plan_pages: %lld tokens", (long long)tokens);
+  const int64_t wide = width > tokens ? width : tokens;
+  const bool apart = lengths_out != lengths && free_out != free_in && table_out != table && requests <= kPlanThreads;
+  const bool few = requests * (table_out == table ? tokens : wide) <= kFewEntries;
+  PSA_REQUIRE(apart || (scratch && scratch_bytes >= psa_plan_pages_scratch_bytes(requests)), PSA_ERR_ARG, "psa_plan_pages: scratch of %zu bytes",
+              scratch_bytes);
   cudaStream_t st = (cudaStream_t)stream;
   PlanArgs a = {table, lengths, counts, pool, free_in, table_out, lengths_out, free_out, slots, status,
                 reinterpret_cast<Grant*>(static_cast<char*>(scratch) + 16), static_cast<int32_t*>(scratch), (int)requests, (int)width, (int)pool_size,
@@ -258,12 +262,10 @@ extern "C" int psa_plan_pages(const int32_t* table, const int32_t* lengths, cons
   if ((page_size & (page_size - 1)) == 0)
     for (a.shift = 0; 1 << a.shift < page_size;) ++a.shift;
   a.fours = ((((uintptr_t)table_out | (uintptr_t)slots) & 15) | (uintptr_t)(width & 3) | (uintptr_t)(tokens & 3)) == 0;
-  const int64_t wide = width > tokens ? width : tokens;
   const dim3 rows((unsigned)cdiv64(wide, kRowEntries), (unsigned)requests);
-  const bool apart = lengths_out != lengths && free_out != free_in && table_out != table;
-  if (apart && requests <= kPlanThreads) {
+  if (apart) {
     plan_rows_kernel<<<rows, kRowThreads, 0, st>>>(a);
-  } else if (requests * (table_out == table ? tokens : wide) <= kFewEntries) {
+  } else if (few) {
     plan_kernel<true><<<1, kPlanThreads, 0, st>>>(a);
   } else {
     plan_kernel<false><<<1, kPlanThreads, 0, st>>>(a);

@@ -894,7 +894,7 @@ def _rotary_plan(head_dim: int, sections: Tuple[int, ...], theta: float, per_axi
 def _rotate(xs, positions: torch.Tensor, plan, half: bool, inverse: bool):
     """xs: 1 or 2 tensors [B, H, S, D], positions [axes, S] or [axes, B or 1, S] -> turned copies."""
     x, n = xs[0], len(xs)
-    outs = _calls.rotate(x, xs[1] if n == 2 else None, positions, plan[0], plan[1], half, inverse)
+    outs = _calls.rotate(x, xs[1] if n == 2 else None, positions, plan[0], plan[1], half, inverse, positions.shape[0])
     if outs is not None:
         if type(outs) is int:
             check(outs, "psa_rotate_axes")
@@ -957,19 +957,24 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     inv_freq: D/2 frequencies instead.  layout: "half" pairs channels (i, i + D/2), "pairs" (2i, 2i + 1).  A position of zero
     leaves a token as it is.  Angles are exact to 2^-24 turns at any position; values are computed in 32 bits and rounded once.
     Returns the turned copies (q, or (q, k)), in the order of dimensions of their inputs; differentiable in q and k."""
+    sections = tuple(map(int, sections))
+    plan = _rotary_plan(q.size(-1), sections, float(theta), bool(per_axis), None if inv_freq is None else tuple(map(float, inv_freq)))
+    half = layout == "half"
+    if half or layout == "pairs":
+        outs = _calls.rotate(q, k, positions, plan[0], plan[1], half, False, len(sections))
+        if type(outs) is tuple:
+            return outs[0] if k is None else outs
     xs = [q] if k is None else [q, k]
-    if q.dim() != 4:
+    if any(x.dim() != 4 for x in xs):
         raise ValueError("rotate_axes: q [B, H, S, D] and k [B, Hkv, S, D] of one dtype")
     if layout not in ("half", "pairs"):
         raise ValueError(f"rotate_axes: layout must be 'half' or 'pairs', got {layout!r}")
-    sections = tuple(map(int, sections))
     if positions.dim() not in (2, 3) or positions.size(0) != len(sections):
         raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{len(sections)}, {q.size(0)}, {q.size(2)}]")
-    plan = _rotary_plan(q.size(3), sections, float(theta), bool(per_axis), None if inv_freq is None else tuple(map(float, inv_freq)))
-    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
-        outs = _RotateAxes.apply(positions, plan, layout == "half", False, *xs)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        outs = _RotateAxes.apply(positions, plan, half, False, *xs)
     else:
-        outs = _rotate(xs, positions, plan, layout == "half", False)
+        outs = _rotate(xs, positions, plan, half, False)
     return outs[0] if k is None else outs
 
 

@@ -185,8 +185,8 @@ def test_calls_leave_what_is_out_of_the_ordinary_to_their_wrappers(ops):
     from psa_b200 import _calls
     i, data = torch.zeros(2, dtype=torch.int32), ops.kv4_empty(2, 1, 16, 64, 32, "cpu")
     turns, axis = ops._rotary_plan(64, (32,), 1e4, False, None)
-    assert _calls.rotate(x(2, 1, 1, 64), None, i.view(1, 2), turns, axis, True, False) is None
-    assert _calls.rotate(3, None, i, turns, axis, True, False) is None and _calls.rotate() is None
+    assert _calls.rotate(x(2, 1, 1, 64), None, i.view(1, 2), turns, axis, True, False, 1) is None
+    assert _calls.rotate(3, None, i, turns, axis, True, False, 1) is None and _calls.rotate() is None
     assert _calls.plan_pages(i.view(2, 1), i, i, i, i[:1], 16, 1, None) is None and _calls.plan_pages(None) is None
     assert _calls.append(data, x(1, 1, 2, 64), x(1, 1, 2, 64), i[None], 32) is None and _calls.append(data, 1, 2, 3, 4) is None
     assert _calls.read(data, i[None], 64, 32, 2) is None and _calls.read(data, i[None], 64, 2 ** 70, None) is None
