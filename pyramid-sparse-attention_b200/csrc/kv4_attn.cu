@@ -123,18 +123,17 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
     }
     widest = fmaxf(s0, s1);
   }
-  bool rises = widest > s.cap;
-  float e[NT][4];
+  float e[NT][4], most = -INFINITY;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       e[nt][j] = fmaf(x[nt][j], s.factor[nt][j & 1], -s.ref[nt][j & 1]);
       if (MASKED && token + 8 * (j >> 1) >= s.seen[nt][j & 1]) e[nt][j] = -INFINITY;
-      rises = rises || e[nt][j] > s.limit;
+      most = fmaxf(most, e[nt][j]);
     }
   // ---- the references move seldom: when a weight times a step could leave f16
-  if (__any_sync(~0u, rises)) {
+  if (__any_sync(~0u, widest > s.cap || most > s.limit)) {
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
     const float old = log2f(s.cap);
@@ -264,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   const bool whole_tiles = a.page % kTile == 0;
   int stage = 0;
   uint32_t phase = 0;
-  bool dead = false;   // a wait ran out: nothing is waited for any more, and what is computed does not count
+  bool dead = false;   // a wait ran out: nothing is copied or handed back any more, and what is computed does not count
   Walk walk = {request, base, shares.first(blockIdx.x), shares.first(blockIdx.x + 1)};
   Piece p;
   while (walk.next(a, kRows, p)) {
@@ -305,17 +304,27 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         s.limit = kHead + kLazy + 24.f;
         s.last = length;
         const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
-        int t0 = p.tile0 * kTile + 16 * warp;
-        for (int i = 0; i < p.tiles; ++i, t0 += kTile) {
-          if (!dead && !__all_sync(~0u, tc::mbar_try_wait(full + stage, phase))) dead = !__all_sync(~0u, tc::mbar_wait(full + stage, phase, abort_flag));
-          if (!dead && (valid[stage] >> warp & 1)) {
-            const uint8_t* slice = smem + (stage * kWarps + warp) * L::kSlice;
-            if (t0 + 16 <= all_see) take_slice<T, D, G, NT, false>(s, slice, t0);
-            else take_slice<T, D, G, NT, true>(s, slice, t0);
-          }
+        // tiles whose tokens every row sees, then the others
+        const int first = p.tile0 * kTile + 16 * warp, plain = all_see - 16 >= first ? min((all_see - 16 - first) / kTile + 1, p.tiles) : 0;
+        auto wait = [&]() {
+          if (!tc::mbar_try_wait(full + stage, phase) && !tc::mbar_wait(full + stage, phase, abort_flag)) dead = true;
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(empty + stage);
+        };
+        auto leave = [&]() {
+          __syncwarp();
+          if (lane == 0 && !dead) tc::mbar_arrive(empty + stage);
           if (++stage == kStages) stage = 0, phase ^= 1;
+        };
+        int i = 0;
+        for (; i < plain; ++i) {
+          wait();
+          if (valid[stage] & 1u << warp) take_slice<T, D, G, NT, false>(s, smem + (stage * kWarps + warp) * L::kSlice, 0);
+          leave();
+        }
+        for (; i < p.tiles; ++i) {
+          wait();
+          if (valid[stage] & 1u << warp) take_slice<T, D, G, NT, true>(s, smem + (stage * kWarps + warp) * L::kSlice, first + i * kTile);
+          leave();
         }
         // ------------------------------------------------------------ the four warps' rows into one
         float* mine = out_s + warp * kRows * S::kOutRow;
