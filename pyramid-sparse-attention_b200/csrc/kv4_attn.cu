@@ -32,7 +32,7 @@ template <int D, int G, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSlice = Kv4<D, G>::kSlice;
-  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kStages = D == 128 ? 4 : 6, kPairs = kStages / 2;           // tiles of the ring; they are waited for in pairs
   static constexpr int kOutRow = D + 4;                                            // floats; 4 more spread the banks
   static constexpr int kOut = kStages * kWarps * kSlice;                           // [warps][rows][kOutRow]
   static constexpr int kStats = kOut + kWarps * kRows * kOutRow * 4;               // [warps][rows][2]
@@ -240,14 +240,14 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   float* out_s = reinterpret_cast<float*>(smem + S::kOut);
   float* stats_s = reinterpret_cast<float*>(smem + S::kStats);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
-  uint64_t* empty = full + kStages;
+  uint64_t* empty = full + S::kPairs;
   int* scan = reinterpret_cast<int*>(smem + S::kMore);
   volatile int* abort_flag = scan + 8;
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(scan + 9);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      tc::mbar_init(full + i, 1);
+    for (int i = 0; i < S::kPairs; ++i) {
+      tc::mbar_init(full + i, 2);
       tc::mbar_init(empty + i, kWarps);
     }
     tc::fence_mbar_init();
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   if ((int)blockIdx.x >= shares.blocks) return;
   const int group = a.group;
   const bool whole_tiles = a.page % kTile == 0;
-  int stage = 0;
+  int pair = 0;
   uint32_t phase = 0;
   bool dead = false;   // a wait ran out: nothing is copied or handed back any more, and what is computed does not count
   Walk walk = {request, base, shares.first(blockIdx.x), shares.first(blockIdx.x + 1)};
@@ -271,11 +271,20 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         // ------------------------------------------------------------ copies: one a tile where pages hold whole ones, else one a slice
         const int last_slice = min((p.length + 15) / 16, (p.tile0 + p.tiles) * kWarps);
         Lookup found;
-        for (int i = 0; i < p.tiles; ++i) {
-          if ((i & (whole_tiles ? 31 : 7)) == 0) found.look(a, p, i, whole_tiles, last_slice);
-          if (!dead && !__all_sync(~0u, tc::mbar_wait(empty + stage, phase ^ 1, abort_flag))) dead = true;
-          if (!dead) found.copy<L::kSlice>(a, i, whole_tiles, last_slice - (p.tile0 + i) * kWarps, smem + stage * kWarps * L::kSlice, full + stage, valid + stage);
-          if (++stage == kStages) stage = 0, phase ^= 1;
+        for (int i = 0; i < p.tiles; i += 2) {
+          if (!dead && !__all_sync(~0u, tc::mbar_wait(empty + pair, phase ^ 1, abort_flag))) dead = true;
+          for (int k = 0; k < 2; ++k) {
+            const int t = i + k, at = 2 * pair + k;
+            if (t < p.tiles && (t & (whole_tiles ? 31 : 7)) == 0) found.look(a, p, t, whole_tiles, last_slice);
+            if (dead) continue;
+            if (t < p.tiles) {
+              found.copy<L::kSlice>(a, t, whole_tiles, last_slice - (p.tile0 + t) * kWarps, smem + at * kWarps * L::kSlice, full + pair, valid + at);
+            } else if (lane == 0) {
+              valid[at] = 0;
+              tc::mbar_arrive(full + pair);
+            }
+          }
+          if (++pair == S::kPairs) pair = 0, phase ^= 1;
         }
       } else {
         // ------------------------------------------------------------ products
@@ -307,23 +316,29 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         // tiles whose tokens every row sees, then the others
         const int first = p.tile0 * kTile + 16 * warp, plain = all_see - 16 >= first ? min((all_see - 16 - first) / kTile + 1, p.tiles) : 0;
         auto wait = [&]() {
-          if (!tc::mbar_try_wait(full + stage, phase) && !tc::mbar_wait(full + stage, phase, abort_flag)) dead = true;
+          if (!tc::mbar_try_wait(full + pair, phase) && !tc::mbar_wait(full + pair, phase, abort_flag)) dead = true;
           __syncwarp();
         };
         auto leave = [&]() {
           __syncwarp();
-          if (lane == 0 && !dead) tc::mbar_arrive(empty + stage);
-          if (++stage == kStages) stage = 0, phase ^= 1;
+          if (lane == 0 && !dead) tc::mbar_arrive(empty + pair);
+          if (++pair == S::kPairs) pair = 0, phase ^= 1;
         };
         int i = 0;
-        for (; i < plain; ++i) {
+        for (; i + 1 < plain; i += 2) {
           wait();
-          if (valid[stage] & 1u << warp) take_slice<T, D, G, NT, false>(s, smem + (stage * kWarps + warp) * L::kSlice, 0);
+          const uint8_t* slice = smem + (2 * pair * kWarps + warp) * L::kSlice;
+#pragma unroll 2
+          for (int k = 0; k < 2; ++k)
+            if (valid[2 * pair + k] & 1u << warp) take_slice<T, D, G, NT, false>(s, slice + k * kWarps * L::kSlice, 0);
           leave();
         }
-        for (; i < p.tiles; ++i) {
+        for (; i < p.tiles; i += 2) {
           wait();
-          if (valid[stage] & 1u << warp) take_slice<T, D, G, NT, true>(s, smem + (stage * kWarps + warp) * L::kSlice, first + i * kTile);
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k)
+            if (valid[2 * pair + k] & 1u << warp)
+              take_slice<T, D, G, NT, true>(s, smem + ((2 * pair + k) * kWarps + warp) * L::kSlice, first + (i + k) * kTile);
           leave();
         }
         // ------------------------------------------------------------ the four warps' rows into one
@@ -390,9 +405,9 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
     if (threadIdx.x == 0) *a.status = PSA_ERR_TIMEOUT;
     // copies still in flight must have landed before the block's memory is another's
     if (warp == kWarps && lane == 0)
-      for (int i = 0; i < kStages; ++i) {
+      for (int i = 0; i < S::kPairs; ++i) {
         int unused = 0;
-        tc::mbar_wait(full + i, i < stage ? phase : phase ^ 1, &unused);
+        tc::mbar_wait(full + i, i < pair ? phase : phase ^ 1, &unused);
       }
   }
 }
