@@ -64,14 +64,12 @@ struct Rows {
   int last;                 // keys of the request
 };
 
-template <typename T, int D, int G, int NT, bool MASKED>
-__device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* slice, int t0) {
+// A slice's scores: rows are the tokens r/2 + 4 (r % 2) and that + 8, which lie in rows r and r + 8 of the keys.
+template <typename T, int D, int G, int NT>
+__device__ __forceinline__ void score(float (&x)[NT][4], const Rows<T, D, G, NT>& s, const uint8_t* slice) {
   using L = Kv4<D, G>;
   constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
-  constexpr int kTerms = kWeightTerms<T>;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  // ---- scores: rows are the tokens r/2 + 4 (r % 2) and that + 8, which lie in rows r and r + 8 of the keys
-  float x[NT][4];
   {
     // sum_g lo_g (sum of q over g) is a product too: the parameter words themselves are its operand, a group's step against 0
     const uint8_t* p = slice + L::kParams + (c < NG ? c : 0) * 4;
@@ -86,52 +84,63 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
       }
     }
   }
-  {
-    const Words<NB> k0 = lds<NB>(slice + r * L::kRow + c * NB * 4), k1 = lds<NB>(slice + (r + 8) * L::kRow + c * NB * 4);
-    const Words<NG> p0 = lds<NG>(slice + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kParams + (r + 8) * NG * 4);
+  const Words<NB> k0 = lds<NB>(slice + r * L::kRow + c * NB * 4), k1 = lds<NB>(slice + (r + 8) * L::kRow + c * NB * 4);
+  const Words<NG> p0 = lds<NG>(slice + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kParams + (r + 8) * NG * 4);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float acc[NT][4];
+  for (int g = 0; g < NG; ++g) {
+    float acc[NT][4];
 #pragma unroll
-      for (int i = 0; i < BG; ++i)
+    for (int i = 0; i < BG; ++i)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t w0 = k0.w[g * BG + i], w1 = k1.w[g * BG + i];
-          const uint32_t a[4] = {codes(w0, 2 * k), codes(w1, 2 * k), codes(w0, 2 * k + 1), codes(w1, 2 * k + 1)};
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t w0 = k0.w[g * BG + i], w1 = k1.w[g * BG + i];
+        const uint32_t a[4] = {codes(w0, 2 * k), codes(w1, 2 * k), codes(w0, 2 * k + 1), codes(w1, 2 * k + 1)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (i == 0 && k == 0) mma_new<__half>(acc[nt], a, s.q[nt][g * BG][0]);
-            else MmaOp<__half>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          if (i == 0 && k == 0) mma_new<__half>(acc[nt], a, s.q[nt][g * BG][0]);
+          else MmaOp<__half>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
         }
-      const float s0 = param<T>(p0.w[g]).x, s1 = param<T>(p1.w[g]).x;
+      }
+    const float s0 = param<T>(p0.w[g]).x, s1 = param<T>(p1.w[g]).x;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[nt][j] = fmaf(j < 2 ? s0 : s1, acc[nt][j], x[nt][j]);
-    }
+      for (int j = 0; j < 4; ++j) x[nt][j] = fmaf(j < 2 ? s0 : s1, acc[nt][j], x[nt][j]);
   }
+}
+
+// N slices at once (two hide each other's latencies), the n-th from token t0[n] on.
+template <typename T, int D, int G, int NT, int N, bool MASKED>
+__device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const (&slice)[N], const int (&t0)[N]) {
+  using L = Kv4<D, G>;
+  constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;
+  constexpr int kTerms = kWeightTerms<T>;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  float x[N][NT][4], e[N][NT][4];
+#pragma unroll
+  for (int n = 0; n < N; ++n) score<T, D, G, NT>(x[n], s, slice[n]);
   // ---- the largest step of the values: a lane looks at one group of its two rows
-  const int token = t0 + (r >> 1) + 4 * (r & 1);
-  float widest;
-  {
-    const uint8_t* p = slice + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
+  float widest = 0.f, most = -INFINITY;
+  int token[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    token[n] = t0[n] + (r >> 1) + 4 * (r & 1);
+    const uint8_t* p = slice[n] + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
     float s0 = param<T>(lds<1>(p + r * NG * 4).w[0]).x, s1 = param<T>(lds<1>(p + (r + 8) * NG * 4).w[0]).x;
     if (MASKED) {   // what lies behind the last key may be anything
-      s0 = token < s.last ? s0 : 0.f;
-      s1 = token + 8 < s.last ? s1 : 0.f;
+      s0 = token[n] < s.last ? s0 : 0.f;
+      s1 = token[n] + 8 < s.last ? s1 : 0.f;
     }
-    widest = fmaxf(s0, s1);
+    widest = fmaxf(widest, fmaxf(s0, s1));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        e[n][nt][j] = fmaf(x[n][nt][j], s.factor[nt][j & 1], -s.ref[nt][j & 1]);
+        if (MASKED && token[n] + 8 * (j >> 1) >= s.seen[nt][j & 1]) e[n][nt][j] = -INFINITY;
+        most = fmaxf(most, e[n][nt][j]);
+      }
   }
-  float e[NT][4], most = -INFINITY;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      e[nt][j] = fmaf(x[nt][j], s.factor[nt][j & 1], -s.ref[nt][j & 1]);
-      if (MASKED && token + 8 * (j >> 1) >= s.seen[nt][j & 1]) e[nt][j] = -INFINITY;
-      most = fmaxf(most, e[nt][j]);
-    }
   // ---- the references move seldom: when a weight times a step could leave f16
   if (__any_sync(~0u, widest > s.cap || most > s.limit)) {
 #pragma unroll
@@ -144,8 +153,14 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const bool hide0 = MASKED && token >= s.seen[nt][j], hide1 = MASKED && token + 8 >= s.seen[nt][j];
-        float m = fmaxf(hide0 ? -INFINITY : x[nt][j] * s.factor[nt][j], hide1 ? -INFINITY : x[nt][2 + j] * s.factor[nt][j]);
+        float m = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            e[n][nt][2 * i + j] = MASKED && token[n] + 8 * i >= s.seen[nt][j] ? -INFINITY : x[n][nt][2 * i + j] * s.factor[nt][j];
+            m = fmaxf(m, e[n][nt][2 * i + j]);
+          }
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
@@ -160,71 +175,73 @@ __device__ __forceinline__ void take_slice(Rows<T, D, G, NT>& s, const uint8_t* 
           s.out[nt][i][j] *= fade;
           s.out[nt][i][2 + j] *= fade;
         }
-        e[nt][j] = hide0 ? -INFINITY : fmaf(x[nt][j], s.factor[nt][j], -ref);
-        e[nt][2 + j] = hide1 ? -INFINITY : fmaf(x[nt][2 + j], s.factor[nt][j], -ref);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          e[n][nt][j] -= ref;
+          e[n][nt][2 + j] -= ref;
+        }
       }
   }
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      e[nt][j] = ex2(e[nt][j]);
-      s.sum[nt][j & 1] += e[nt][j];
-    }
-  // ---- outputs: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12); channels 32 b + 4 r + 0..3
-  constexpr int kV = NB / 2;
-  Words<kV> v[4];
-  {
-    const int u = D == 128 ? r ^ ((c >> 1) << 2) : r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = lds<kV>(slice + L::kHalf + (c + 4 * i) * L::kRow + u * NB * 2);
-  }
-  const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
-    // a slice's first eight tokens: lo + s n; the others: hi - s (15 - n)
-    const float ends[2] = {u0.y, fmaf(15.f, u1.x, u1.y)};
-    uint32_t w[kTerms][NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float y[4];
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        y[j] = e[nt][j] * (j < 2 ? u0.x : -u1.x);
-        const float z = e[nt][j] * ends[j >> 1];
-        if (MASKED) {   // nor does what a row does not see count, NaN or not
-          const bool hidden = token + 8 * (j >> 1) >= s.seen[nt][j & 1];
-          y[j] = hidden ? 0.f : y[j];
-          s.mid[nt][g][j & 1] += hidden ? 0.f : z;
-        } else {
-          s.mid[nt][g][j & 1] += z;
-        }
+        e[n][nt][j] = ex2(e[n][nt][j]);
+        s.sum[nt][j & 1] += e[n][nt][j];
       }
+  // ---- outputs: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12); channels 32 b + 4 r + 0..3
+  constexpr int kV = NB / 2;
 #pragma unroll
-      for (int k = 0; k < kTerms; ++k) {
-        float first[4];   // 11 bits, cut off where another term follows
+  for (int n = 0; n < N; ++n) {
+    Words<kV> v[4];
+    {
+      const int u = D == 128 ? r ^ ((c >> 1) << 2) : r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = lds<kV>(slice[n] + L::kHalf + (c + 4 * i) * L::kRow + u * NB * 2);
+    }
+    const Words<NG> p0 = lds<NG>(slice[n] + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice[n] + L::kHalf + L::kParams + (r + 8) * NG * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float2 u0 = param<T>(p0.w[g]), u1 = param<T>(p1.w[g]);
+      // a slice's first eight tokens: lo + s n; the others: hi - s (15 - n)
+      const float ends[2] = {u0.y, fmaf(15.f, u1.x, u1.y)};
+      uint32_t w[kTerms][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          first[j] = k + 1 < kTerms ? __uint_as_float(__float_as_uint(y[j]) & 0xffffe000u) : y[j];
-          y[j] -= first[j];
+          y[j] = e[n][nt][j] * (j < 2 ? u0.x : -u1.x);
+          if (MASKED && token[n] + 8 * (j >> 1) >= s.seen[nt][j & 1]) y[j] = 0.f;   // nor does what a row does not see count, NaN or not
+          else s.mid[nt][g][j & 1] = fmaf(e[n][nt][j], ends[j >> 1], s.mid[nt][g][j & 1]);
         }
-        w[k][nt][0] = movmatrix(MmaOp<__half>::pack(first[0], first[1]));
-        w[k][nt][1] = movmatrix(MmaOp<__half>::pack(first[2], first[3]));
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) {
+          float first[4];   // 11 bits, cut off where another term follows
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            first[j] = k + 1 < kTerms ? __uint_as_float(__float_as_uint(y[j]) & 0xffffe000u) : y[j];
+            y[j] -= first[j];
+          }
+          w[k][nt][0] = movmatrix(MmaOp<__half>::pack(first[0], first[1]));
+          w[k][nt][1] = movmatrix(MmaOp<__half>::pack(first[2], first[3]));
+        }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < BG; ++i) {
-      const int b = g * BG + i;
-      const uint32_t pick = b & 1 ? 0x7632u : 0x5410u;
-      const uint32_t v0 = __byte_perm(v[0].w[b >> 1], v[1].w[b >> 1], pick), v1 = __byte_perm(v[2].w[b >> 1], v[3].w[b >> 1], pick);
+      for (int i = 0; i < BG; ++i) {
+        const int b = g * BG + i;
+        const uint32_t pick = b & 1 ? 0x7632u : 0x5410u;
+        const uint32_t v0 = __byte_perm(v[0].w[b >> 1], v[1].w[b >> 1], pick), v1 = __byte_perm(v[2].w[b >> 1], v[3].w[b >> 1], pick);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t a[4] = {codes(v0, 2 * h), codes(v0, 2 * h + 1), rest(v1, 2 * h), rest(v1, 2 * h + 1)};
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t a[4] = {codes(v0, 2 * h), codes(v0, 2 * h + 1), rest(v1, 2 * h), rest(v1, 2 * h + 1)};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < kTerms; ++k) MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[k][nt]);
+            for (int k = 0; k < kTerms; ++k) MmaOp<__half>::run(s.out[nt][2 * b + h], a, w[k][nt]);
+        }
       }
     }
   }
@@ -236,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   using S = Shape<D, G, NT>;
   using R = Rows<T, D, G, NT>;
   constexpr int NG = L::kGroups, NB = L::kBlocks, kRows = S::kRows, kStages = S::kStages;
+  constexpr bool kJoint = NT == 1;   // two slices' instructions mixed; with 16 rows the registers are not there for it
   extern __shared__ __align__(128) uint8_t smem[];
   float* out_s = reinterpret_cast<float*>(smem + S::kOut);
   float* stats_s = reinterpret_cast<float*>(smem + S::kStats);
@@ -243,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   uint64_t* empty = full + S::kPairs;
   int* scan = reinterpret_cast<int*>(smem + S::kMore);
   volatile int* abort_flag = scan + 8;
-  volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(scan + 9);
+  volatile uint16_t* valid = reinterpret_cast<volatile uint16_t*>(scan + 9);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kPairs; ++i) {
@@ -328,9 +346,20 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         for (; i + 1 < plain; i += 2) {
           wait();
           const uint8_t* slice = smem + (2 * pair * kWarps + warp) * L::kSlice;
-#pragma unroll 2
-          for (int k = 0; k < 2; ++k)
-            if (valid[2 * pair + k] & 1u << warp) take_slice<T, D, G, NT, false>(s, slice + k * kWarps * L::kSlice, 0);
+          const uint32_t there = *reinterpret_cast<volatile const uint32_t*>(valid + 2 * pair) & 0x10001u << warp;   // the slices, a bit each
+          if (kJoint && there == 0x10001u << warp) {
+            const uint8_t* const two[2] = {slice, slice + kWarps * L::kSlice};
+            const int at[2] = {};
+            take<T, D, G, NT, 2, false>(s, two, at);
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k)
+              if (there >> (16 * k) & 0xffff) {
+                const uint8_t* const one[1] = {slice + k * kWarps * L::kSlice};
+                const int at[1] = {};
+                take<T, D, G, NT, 1, false>(s, one, at);
+              }
+          }
           leave();
         }
         for (; i < p.tiles; i += 2) {
@@ -338,7 +367,11 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
 #pragma unroll 1
           for (int k = 0; k < 2; ++k)
             if (valid[2 * pair + k] & 1u << warp)
-              take_slice<T, D, G, NT, true>(s, smem + ((2 * pair + k) * kWarps + warp) * L::kSlice, first + (i + k) * kTile);
+{
+              const uint8_t* const one[1] = {smem + ((2 * pair + k) * kWarps + warp) * L::kSlice};
+              const int at[1] = {first + (i + k) * kTile};
+              take<T, D, G, NT, 1, true>(s, one, at);
+            }
           leave();
         }
         // ------------------------------------------------------------ the four warps' rows into one

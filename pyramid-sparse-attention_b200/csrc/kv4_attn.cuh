@@ -177,6 +177,27 @@ struct Walk {
     return false;
   }
 };
+// Two 32-bit operations in one instruction: the scheduler's slots are what these kernels run out of.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // Codes of nibbles i and i + 4 as two f16 numbers: n 2^-24 for even i, n 2^-20 for odd ones.  (Subnormal numbers: a nibble is a number
 // where it stands, with no exponent to add and no offset to take off again.)
 __device__ __forceinline__ uint32_t codes(uint32_t w, int i) { return (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
@@ -270,13 +291,13 @@ struct Lookup {
     }
   }
   // Tile `tile` of the piece, of which `slices` slices are there, to `to`; valid: a bit for every slice that is.
-  template <int SLICE>
-  __device__ __forceinline__ void copy(const AttnArgs& a, int tile, bool whole, int slices, uint8_t* to, uint64_t* full, volatile uint32_t* valid) const {
+  template <int SLICE, typename V>
+  __device__ __forceinline__ void copy(const AttnArgs& a, int tile, bool whole, int slices, uint8_t* to, uint64_t* full, volatile V* valid) const {
     const int lane = threadIdx.x & 31, k = whole ? tile & 31 : (tile & 7) * kWarps;
     const uint32_t in = (1u << min(kWarps, slices)) - 1, good = __ballot_sync(~0u, from >= 0);
     const uint32_t bits = whole ? (good >> k & 1 ? in : 0u) : good >> k & in;
     if (lane == k) {
-      *valid = bits;
+      *valid = (V)bits;
       tc::mbar_arrive_expect_tx(full, __popc(bits) * SLICE);
     }
     __syncwarp();
