@@ -7,20 +7,24 @@
 //   o_d    = sum_t (p_t s_t) n_td + sum_t p_t lo_t                        the first sum is a product of codes with the weights
 //                                                                         times the step, the second a number per row and group
 //
-// Codes are exact in f16, and so is q times a power of two per row.  The weights times the step are rounded to f16 (11 bits, whatever the
-// tensors' type); the references of the rows keep them in its range.  Half of a slice's tokens enter as hi - s (15 - n): that keeps the
+// Codes are exact in f16, and so is q times a power of two per row.  The weights times the step are rounded to f16 (11 bits; for f16 tensors
+// in two terms); the references of the rows keep them in its range.  Half of a slice's tokens enter as hi - s (15 - n): that keeps the
 // accumulators near zero.  Sums of codes alone would grow with the context, the tensor cores cut their sums off, and what is cut off
 // adds up (0.1 % of an output of 131072 evenly weighted keys).
 //
-// Work: one tile is 64 tokens of one key head, for up to R = 8 NT query rows (new tokens x query heads of that key head).  All tiles of
-// all requests stand in one line, and every block takes an equal stretch of it, computed from the lengths on the device: requests of
-// any mix of lengths load the GPU evenly.  A row's tiles may lie in several blocks; their parts (running maximum, sum, output) are
-// joined in order by a second kernel.  A block: one warp copies slices (16 tokens, contiguous) into a ring, four warps take a slice of
-// each tile.  A slice's bytes go from shared memory to matrix operands with masks and shifts: tokens are the 16 rows of
-// m16n8k16, query rows its 8 columns, and the channel order within a product is whatever the stored words give, the same for q.
+// Work: one tile is 64 tokens of one key head, for up to R query rows (new tokens x query heads of that key head; 8 or 16 here, 32 or 48 in
+// kv4_attn_rows.cu).  All tiles of all requests stand in one line, and every block takes an equal stretch of it, computed from the lengths
+// on the device: requests of any mix of lengths load the GPU evenly.  A row's tiles may lie in several blocks; their parts (running
+// maximum, sum, output) are joined in order by a second kernel.  A block: one warp copies tiles into a ring (one copy where pages hold
+// whole tiles, else one a slice), four warps take a slice of each (16 tokens, contiguous).  A slice's bytes go from shared memory to
+// matrix operands with masks and shifts: tokens are the 16 rows of m16n8k16, query rows its 8 columns, and the channel order within a
+// product is whatever the stored words give, the same for q.
 //
-// The bound is the cache's bytes (160 a token and key head at head_dim 128, groups of 32).  mma.sync and not tcgen05: 8 query rows
-// against 128 rows of a tcgen05 tile, and operands that are made in registers; the products take a fifth of a warp's issue slots.
+// The floor is the cache's bytes (160 a token and key head at head_dim 128, groups of 32).  mma.sync and not tcgen05: 8 query rows
+// against 128 rows of a tcgen05 tile, and operands that are made in registers; the products take a fifth of a warp's issue slots.  8 requests
+// of 131071 tokens, 28 heads on 4, bf16: 134-139 us (5.0 TB/s; 103 us at copy speed).  The copies alone take 104: what bounds it is issue
+// slots, 358 instructions a slice - 88 take the codes apart, 17 are products - at two thirds of a slot a cycle.  Waiting for tiles one by
+// one cost 30 instructions more (149 us), a ring of its own for every warp 170 us, outputs split by channels as in kv4_attn_rows.cu 164.
 #include "kv4_attn.cuh"
 
 namespace psa {
@@ -37,7 +41,7 @@ struct Shape {
   static constexpr int kOut = kStages * kWarps * kSlice;                           // [warps][rows][kOutRow]
   static constexpr int kStats = kOut + kWarps * kRows * kOutRow * 4;               // [warps][rows][2]
   static constexpr int kBars = kStats + kWarps * kRows * 2 * 4;                    // full, empty
-  static constexpr int kMore = kBars + 2 * kStages * 8;                            // valid[stages], scan[8], abort
+  static constexpr int kMore = kBars + 2 * kStages * 8;                            // scan[8], abort, valid[stages]
   static constexpr int kBytes = kMore + (kStages + 16) * 8;
   // scratch: [ctas][2 parts] of output rows and {maximum, sum}
   static constexpr int64_t kPart = (int64_t)kRows * (D + 2);

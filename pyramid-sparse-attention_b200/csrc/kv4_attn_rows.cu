@@ -1,12 +1,16 @@
 // Attention over the 4-bit cache for more than 16 query rows a key head (kv4_attn.cu has the arithmetic, and the kernel for fewer): drafted
 // tokens, pieces of a prompt.
 //
-// A code is decoded once for 16 or 24 rows, in a warp that carries few outputs.  Eight warps share a tile of 64 tokens twice: first a slice's 16 tokens each
-// and half of the rows, for the scores; then 32 channels each (at head_dim 64: 32 channels of two slices) and half of the rows, for the
-// outputs.  The weights times the steps pass through shared memory.  So a warp carries outputs of 32 channels instead of 128, and 16 warps
-// with 24 rows each fit on an SM.  All references of a row are one for the block, and move together.
+// A code is decoded once for 16 or 24 rows, in a warp that carries few outputs.  Eight warps share a tile of 64 tokens twice: first a slice's
+// 16 tokens each and half of the rows, for the scores; then 32 channels each (at head_dim 64: 32 channels of two slices) and half of the
+// rows, for the outputs.  The weights times the steps pass through shared memory.  So a warp carries outputs of 32 channels instead of 128,
+// and 16 warps with 24 rows each fit on an SM.  All references of a row are one for the block, and move together.  The first warp copies
+// tiles ahead: when the block meets between a tile's scores and outputs, the tile before it is done with.
 //
-// The first warp copies tiles ahead: when the block meets between a tile's scores and outputs, the tile before it is done with.
+// 5 requests of 20000 tokens, 6 new ones, 28 heads on 4, head_dim 128, groups of 64: 57 us; units of 16 rows in the other kernel 78, four warps
+// with 48 rows each 78 (168 registers, 8 warps on an SM, 36 % of the issue slots).  At 80000 tokens: 553 instructions for 24 rows and 16
+// tokens, 54 % of the issue slots, tensor pipe 40 % (one m16n8k16 every 8 cycles: 576 TFLOP/s is what mma.sync has).  For 16 rows the other
+// kernel is better (20000 tokens: 34 us, 42 here).
 #include "kv4_attn.cuh"
 
 namespace psa {

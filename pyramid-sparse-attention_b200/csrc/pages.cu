@@ -5,7 +5,8 @@
 // lacks come from the top of the pool of free pages, in the order of the requests, which makes their places an exclusive prefix sum
 // over the requests' needs.  A request that needs pages gets them as long as the running total of all needs up to it fits the pool;
 // the others are given no room at all.  Integers only, and a few thousand of them: a step is bound by the launch and by a chain of
-// dependent loads, not by a rate.
+// dependent loads, not by a rate: 64 requests and one token 3.0 us, 250 requests with 8192 slots each 5.9 us (8.2 MB of slots; 9.4 with a
+// number a thread and a division each).
 #include "psa_common.cuh"
 
 namespace psa {
