@@ -150,7 +150,7 @@ __device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const 
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
     const float old = log2f(s.cap);
-    while (s.cap < widest) s.cap *= 2.f;
+    s.cap = power_above(s.cap, widest);
     const float up = log2f(s.cap);
     s.limit = kHead + kLazy - up;
 #pragma unroll
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
           for (int i = 0; i < 2 * NB; ++i) s.out[nt][i][0] = s.out[nt][i][1] = s.out[nt][i][2] = s.out[nt][i][3] = 0.f;
         }
         s.cap = kLeastCap;
-        s.limit = kHead + kLazy + 24.f;
+        s.limit = kHead + kLazy - kLeastCapLog2;
         s.last = length;
         const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
         // tiles whose tokens every row sees, then the others

@@ -44,7 +44,12 @@ constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has se
 // 2^kHead, and move when a weight times a step could be 2^kLazy times that: f16 has its full precision from 2^-14 to 2^16, so a
 // weight 2^-21 of the largest is still rounded to 11 bits.
 constexpr float kHead = 7.f, kLazy = 8.f;
-constexpr float kLeastCap = 5.9604644775390625e-8f;   // 2^-24
+// Steps from 2^-80 on keep that precision (weights of 2^17 keys times 2^95 still fit 32 bits), and up to 2^100 (below 2^-126 weights are 0).
+constexpr float kLeastCapLog2 = -80.f, kLeastCap = 8.271806125530277e-25f;
+// The smallest power of two that is not below x, or `least` if that is larger.
+__device__ __forceinline__ float power_above(float least, float x) {
+  return x > least ? __uint_as_float((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u) : least;
+}
 // Sums of q are kept in units of scores, 2^-24 of q's operands - in f16, whose numbers end there, 2^12 times that.
 // A weight times a step in one term of 11 bits is as exact as a bf16 output needs (2^-12 of what the codes add, against its 2^-9); an f16
 // output shows it (0.00041 of the output's norm instead of 0.00021), so there it is two terms: 25 products a slice instead of 17.

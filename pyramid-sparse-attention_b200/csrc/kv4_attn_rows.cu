@@ -263,7 +263,7 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
 #pragma unroll
   for (int w = 0; w < kWarps * kHalves; ++w) widest = fmaxf(widest, wide[w]);
   const float old = log2f(s.cap);
-  while (s.cap < widest) s.cap *= 2.f;
+  s.cap = power_above(s.cap, widest);
   const float up = log2f(s.cap);
   s.limit = kHead + kLazy - up;
 #pragma unroll
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT * kHalves)) kv4_att
       for (int j = 0; j < 8; ++j) s.out[nt][j / 4][j % 4] = 0.f;
     }
     s.cap = kLeastCap;
-    s.limit = kHead + kLazy + 24.f;
+    s.limit = kHead + kLazy - kLeastCapLog2;
     __syncthreads();
     const int all_see = p.length - p.count + p.row0 / group + 1;   // keys that every row of the unit sees
     const uint32_t area_at = tc::smem_u32(area);

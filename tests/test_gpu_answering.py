@@ -855,3 +855,12 @@ def test_cache_ties_go_to_the_even_code(ops, dtype):
     want = stands_for(x, 64)
     for y in (k, v):
         assert bool(((y.double() - want).abs() <= HALF[dtype] * 1.001 * want.abs()).all())
+
+
+@pytest.mark.parametrize("H,n", [(7, 1), (12, 1), (10, 3)])
+@pytest.mark.parametrize("v_scale", [1e-20, 1e-12, 1e20, 1e29])
+def test_attention_of_very_large_and_small_values(ops, H, n, v_scale):
+    """Weights times steps stay within f16 wherever the steps are: the references take them along."""
+    g = gen(50)
+    c = Filled(ops, g, [900, 64, 5], 1, 64, 32, torch.bfloat16, 32, v_scale=v_scale)
+    check_attention(ops, randn(g, 3, H, n, 64, dtype=torch.bfloat16), c)
