@@ -864,3 +864,37 @@ def test_attention_of_very_large_and_small_values(ops, H, n, v_scale):
     g = gen(50)
     c = Filled(ops, g, [900, 64, 5], 1, 64, 32, torch.bfloat16, 32, v_scale=v_scale)
     check_attention(ops, randn(g, 3, H, n, 64, dtype=torch.bfloat16), c)
+
+
+def test_rotary_axes_gradients_of_any_layout(ops):
+    """Operands and gradients that cannot be read word by word, or are broadcast, in both orders; k without a gradient, q without one;
+    a second derivative through both operands."""
+    g = gen(51)
+    pos = torch.randint(0, 999, (2, 2, 9), generator=g, device=DEV)
+    ang = angles(pos, (12, 20), 1e4, False, 64)
+    odd = randn(g, 2, 3, 9, 65, dtype=torch.bfloat16).requires_grad_()
+    k = randn(g, 2, 9, 2, 64, dtype=torch.bfloat16).transpose(1, 2).detach().requires_grad_()
+    for q in (odd[..., 1:], odd[..., :64].contiguous()):
+        x, y = ops.rotate_axes(q, k, pos, (12, 20))
+        near_turned(x.detach(), q.detach(), ang, "half")
+        up = randn(g, 2, 1, 9, 1, dtype=torch.bfloat16).expand(-1, 3, -1, 64)
+        down = randn(g, 2, 2, 64, 9, dtype=torch.bfloat16).transpose(2, 3)
+        dq, dk = torch.autograd.grad((x, y), (q, k), (up, down), retain_graph=True)
+        near_turned(dq, up, -ang, "half"), near_turned(dk, down, -ang, "half")
+        (only,) = torch.autograd.grad(y, k, down, retain_graph=True)
+        assert torch.equal(only, dk)
+        x, y = ops.rotate_axes(q.detach(), k, pos, (12, 20))
+        assert torch.equal(torch.autograd.grad((x, y), k, (up, down))[0], dk)
+        x, y = ops.rotate_axes(q, k.detach(), pos, (12, 20))
+        assert torch.equal(torch.autograd.grad((x, y), q, (up, down))[0], dq)
+    a, b = randn(g, 2, 3, 9, 64).requires_grad_(), randn(g, 2, 2, 9, 64).requires_grad_()
+    x, y = ops.rotate_axes(a, b, pos, (12, 20), layout="pairs")
+    da, db = torch.autograd.grad((x.pow(3).sum() + y.pow(2).sum()), (a, b), create_graph=True)
+    (daa,) = torch.autograd.grad(da.sum(), a)
+    # d/da sum(R^T 3 (R a)^2) = R^T (6 (R a) * R 1)
+    ones = torch.ones_like(a)
+    r1 = turned(ones, ang, "pairs")
+    want = turned(6 * turned(a.detach(), ang, "pairs") * r1, -ang, "pairs")
+    assert float((daa.double() - want).abs().max()) < 2.0 ** -18 * float(want.abs().max())      # four rotations, 2^-21 each (near_turned)
+    assert float((db.detach() - 2 * b.detach()).abs().max()) < 2.0 ** -17                       # R^T 2 R b; |b| up to about 5
+    ops.check_status()
