@@ -529,7 +529,7 @@ constexpr int kMostSms = 160;   // parts of the scratch are laid out for them
 // Rows of a unit: as few units as 48 rows each make, and no more rows than they need.
 int rows_per_tile(int64_t rows) {
   const int64_t most = cdiv64(rows, cdiv64(rows, 48));
-  return most <= 8 ? 8 : most <= 16 ? 16 : most <= 32 ? 32 : 48;
+  return most <= 8 ? 8 : most <= 16 ? 16 : most <= 24 ? 24 : most <= 32 ? 32 : 48;
 }
 // What a unit's beginning and end cost, in tiles (33 requests of 17 to 16384 tokens, 16 key heads of 64 channels: 87 us with 1, 62 with 2, 46
 // with 4, 41 with 8, 45 with 12; 4 key heads of 128 with 5 tokens: 74 us with 2, 64 with 3, 63 with 4).

@@ -16,16 +16,16 @@
 namespace psa {
 namespace {
 
-constexpr int kHalves = 2, kThreads = 32 * kWarps * kHalves;
-
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, int HALVES>
 struct Shape {
   using L = Kv4<D, G>;
+  static constexpr int kHalves = HALVES, kThreads = 32 * kWarps * HALVES;
   static constexpr int kTiles = NT * kHalves, kRows = 8 * kTiles, kTerms = kWeightTerms<T>;   // 8-row tiles
-  static constexpr int kTileBytes = kWarps * L::kSlice, kStages = D == 128 ? 4 : 6;
+  static constexpr int kTileBytes = kWarps * L::kSlice;
   static constexpr int kParts = kWarps / L::kBlocks;                               // warps that share a block of channels and its rows
   // Weights times the steps of a group: [terms][groups][slices][kTiles] matrices of 16 tokens x 8 rows.  Two buffers spare a barrier a tile.
-  static constexpr int kWeights = kTerms * L::kGroups * kWarps * kTiles * 256, kBuffers = kWeights <= 16384 ? 2 : 1;
+  static constexpr int kWeights = kTerms * L::kGroups * kWarps * kTiles * 256, kBuffers = kWeights <= 8192 * HALVES ? 2 : 1;
+  static constexpr int kStages = HALVES == 2 ? (D == 128 ? 4 : 6) : D == 64 ? 5 : kWeights > 16384 ? 2 : 3;   // tiles of the ring
   static constexpr int kOutRow = D + 4;                                            // floats; 4 more spread the banks
   static constexpr int kOuts = kParts * kRows * kOutRow * 4;                       // after the last tile: [parts][rows][kOutRow],
   static constexpr int kTotals = kWarps * (L::kGroups + 1) * kRows * 4;            // [slices][middle values of the groups, sums][rows]
@@ -68,10 +68,10 @@ struct Rows {
 };
 
 // Scores of a slice's 16 tokens and the warp's rows, from 8-row tile `tile0` on: rows of x are the tokens r/2 + 4 (r % 2) and that + 8.
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, int HALVES>
 __device__ __forceinline__ void score(float (&x)[NT][4], int tile0, const uint8_t* smem, const uint8_t* slice) {
   using L = Kv4<D, G>;
-  using S = Shape<T, D, G, NT>;
+  using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   {
@@ -121,11 +121,11 @@ __device__ __forceinline__ void score(float (&x)[NT][4], int tile0, const uint8_
 
 // Weights e of a slice's tokens: into the sums and the shares of the middle values (count), and times the steps of each group to `to`, the
 // place of the slice's first matrix of the warp's rows.  MASKED: nothing that a row does not see counts, NaN or not.
-template <typename T, int D, int G, int NT, bool MASKED>
+template <typename T, int D, int G, int NT, int HALVES, bool MASKED>
 __device__ __forceinline__ void weigh(Rows<T, D, G, NT>& s, const float (&e)[NT][4], bool count, const float4* columns, const uint8_t* slice, int token,
                                       uint32_t to) {
   using L = Kv4<D, G>;
-  using S = Shape<T, D, G, NT>;
+  using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = L::kGroups, kTerms = S::kTerms, kGroup = kWarps * S::kTiles * 256, kTerm = NG * kGroup;
   const int lane = threadIdx.x & 31, r = lane >> 2;
   const Words<NG> p0 = lds<NG>(slice + L::kHalf + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kHalf + L::kParams + (r + 8) * NG * 4);
@@ -187,15 +187,15 @@ __device__ __forceinline__ void weigh(Rows<T, D, G, NT>& s, const float (&e)[NT]
 
 // Scores and weights of the warp's 16 tokens of a tile; true, and scores times factors in e, where a weight times a step could leave f16 and
 // the references have to move first - which is seldom.
-template <typename T, int D, int G, int NT, bool MASKED>
+template <typename T, int D, int G, int NT, int HALVES, bool MASKED>
 __device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4], int tile0, uint8_t* smem, const uint8_t* slice, int token, int length,
                                           uint32_t to) {
   using L = Kv4<D, G>;
-  using S = Shape<T, D, G, NT>;
+  using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = L::kGroups;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const float4* columns = reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c;   // of rows 2 c and 2 c + 1
-  score<T, D, G, NT>(e, tile0, smem, slice);
+  score<T, D, G, NT, HALVES>(e, tile0, smem, slice);
   // the largest step of the values: a lane looks at one group of its two rows
   float widest, most = -INFINITY;
   {
@@ -245,23 +245,23 @@ __device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) e[nt][j] = ex2(t[nt][j]);
-    weigh<T, D, G, NT, MASKED>(s, e, true, columns, slice, token, to);
+    weigh<T, D, G, NT, HALVES, MASKED>(s, e, true, columns, slice, token, to);
   }
   return rises;
 }
 
 // All warps' references to where the ones that rise want them, and this warp's weights again.
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, int HALVES>
 __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], bool rises, int tile0, uint8_t* smem, const uint8_t* slice, int token,
                                       uint32_t to) {
-  using S = Shape<T, D, G, NT>;
+  using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = D / G;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
   float* rise = reinterpret_cast<float*>(smem + S::kRise) + 8 * tile0;
   float* wide = reinterpret_cast<float*>(smem + S::kWide);
   float widest = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps * kHalves; ++w) widest = fmaxf(widest, wide[w]);
+  for (int w = 0; w < kWarps * HALVES; ++w) widest = fmaxf(widest, wide[w]);
   const float old = log2f(s.cap);
   s.cap = power_above(s.cap, widest);
   const float up = log2f(s.cap);
@@ -288,7 +288,7 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
       e[nt][j] = rises ? ex2(e[nt][j] - ref) : e[nt][j] * fade;
       e[nt][2 + j] = rises ? ex2(e[nt][2 + j] - ref) : e[nt][2 + j] * fade;
     }
-  weigh<T, D, G, NT, true>(s, e, rises, reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c, slice, token, to);
+  weigh<T, D, G, NT, HALVES, true>(s, e, rises, reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c, slice, token, to);
   __syncthreads();
   if (rises) {   // nothing asked for any more
     for (int i = lane; i < 8 * NT; i += 32) rise[warp % kWarps * S::kRows + i] = -INFINITY;
@@ -298,10 +298,10 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
 
 // Outputs of the warp's 32 channels and rows from its slices of a tile: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12).
 // weights: the first matrix of the warp's rows.
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, int HALVES>
 __device__ __forceinline__ void collect(Rows<T, D, G, NT>& s, const uint8_t* tile, uint32_t weights) {
   using L = Kv4<D, G>;
-  using S = Shape<T, D, G, NT>;
+  using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = L::kGroups, NB = L::kBlocks, kTerms = S::kTerms, kSlices = kWarps / S::kParts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32 % kWarps, r = lane >> 2, c = lane & 3, b = warp % NB, first = warp / NB * kSlices;
   const uint8_t* v = tile + first * L::kSlice + L::kHalf + (((D == 128 ? r ^ ((c >> 1) << 2) : r) * NB + b) * 2) + c * L::kRow;
@@ -337,11 +337,11 @@ struct Ahead {
   int next, last_slice;
 };
 
-template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_of(8 * NT * kHalves)) kv4_attn_rows_kernel(const __grid_constant__ AttnArgs a) {
+template <typename T, int D, int G, int NT, int HALVES>
+__global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVES)) kv4_attn_rows_kernel(const __grid_constant__ AttnArgs a) {
   using L = Kv4<D, G>;
-  using S = Shape<T, D, G, NT>;
-  constexpr int NG = L::kGroups, NB = L::kBlocks, kRows = S::kRows, kStages = S::kStages;
+  using S = Shape<T, D, G, NT, HALVES>;
+  constexpr int NG = L::kGroups, NB = L::kBlocks, kRows = S::kRows, kStages = S::kStages, kHalves = HALVES, kThreads = S::kThreads;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Ahead ahead;
   uint8_t* area = smem + kStages * S::kTileBytes;
@@ -446,13 +446,13 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT * kHalves)) kv4_att
       const uint32_t weights = area_at + (S::kBuffers == 2 && (i & 1) ? S::kWeights : 0) + tile0 * 256, to = weights + own * (S::kTiles * 256);
       float e[NT][4];
       if (S::kBuffers == 1 && i) __syncthreads();                          // the weights before have been used
-      const bool rises = there && t0 + 16 <= all_see ? first_try<T, D, G, NT, false>(s, e, tile0, smem, slice, token, p.length, to)
-                                                     : first_try<T, D, G, NT, true>(s, e, tile0, smem, slice, token, p.length, to);
+      const bool rises = there && t0 + 16 <= all_see ? first_try<T, D, G, NT, HALVES, false>(s, e, tile0, smem, slice, token, p.length, to)
+                                                     : first_try<T, D, G, NT, HALVES, true>(s, e, tile0, smem, slice, token, p.length, to);
       const bool move = __syncthreads_or(rises);
       if (warp == 0 && behind && !dead) copy_next(stage ? stage - 1 : kStages - 1);
       behind = true;
-      if (__builtin_expect(move, 0)) raise<T, D, G, NT>(s, e, rises, tile0, smem, slice, token, to);
-      collect<T, D, G, NT>(s, tile, weights);
+      if (__builtin_expect(move, 0)) raise<T, D, G, NT, HALVES>(s, e, rises, tile0, smem, slice, token, to);
+      collect<T, D, G, NT, HALVES>(s, tile, weights);
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
     // ------------------------------------------------------------ the warps' shares of the rows
@@ -516,10 +516,10 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT * kHalves)) kv4_att
   }
 }
 
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, int HALVES>
 int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
-  using S = Shape<T, D, G, NT>;
-  auto kernel = kv4_attn_rows_kernel<T, D, G, NT>;
+  using S = Shape<T, D, G, NT, HALVES>;
+  auto kernel = kv4_attn_rows_kernel<T, D, G, NT, HALVES>;
   static thread_local uint64_t ready = 0;   // devices that know the kernel's shared memory, per thread
   int dev = 0;
   cudaGetDevice(&dev);
@@ -530,7 +530,7 @@ int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
     }
     if (dev < 64) ready |= (uint64_t)1 << dev;
   }
-  kernel<<<sms * blocks_of(S::kRows), kThreads, S::kBytes, st>>>(a);
+  kernel<<<sms * blocks_of(S::kRows), S::kThreads, S::kBytes, st>>>(a);
   PSA_CHECK_LAUNCH("psa_kv4_attention");
   return PSA_OK;
 }
@@ -539,7 +539,7 @@ int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
 
 template <typename T, int D, int G>
 int launch_rows(const AttnArgs& a, int sms, int rows_per_tile, cudaStream_t st) {
-  return rows_per_tile == 32 ? launch_tiles<T, D, G, 2>(a, sms, st) : launch_tiles<T, D, G, 3>(a, sms, st);
+  return rows_per_tile == 24 ? launch_tiles<T, D, G, 3, 1>(a, sms, st) : rows_per_tile == 32 ? launch_tiles<T, D, G, 2, 2>(a, sms, st) : launch_tiles<T, D, G, 3, 2>(a, sms, st);
 }
 #define PSA_ROWS(T, D, G) template int launch_rows<T, D, G>(const AttnArgs&, int, int, cudaStream_t)
 #define PSA_ROWS_OF(T) PSA_ROWS(T, 64, 32); PSA_ROWS(T, 64, 64); PSA_ROWS(T, 128, 32); PSA_ROWS(T, 128, 64); PSA_ROWS(T, 128, 128)
