@@ -313,6 +313,6 @@ struct Lookup {
 
 // The kernel for more than 16 rows a key head (kv4_attn_rows.cu), launched.
 template <typename T, int D, int G> int launch_rows(const AttnArgs& a, int sms, int rows_per_tile, cudaStream_t st);
-__host__ __device__ constexpr int blocks_of(int rows) { return rows <= 8 ? 3 : rows == 24 ? 4 : 2; }   // of an SM, by the registers that rows take
+__host__ __device__ constexpr int blocks_of(int rows) { return rows <= 8 ? 3 : rows == 24 ? 4 : rows == 32 ? 3 : 2; }   // of an SM, by the registers that rows take
 
 }  // namespace psa

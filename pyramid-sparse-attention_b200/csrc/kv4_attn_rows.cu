@@ -1,16 +1,17 @@
 // Attention over the 4-bit cache for more than 16 query rows a key head (kv4_attn.cu has the arithmetic, and the kernel for fewer): drafted
 // tokens, pieces of a prompt.
 //
-// A code is decoded once for 16 or 24 rows, in a warp that carries few outputs.  Eight warps share a tile of 64 tokens twice: first a slice's
-// 16 tokens each and half of the rows, for the scores; then 32 channels each (at head_dim 64: 32 channels of two slices) and half of the
-// rows, for the outputs.  The weights times the steps pass through shared memory.  So a warp carries outputs of 32 channels instead of 128,
-// and 16 warps with 24 rows each fit on an SM.  All references of a row are one for the block, and move together.  The first warp copies
-// tiles ahead: when the block meets between a tile's scores and outputs, the tile before it is done with.
+// A code is decoded once for 24 or 32 rows, in a warp that carries few outputs.  Four warps share a tile of 64 tokens twice: first a slice's 16
+// tokens each, for the scores; then 32 channels each (at head_dim 64: 32 channels of two slices), for the outputs.  The weights times the
+// steps pass through shared memory.  So a warp carries outputs of 32 channels instead of 128: 16 warps with 24 rows each fit on an SM, or
+// 12 with 32; for 48 rows eight warps take half of them each.  All references of a row are one for the block, and move together.  The first
+// warp copies tiles ahead: when the block meets between a tile's scores and outputs, the tile before it is done with.
 //
-// 5 requests of 20000 tokens, 6 new ones, 28 heads on 4, head_dim 128, groups of 64: 57 us; units of 16 rows in the other kernel 78, four warps
-// with 48 rows each 78 (168 registers, 8 warps on an SM, 36 % of the issue slots).  At 80000 tokens: 553 instructions for 24 rows and 16
-// tokens, 54 % of the issue slots, tensor pipe 40 % (one m16n8k16 every 8 cycles: 576 TFLOP/s is what mma.sync has).  For 16 rows the other
-// kernel is better (20000 tokens: 34 us, 42 here).
+// 5 requests of 20000 tokens, 28 heads on 4, head_dim 128, groups of 64, bf16: 3 new tokens 37 us (as 32 rows 45, as two units of 16 in the other
+// kernel 53), 4 new ones 48 (eight warps with 16 rows each 50), 6 new ones 57 (as two units of 24 59; units of 16 in the other kernel 78;
+// four warps with 48 rows each 78: 168 registers, 8 warps on an SM, 36 % of the issue slots).  6 at 80000 tokens: 485 instructions for 24
+// rows and 16 tokens, half of the issue slots, tensor pipe 42 % (one m16n8k16 every 8 cycles: 576 TFLOP/s is what mma.sync has).  For 16
+// rows the other kernel is as good (32 us, 33 here).
 #include "kv4_attn.cuh"
 
 namespace psa {
@@ -539,7 +540,7 @@ int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
 
 template <typename T, int D, int G>
 int launch_rows(const AttnArgs& a, int sms, int rows_per_tile, cudaStream_t st) {
-  return rows_per_tile == 24 ? launch_tiles<T, D, G, 3, 1>(a, sms, st) : rows_per_tile == 32 ? launch_tiles<T, D, G, 2, 2>(a, sms, st) : launch_tiles<T, D, G, 3, 2>(a, sms, st);
+  return rows_per_tile == 24 ? launch_tiles<T, D, G, 3, 1>(a, sms, st) : rows_per_tile == 32 ? launch_tiles<T, D, G, 4, 1>(a, sms, st) : launch_tiles<T, D, G, 3, 2>(a, sms, st);
 }
 #define PSA_ROWS(T, D, G) template int launch_rows<T, D, G>(const AttnArgs&, int, int, cudaStream_t)
 #define PSA_ROWS_OF(T) PSA_ROWS(T, 64, 32); PSA_ROWS(T, 64, 64); PSA_ROWS(T, 128, 32); PSA_ROWS(T, 128, 64); PSA_ROWS(T, 128, 128)
