@@ -6,8 +6,9 @@
 // misses by 15 units of its last place at most, an eighth of a step in bf16).  A group that holds an infinity or a NaN, or
 // whose range does not fit 32 bits, reads as NaN.
 //
-// The floor is HBM, 86 MB and 13.1 us each way for 32761 tokens of 4 heads x 128.  Reading takes 15.9 us.  Appending takes 24.6, bound by
-// instructions (about 600 a thread for 32 values; 72 % of the issue slots): unpacking, two sums and a product a value, the extrema.
+// The floor is HBM, 86 MB and 13.1 us each way for 32761 tokens of 4 heads x 128.  Reading takes 15.1 us.  Appending takes 23.1, bound by
+// instructions (some 560 a thread for 32 values; 72 % of the issue slots): unpacking, two sums and a product a value, the extrema.
+// (Divisions by page sizes and numbers of tokens that need none cost 1.5 us each way.)
 #include "kv4.cuh"
 
 namespace psa {
@@ -21,7 +22,8 @@ struct CacheArgs {
   const int32_t* slots;        // [batch][tokens]
   int32_t* status;
   int64_t batch, tokens, slots_total;
-  int heads, page;
+  int64_t head_bytes, page_bytes;   // of the cache
+  int heads, page, shift;           // shift: of a page that is a power of two, or -1
 };
 
 // A quotient of which only the rounded value counts, as a product with the inverse.  The inverse is off by 2^-24 of itself at most, the
@@ -66,9 +68,9 @@ struct Slot {
     const int slot = a.slots[in ? row : 0];
     good = in && slot >= 0 && slot < a.slots_total;
     if (in && !good && slot != -1) *a.status = PSA_ERR_ARG;
-    const int page = good ? slot / a.page : 0, at = good ? slot - page * a.page : 0;
-    slice = ((int64_t)page * a.heads * (a.page / 16) + at / 16) * slice_bytes;
-    place = at & 15;
+    const uint32_t of = good ? (uint32_t)slot : 0u, page = a.shift >= 0 ? of >> a.shift : of / (uint32_t)a.page, at = of - page * (uint32_t)a.page;
+    slice = page * a.page_bytes + (int)(at / 16 * (uint32_t)slice_bytes);
+    place = (int)(at & 15);
   }
 };
 template <int D, int G, int HS>
@@ -83,10 +85,10 @@ struct Rows {
     u = threadIdx.x % (D / 8);
     head0 = blockIdx.y * kHeads;
     heads = a.heads - head0;
-    apart = (int64_t)(a.page / 16) * Kv4<D, G>::kSlice;
+    apart = a.head_bytes;
     stride = strides[1];
     const uint32_t row = (blockIdx.x * (256 / (D / 8)) + threadIdx.x / (D / 8)) * kTokens;
-    uint32_t b = row / (uint32_t)a.tokens, t = row - b * (uint32_t)a.tokens;
+    uint32_t b = a.batch == 1 ? 0u : row / (uint32_t)a.tokens, t = row - b * (uint32_t)a.tokens;
 #pragma unroll
     for (int k = 0; k < kTokens; ++k) {
       const Slot s(a, row + k, Kv4<D, G>::kSlice);
@@ -243,7 +245,7 @@ int check(const char* what, const void* data, const void* k, const void* v, cons
 
 int heads_shift(int heads) { return heads >= 3 ? 2 : heads - 1; }
 
-CacheArgs arguments(const void* data, const int64_t* strides, const int32_t* slots, int64_t pages, int heads, int page, int64_t batch,
+CacheArgs arguments(const void* data, const int64_t* strides, const int32_t* slots, int64_t pages, int heads, int page, int slice_bytes, int64_t batch,
                     int64_t tokens, int32_t* status) {
   CacheArgs a = {};
   a.data = static_cast<uint8_t*>(const_cast<void*>(data));
@@ -255,6 +257,11 @@ CacheArgs arguments(const void* data, const int64_t* strides, const int32_t* slo
   a.slots_total = pages * page;
   a.heads = heads;
   a.page = page;
+  a.head_bytes = (int64_t)(page / 16) * slice_bytes;
+  a.page_bytes = heads * a.head_bytes;
+  a.shift = -1;
+  if ((page & (page - 1)) == 0)
+    for (a.shift = 0; 1 << a.shift < page;) ++a.shift;
   return a;
 }
 
@@ -269,7 +276,7 @@ extern "C" int psa_kv4_append(void* data, const void* k, const void* v, const in
                               int page_size, int64_t batch, int64_t tokens, int head_dim, int group, int dtype, int32_t* status, void* stream) {
   using namespace psa;
   if (int rc = check("psa_kv4_append", data, k, v, strides, slots, pages, kv_heads, page_size, batch, tokens, head_dim, group, dtype, status)) return rc;
-  CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, batch, tokens, status);
+  CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, psa::kv4_slice_bytes(head_dim, group), batch, tokens, status);
   a.src[0] = k;
   a.src[1] = v;
   const int hs = heads_shift(kv_heads);
@@ -285,7 +292,7 @@ extern "C" int psa_kv4_read(const void* data, void* k, void* v, const int64_t* s
                             int page_size, int64_t batch, int64_t tokens, int head_dim, int group, int dtype, int32_t* status, void* stream) {
   using namespace psa;
   if (int rc = check("psa_kv4_read", data, k, v, strides, slots, pages, kv_heads, page_size, batch, tokens, head_dim, group, dtype, status)) return rc;
-  CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, batch, tokens, status);
+  CacheArgs a = arguments(data, strides, slots, pages, kv_heads, page_size, psa::kv4_slice_bytes(head_dim, group), batch, tokens, status);
   a.dst[0] = k;
   a.dst[1] = v;
   const int hs = heads_shift(kv_heads);
