@@ -372,8 +372,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
     if (ahead.next == ahead.piece.tiles) {
       __syncwarp();
       Walk w = ahead.walk;
-      Piece p;
-      p.tiles = 0;
+      Piece p = {};
       const bool more = w.next(a, kRows, p);
       __syncwarp();
       if (lane == 0) {

@@ -898,3 +898,36 @@ def test_rotary_axes_gradients_of_any_layout(ops):
     assert float((daa.double() - want).abs().max()) < 2.0 ** -18 * float(want.abs().max())      # four rotations, 2^-21 each (near_turned)
     assert float((db.detach() - 2 * b.detach()).abs().max()) < 2.0 ** -17                       # R^T 2 R b; |b| up to about 5
     ops.check_status()
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("H,n", [(3, 1), (12, 1), (7, 3), (10, 3), (12, 4)])
+def test_attention_skips_bad_pages_wherever_they_are(ops, page, H, n):
+    """Page numbers that the cache does not have, alone and next to each other, first and last of a request: their tokens are hidden, all
+    others' outputs are those without them; a request of bad pages alone gives rows of nothing."""
+    g = gen(60 + page)
+    c = Filled(ops, g, [700, 130, 900, 60], 1, 128, 64, torch.bfloat16, page)
+    q = randn(g, 4, H, n, 128, dtype=torch.bfloat16)
+    bad = c.table.clone()
+    for b, entries in ((0, (0, 2, 3, 4)), (1, (1,)), (2, (1, 3, 6))):
+        for e in entries:
+            if e * page < c.lengths[b]:
+                bad[b, e] = (-1, 10 ** 6, c.data.shape[0])[e % 3]
+    bad[3] = -5
+    got, lse = ops.kv4_attention(q, c.data, bad, c.len, 64, return_lse=True)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    k, v = (stands_for(x, 64)[:, 0] for x in (c.k, c.v))
+    for b in range(4):
+        L = c.lengths[b]
+        hidden = ((bad[b] < 0) | (bad[b] >= c.data.shape[0])).repeat_interleave(page)[:L]
+        s = q[b].double() @ k[b, :L].T * 128 ** -0.5
+        s = s.masked_fill(hidden | (torch.arange(L, device=DEV) > L - n + torch.arange(n, device=DEV)[:, None]), -math.inf)
+        if bool(hidden.all()):
+            assert not bool(got[b].any()) and bool((lse[b] == -math.inf).all())
+            continue
+        want = torch.softmax(s, -1) @ v[b, :L]
+        size = torch.softmax(s, -1) @ v[b, :L].abs()
+        # bf16's half step, the weights' 2^-11 on what the codes add (at most 8 / 15 of a group's range, twice the values' size), scores to 2^-9
+        assert bool(((got[b].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * size + 2.0 ** -10 * v[b, :L].abs().amax()).all())
+    assert not bool(got.isnan().any())
