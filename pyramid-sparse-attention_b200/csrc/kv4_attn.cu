@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   constexpr int NG = L::kGroups, NB = L::kBlocks, kRows = S::kRows, kStages = S::kStages;
   constexpr bool kJoint = NT == 1;   // two slices' instructions mixed; with 16 rows the registers are not there for it
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Piece piece;   // of the four warps
   float* out_s = reinterpret_cast<float*>(smem + S::kOut);
   float* stats_s = reinterpret_cast<float*>(smem + S::kStats);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -287,9 +288,10 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   uint32_t phase = 0;
   bool dead = false;   // a wait ran out: nothing is copied or handed back any more, and what is computed does not count
   Walk walk = {request, base, shares.first(blockIdx.x), shares.first(blockIdx.x + 1)};
-  Piece p;
-  while (walk.next(a, kRows, p)) {
+  while (true) {
       if (warp == kWarps) {
+        Piece p;
+        if (!walk.next(a, kRows, p)) break;
         // ------------------------------------------------------------ copies: one a tile where pages hold whole ones, else one a slice
         const int last_slice = min((p.length + 15) / 16, (p.tile0 + p.tiles) * kWarps);
         Lookup found;
@@ -310,6 +312,14 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         }
       } else {
         // ------------------------------------------------------------ products
+        if (warp == 0) {
+          Piece next;
+          if (!walk.next(a, kRows, next)) next.tiles = 0;
+          if (lane == 0) piece = next;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+        const Piece& p = piece;   // read where it is needed: registers are what is short
+        if (p.tiles == 0) break;
         R s;
         const int r = lane >> 2, c = lane & 3, length = p.length, count = p.count, row0 = p.row0;
         const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + 8 * c;
@@ -467,6 +477,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const __grid_con
   if (i < count && span.tiles) {
     owners = a.owners[((int64_t)b * a.kv_heads + head / group) * a.row_tiles + row / rows_per_tile];
     if (owners.x == owners.y) return;
+    owners = make_int2(max(owners.x, 0), min(owners.y, a.blocks - 1));
   }
   const int64_t size = (int64_t)rows_per_tile * (D + 2);
   float top = kLowest, sum = 0.f;
@@ -539,7 +550,7 @@ int least_cells(int rows) { return rows > 16 ? 1 : 2; }
 size_t owners_bytes(int64_t batch, int kv_heads, int64_t row_tiles) { return ((size_t)batch * kv_heads * row_tiles * sizeof(int2) + 255) & ~(size_t)255; }
 
 template <typename T, int D, int G, int NT>
-int launch_few(const AttnArgs& a, int sms, cudaStream_t st) {
+int launch_few(const AttnArgs& a, cudaStream_t st) {
   using S = Shape<D, G, NT>;
   auto kernel = kv4_attn_kernel<T, D, G, NT>;
   static thread_local uint64_t ready = 0;   // devices that know the kernel's shared memory, per thread
@@ -552,14 +563,13 @@ int launch_few(const AttnArgs& a, int sms, cudaStream_t st) {
     }
     if (dev < 64) ready |= (uint64_t)1 << dev;
   }
-  kernel<<<sms * blocks_of(S::kRows), kThreads, S::kBytes, st>>>(a);
+  kernel<<<a.blocks, kThreads, S::kBytes, st>>>(a);
   PSA_CHECK_LAUNCH("psa_kv4_attention");
   return PSA_OK;
 }
 template <typename T, int D, int G>
 int launch(const AttnArgs& a, int rows, cudaStream_t st) {
-  const int sms = sm_count() < kMostSms ? sm_count() : kMostSms;
-  const int first = rows == 8 ? launch_few<T, D, G, 1>(a, sms, st) : rows == 16 ? launch_few<T, D, G, 2>(a, sms, st) : launch_rows<T, D, G>(a, sms, rows, st);
+  const int first = rows == 8 ? launch_few<T, D, G, 1>(a, st) : rows == 16 ? launch_few<T, D, G, 2>(a, st) : launch_rows<T, D, G>(a, rows, st);
   if (first != PSA_OK) return first;
   const dim3 grid((unsigned)a.tokens, (unsigned)a.heads, (unsigned)a.batch);
   cudaLaunchConfig_t how = {};
@@ -634,6 +644,7 @@ extern "C" int psa_kv4_attention(const void* q, const int64_t* q_strides, const 
   const int64_t rows = tokens * (heads / kv_heads);
   a.unit_cells = unit_cells(head_dim, rows_per_tile(rows));
   a.least_cells = least_cells(rows_per_tile(rows));
+  a.blocks = (sm_count() < kMostSms ? sm_count() : kMostSms) * blocks_of(rows_per_tile(rows));
   a.row_tiles = (int)cdiv64(rows, rows_per_tile(rows));
   PSA_REQUIRE(rows < ((int64_t)1 << 31), PSA_ERR_ARG, "psa_kv4_attention: %lld rows a key head", (long long)rows);
   PSA_REQUIRE((double)batch * (cdiv64(width * page_size, kTile) + a.unit_cells) * a.row_tiles * kv_heads < 2147483648.0, PSA_ERR_UNSUPPORTED,

@@ -23,6 +23,7 @@ struct AttnArgs {
   int unit_cells;      // what a unit's beginning and end cost, in tiles
   int least_cells;     // a block takes at least so many
   int row_tiles;       // of a request that brings all `tokens`
+  int blocks;          // of the first kernel
   int2* owners;        // [batch][kv_heads][row_tiles]: first and last block of a unit (rows of a tile x a key head)
   float* parts;        // [blocks][2]: what a block has of a unit that began before it, and of one that goes on behind it
 };
@@ -118,6 +119,8 @@ __device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int
   // whose tile it is: requests in rounds of one a thread
   const int first = shares.first(blockIdx.x);
   int before = 0;
+  if (threadIdx.x == 0) scan[THREADS / 32] = scan[THREADS / 32 + 1] = 0;
+  __syncthreads();
   for (int b0 = 0;; b0 += THREADS) {
     int own = own0;
     if (a.batch > THREADS) {
@@ -143,7 +146,7 @@ __device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int
       scan[THREADS / 32] = b0 + threadIdx.x;
       scan[THREADS / 32 + 1] = start;
     }
-    if (before > first) break;
+    if (before > first || b0 + THREADS >= a.batch) break;
   }
   __syncthreads();
   request = scan[THREADS / 32];
@@ -151,6 +154,9 @@ __device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int
   return work;
 }
 
+// Lengths that another stream changes meanwhile give wrong outputs, but no wait without end and no access out of range: one warp reads
+// them for those that meet at barriers, requests and blocks are bounded by what there is, and waits for tiles run out.
+//
 // What a block has of a unit: tiles tile0 .. tile0 + tiles - 1 of key head `head` for the rows from row0 on.
 struct Piece {
   int b, head, row0, rows, tile0, tiles, all_tiles, length, count;
@@ -159,7 +165,7 @@ struct Piece {
 struct Walk {
   int b, base, at, last;   // the next cell, the block's end, the request it lies in and where that begins
   __device__ __forceinline__ bool next(const AttnArgs& a, int rows_per_tile, Piece& p) {
-    while (at < last) {
+    while (at < last && b < a.batch) {
       const Span span = span_of(a, b, rows_per_tile, p.length, p.count);
       if (at >= base + span.work) {
         base += span.work;
@@ -312,7 +318,7 @@ struct Lookup {
 };
 
 // The kernel for more than 16 rows a key head (kv4_attn_rows.cu), launched.
-template <typename T, int D, int G> int launch_rows(const AttnArgs& a, int sms, int rows_per_tile, cudaStream_t st);
+template <typename T, int D, int G> int launch_rows(const AttnArgs& a, int rows_per_tile, cudaStream_t st);
 __host__ __device__ constexpr int blocks_of(int rows) { return rows <= 8 ? 3 : rows == 24 ? 4 : rows == 32 ? 3 : 2; }   // of an SM, by the registers that rows take
 
 }  // namespace psa

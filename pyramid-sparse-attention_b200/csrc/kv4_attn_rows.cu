@@ -345,6 +345,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
   constexpr int NG = L::kGroups, NB = L::kBlocks, kRows = S::kRows, kStages = S::kStages, kHalves = HALVES, kThreads = S::kThreads;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Ahead ahead;
+  __shared__ Piece piece;
   uint8_t* area = smem + kStages * S::kTileBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   int* scan = reinterpret_cast<int*>(smem + S::kMore);
@@ -402,9 +403,16 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
   int stage = 0;
   uint32_t phase = 0;
   bool dead = false, behind = false;   // a wait ran out: nothing is waited for or copied any more, and what is computed does not count; a tile is done with
-  Piece p;
   const int r = lane >> 2, c = lane & 3, tile0 = warp / kWarps * NT, own = warp % kWarps;
-  while (walk.next(a, kRows, p)) {
+  while (true) {
+    if (warp == 0) {
+      Piece next;
+      if (!walk.next(a, kRows, next)) next.tiles = 0;
+      if (lane == 0) piece = next;
+    }
+    __syncthreads();
+    const Piece& p = piece;   // read where it is needed: registers are what is short
+    if (p.tiles == 0) break;
     const T* q = static_cast<const T*>(a.q) + p.b * a.q_stride[0] + 8 * c;
     for (int nt = warp; nt < S::kTiles; nt += kWarps * kHalves) {
       const int row = p.row0 + 8 * nt + r;
@@ -517,7 +525,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
 }
 
 template <typename T, int D, int G, int NT, int HALVES>
-int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
+int launch_tiles(const AttnArgs& a, cudaStream_t st) {
   using S = Shape<T, D, G, NT, HALVES>;
   auto kernel = kv4_attn_rows_kernel<T, D, G, NT, HALVES>;
   static thread_local uint64_t ready = 0;   // devices that know the kernel's shared memory, per thread
@@ -530,7 +538,7 @@ int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
     }
     if (dev < 64) ready |= (uint64_t)1 << dev;
   }
-  kernel<<<sms * blocks_of(S::kRows), S::kThreads, S::kBytes, st>>>(a);
+  kernel<<<a.blocks, S::kThreads, S::kBytes, st>>>(a);
   PSA_CHECK_LAUNCH("psa_kv4_attention");
   return PSA_OK;
 }
@@ -538,10 +546,10 @@ int launch_tiles(const AttnArgs& a, int sms, cudaStream_t st) {
 }  // namespace
 
 template <typename T, int D, int G>
-int launch_rows(const AttnArgs& a, int sms, int rows_per_tile, cudaStream_t st) {
-  return rows_per_tile == 24 ? launch_tiles<T, D, G, 3, 1>(a, sms, st) : rows_per_tile == 32 ? launch_tiles<T, D, G, 4, 1>(a, sms, st) : launch_tiles<T, D, G, 3, 2>(a, sms, st);
+int launch_rows(const AttnArgs& a, int rows_per_tile, cudaStream_t st) {
+  return rows_per_tile == 24 ? launch_tiles<T, D, G, 3, 1>(a, st) : rows_per_tile == 32 ? launch_tiles<T, D, G, 4, 1>(a, st) : launch_tiles<T, D, G, 3, 2>(a, st);
 }
-#define PSA_ROWS(T, D, G) template int launch_rows<T, D, G>(const AttnArgs&, int, int, cudaStream_t)
+#define PSA_ROWS(T, D, G) template int launch_rows<T, D, G>(const AttnArgs&, int, cudaStream_t)
 #define PSA_ROWS_OF(T) PSA_ROWS(T, 64, 32); PSA_ROWS(T, 64, 64); PSA_ROWS(T, 128, 32); PSA_ROWS(T, 128, 64); PSA_ROWS(T, 128, 128)
 PSA_ROWS_OF(__half);
 PSA_ROWS_OF(__nv_bfloat16);
