@@ -71,6 +71,14 @@ at::Tensor made(at::IntArrayRef sizes, at::ScalarType type, const at::Device& on
   return at::Tensor(at::detail::empty_cuda(sizes, type, on, std::nullopt));
 }
 
+// n numbers of a vector, from number `at` on, as a tensor of their own: two that live and die together in one piece of memory.
+at::Tensor part(const at::Tensor& x, int64_t at, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(x.storage()), x.key_set(), x.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 bool integer(PyObject* o, int64_t& n) {
   if (!PyLong_CheckExact(o)) return false;
   int overflow = 0;
@@ -264,8 +272,11 @@ PyObject* plan_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
   }
   c10::cuda::CUDAGuard guard(table->device());
-  if (args[7] == Py_None)
-    for (int i = 0; i < 3; ++i) out[i] = made((i == 0 ? table : i == 1 ? lengths : free)->sizes(), at::kInt, table->device());
+  if (args[7] == Py_None) {
+    out[0] = made(table->sizes(), at::kInt, table->device());
+    const at::Tensor counts_of = made({requests + 1}, at::kInt, table->device());
+    out[1] = part(counts_of, 0, requests), out[2] = part(counts_of, requests, 1);
+  }
   const at::Tensor slots = made({requests, tokens}, at::kInt, table->device());
   const size_t bytes = args[7] == Py_None && requests <= 1024 ? 0 : psa_plan_pages_scratch_bytes(requests);
   const at::Tensor scratch = bytes ? made({(int64_t)bytes}, at::kByte, table->device()) : at::Tensor();
