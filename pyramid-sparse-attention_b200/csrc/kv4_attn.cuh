@@ -304,16 +304,25 @@ struct Lookup {
   // Tile `tile` of the piece, of which `slices` slices are there, to `to`; valid: a bit for every slice that is.
   template <int SLICE, typename V>
   __device__ __forceinline__ void copy(const AttnArgs& a, int tile, bool whole, int slices, uint8_t* to, uint64_t* full, volatile V* valid) const {
-    const int lane = threadIdx.x & 31, k = whole ? tile & 31 : (tile & 7) * kWarps;
-    const uint32_t in = (1u << min(kWarps, slices)) - 1, good = __ballot_sync(~0u, from >= 0);
-    const uint32_t bits = whole ? (good >> k & 1 ? in : 0u) : good >> k & in;
+    const int lane = threadIdx.x & 31, n = min(kWarps, slices);
+    if (whole) {   // the lane that looked the page up does it all
+      if (lane == (tile & 31)) {
+        const int bytes = from >= 0 ? n * SLICE : 0;
+        *valid = (V)(from >= 0 ? (1u << n) - 1 : 0u);
+        tc::mbar_arrive_expect_tx(full, bytes);
+        if (bytes) tc::bulk_load_a(tc::smem_u32(to), a.data + (int64_t)from * SLICE, bytes, tc::smem_u32(full));
+      }
+      return;
+    }
+    const int k = (tile & 7) * kWarps;
+    const uint32_t bits = __ballot_sync(~0u, from >= 0) >> k & ((1u << n) - 1);
     if (lane == k) {
       *valid = (V)bits;
       tc::mbar_arrive_expect_tx(full, __popc(bits) * SLICE);
     }
     __syncwarp();
-    if (whole ? lane == k && bits : lane >= k && lane < k + kWarps && from >= 0)
-      tc::bulk_load_a(tc::smem_u32(to + (lane - k) * SLICE), a.data + (int64_t)from * SLICE, whole ? __popc(bits) * SLICE : SLICE, tc::smem_u32(full));
+    if (lane >= k && lane < k + n && from >= 0)
+      tc::bulk_load_a(tc::smem_u32(to + (lane - k) * SLICE), a.data + (int64_t)from * SLICE, SLICE, tc::smem_u32(full));
   }
 };
 
