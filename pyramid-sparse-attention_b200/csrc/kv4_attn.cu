@@ -58,7 +58,7 @@ template <typename T, int D, int G, int NT>
 struct Rows {
   static constexpr int NG = D / G, NB = D / 32;
   uint32_t q[NT][NB][2][2];
-  uint32_t q_sum[NT][2];    // (0, sum of q over group c) in two terms of the tensors' type
+  uint32_t q_sum[NT][2];    // sum of q over group c in two terms
   float factor[NT][2];      // of a column's scores, to log2
   float ref[NT][2], sum[NT][2];
   float out[NT][2 * NB][4]; // of channels 4 i, 4 i + 2: times 2^-24, of the others: times 2^-20
@@ -75,18 +75,10 @@ __device__ __forceinline__ void score(float (&x)[NT][4], const Rows<T, D, G, NT>
   constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   {
-    // sum_g lo_g (sum of q over g) is a product too: the parameter words themselves are its operand, a group's step against 0
     const uint8_t* p = slice + L::kParams + (c < NG ? c : 0) * 4;
     const uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
-    const uint32_t a[4] = {w0, w1, w0, w1};
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      mma_new<T>(x[nt], a, s.q_sum[nt]);
-      if constexpr (kSumScale<T> != 1.f) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[nt][j] *= kSumScale<T>;
-      }
-    }
+    for (int nt = 0; nt < NT; ++nt) lowest_part<T>(x[nt], w0, w1, s.q_sum[nt]);
   }
   const Words<NB> k0 = lds<NB>(slice + r * L::kRow + c * NB * 4), k1 = lds<NB>(slice + (r + 8) * L::kRow + c * NB * 4);
   const Words<NG> p0 = lds<NG>(slice + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kParams + (r + 8) * NG * 4);
@@ -101,7 +93,7 @@ __device__ __forceinline__ void score(float (&x)[NT][4], const Rows<T, D, G, NT>
         const uint32_t a[4] = {codes(w0, 2 * k), codes(w1, 2 * k), codes(w0, 2 * k + 1), codes(w1, 2 * k + 1)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if (i == 0 && k == 0) mma_new<__half>(acc[nt], a, s.q[nt][g * BG][0]);
+          if (i == 0 && k == 0) mma_new(acc[nt], a, s.q[nt][g * BG][0]);
           else MmaOp<__half>::run(acc[nt], a, s.q[nt][g * BG + i][k]);
         }
       }

@@ -51,9 +51,12 @@ constexpr float kLeastCapLog2 = -80.f, kLeastCap = 8.271806125530277e-25f;
 __device__ __forceinline__ float power_above(float least, float x) {
   return x > least ? __uint_as_float((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u) : least;
 }
-// Sums of q are kept in units of scores, 2^-24 of q's operands - in f16, whose numbers end there, 2^12 times that.
-// A weight times a step in one term of 11 bits is as exact as a bf16 output needs (2^-12 of what the codes add, against its 2^-9); an f16
-// output shows it (0.00041 of the output's norm instead of 0.00021), so there it is two terms: 25 products a slice instead of 17.
+// Sums of q meet the lowest values in two terms of 11 bits each (22 in all: off by 2^-22 of themselves): tf32 for bf16 tensors - two terms of bf16 would
+// be 16 bits, which keys far from zero show - and f16 for f16 ones.  They are kept in units of scores, 2^-24 of q's operands - in f16,
+// whose numbers end there, 2^12 times that.
+// A weight times a step in one term of 11 bits costs a bf16 output a twentieth of its error: its own rounding is 2^-9, that of the weights 2^-12 of
+// what the codes add (0.00175 of the output's norm instead of 0.00166-0.00168; with two terms 8 x 131071 tokens take 157 us instead of 133, 6 drafted
+// tokens 71 instead of 58).  An f16 output would show it (0.00041 instead of 0.00021), so there it is two terms: 25 products a slice for 17.
 template <typename T> constexpr int kWeightTerms = std::is_same<T, __half>::value ? 2 : 1;
 template <typename T> constexpr float kSumScale = std::is_same<T, __half>::value ? 2.44140625e-4f : 1.f;
 
@@ -219,14 +222,29 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The same product on an accumulator of zeros.
-template <typename T> __device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+// MmaOp<__half>'s product on an accumulator of zeros.
+__device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+  uint32_t y;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+  return y;
+}
+// sum_g lo_g (sum of q over g) is a product too.  w0, w1: the parameters of group c (lane 4 r + c) of the tokens in rows r and r + 8; q: from
+// row_operands.  f16: the words themselves are the operand, a group's step against 0; bf16: the lowest value is a word's upper half, a
+// number of tf32 as it stands.
+template <typename T> __device__ __forceinline__ void lowest_part(float (&x)[4], uint32_t w0, uint32_t w1, const uint32_t (&q)[2]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t a[4] = {w0, w1, w0, w1};
+    mma_new(x, a, q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] *= kSumScale<T>;
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%4,%5}, {%6,%7}, {%8,%8,%8,%8};"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(w0 & 0xffff0000u), "r"(w1 & 0xffff0000u), "r"(q[0]), "r"(q[1]), "f"(0.f));
+  }
 }
 // step and lowest value of a group
 template <typename T> __device__ __forceinline__ float2 param(uint32_t w);
@@ -246,7 +264,7 @@ template <int N> __device__ __forceinline__ Words<N> lds(const uint8_t* p) {
 
 // A lane's operands of a row of q (lane 4 r + c: row r of eight), from its row's start plus 8 c channels, or of no row: q as f16, times the
 // power of two that brings the row's largest value to 2^14 - exact for all that matters to a score; channels 4 i + 1 and 4 i + 3 meet
-// codes of 16 times the unit.  sum: the operand (0, sum of q over group c) in two terms of the tensors' type.  Returns the power of two.
+// codes of 16 times the unit.  sum: lowest_part's operand, the sum of q over group c in two terms.  Returns the power of two.
 template <typename T, int D, int G>
 __device__ __forceinline__ float row_operands(const T* from, bool in, uint32_t (&w)[D / 32][2][2], uint32_t (&sum)[2]) {
   constexpr int NG = D / G, NB = D / 32;
@@ -282,9 +300,14 @@ __device__ __forceinline__ float row_operands(const T* from, bool in, uint32_t (
     sums[g] += __shfl_xor_sync(~0u, sums[g], 2);
     x = c == g ? sums[g] * (grow * 5.9604644775390625e-8f / kSumScale<T>) : x;
   }
-  const float high = Elem<T>::to_f(Elem<T>::from_f(x));
-  sum[0] = MmaOp<T>::pack(0.f, high);
-  sum[1] = MmaOp<T>::pack(0.f, x - high);
+  if constexpr (std::is_same<T, __half>::value) {
+    const float high = Elem<T>::to_f(Elem<T>::from_f(x));
+    sum[0] = MmaOp<T>::pack(0.f, high);
+    sum[1] = MmaOp<T>::pack(0.f, x - high);
+  } else {
+    sum[0] = to_tf32(x);
+    sum[1] = to_tf32(x - __uint_as_float(sum[0]));
+  }
   return grow;
 }
 

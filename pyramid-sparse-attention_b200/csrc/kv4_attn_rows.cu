@@ -76,19 +76,10 @@ __device__ __forceinline__ void score(float (&x)[NT][4], int tile0, const uint8_
   constexpr int NG = L::kGroups, NB = L::kBlocks, BG = G / 32;   // 32-channel blocks of a group
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   {
-    // sum_g lo_g (sum of q over g) is a product too: the parameter words themselves are its operand, a group's step against 0
     const uint8_t* p = slice + L::kParams + (c < NG ? c : 0) * 4;
     const uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
-    const uint32_t a[4] = {w0, w1, w0, w1};
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const Words<2> q = lds<2>(smem + S::kQSum + ((tile0 + nt) * 32 + lane) * 8);
-      mma_new<T>(x[nt], a, q.w);
-      if constexpr (kSumScale<T> != 1.f) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[nt][j] *= kSumScale<T>;
-      }
-    }
+    for (int nt = 0; nt < NT; ++nt) lowest_part<T>(x[nt], w0, w1, lds<2>(smem + S::kQSum + ((tile0 + nt) * 32 + lane) * 8).w);
   }
   const Words<NB> k0 = lds<NB>(slice + r * L::kRow + c * NB * 4), k1 = lds<NB>(slice + (r + 8) * L::kRow + c * NB * 4);
   const Words<NG> p0 = lds<NG>(slice + L::kParams + r * NG * 4), p1 = lds<NG>(slice + L::kParams + (r + 8) * NG * 4);
@@ -105,7 +96,7 @@ __device__ __forceinline__ void score(float (&x)[NT][4], int tile0, const uint8_
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const Words<2> q = lds<2>(smem + S::kQ + (((tile0 + nt) * NB + b) * 32 + lane) * 16 + k * 8);
-          if (i == 0 && k == 0) mma_new<__half>(acc[nt], a0, q.w);
+          if (i == 0 && k == 0) mma_new(acc[nt], a0, q.w);
           else MmaOp<__half>::run(acc[nt], k ? a1 : a0, q.w);
         }
     }

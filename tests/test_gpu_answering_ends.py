@@ -1,0 +1,49 @@
+"""GPU: the ends of the ranges that the operators around the causal attention of a prompt promise - sums of many bits, constant and
+far values, large pages, long rows - against plain implementations in 64 bits.  (test_gpu_answering.py has the ordinary sizes.)"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_answering import DEV, HALF, SIZES, TINY, TYPES, Filled, attention, check_attention, gen, names, ops, randn, stands_for  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+# new tokens and query heads of one key head: rows for each of the five widths that the two attention kernels work in
+ROWS = [(1, 1), (12, 1), (7, 3), (8, 4), (14, 3)]
+
+
+@pytest.mark.parametrize("H,n", ROWS)
+@pytest.mark.parametrize("dtype", TYPES, **names)
+@pytest.mark.parametrize("D,group", SIZES)
+def test_attention_sums_of_q_keep_their_bits(ops, dtype, D, group, H, n):
+    """Keys that are one number in all channels of a token: a score is that number times a sum of q, which two numbers of 8 bits do not
+    hold.  The logarithm of a single weight is the score."""
+    g = torch.Generator().manual_seed(D + group)
+    part = torch.zeros(D)
+    first = (D // group - 1) * group
+    while True:       # numbers of 8 bits and three sizes: a sum of up to 24 bits, exact in 32
+        size = torch.tensor([1.0, 2.0 ** -6, 2.0 ** -12])[torch.randint(0, 3, (group,), generator=g)]
+        part[first:first + group] = torch.randint(128, 256, (group,), generator=g).float() / 4 * size * torch.where(torch.rand(group, generator=g) < 0.5, -1, 1)
+        x = part.sum()
+        rest = x - x.bfloat16().float()
+        if abs(x) > 64 and abs(rest - rest.bfloat16().float()) > 2.0 ** -18.7 * abs(x):
+            break
+    want = float(part.double().sum())
+    assert float(x) == want
+    q = part.to(dtype)
+    assert torch.equal(q.float(), part)
+    q = (q.to(DEV) * torch.where(torch.arange(H, device=DEV) % 2 == 0, 1, -1).to(dtype)[:, None])[None, :, None].expand(1, H, n, D)
+    for key in (1.0, -3.0):
+        c = Filled(ops, gen(1), [n], 1, D, group, dtype, 16)
+        # only the first key is in a row's sight, but for rows of later tokens: those keys are far lower
+        c.k[:] = 0
+        c.k[0, 0, 0] = key
+        ops.kv4_append(c.data, c.k, c.v, c.slots, group)
+        _, lse = ops.kv4_attention(q, c.data, c.table, c.len, group, None, 1.0, return_lse=True)
+        score = want * key * torch.where(torch.arange(H, device=DEV) % 2 == 0, 1.0, -1.0).double()[None, :, None].expand(1, H, n)
+        later = torch.arange(n, device=DEV).double().log()              # keys of zero: a score of 0 each
+        exact = torch.logaddexp(score, later.expand_as(score))
+        # two terms of 11 bits: 2^-22; their products' sum 2^-23 (cut off); factor, product with it, reference, sum with the logarithm and
+        # change of its base 8 roundings of 2^-24; exponential and logarithm 2^-17 (as in `attention`)
+        assert bool(((lse.double() - exact).abs() <= (2.0 ** -22 + 2.0 ** -23 + 2.0 ** -21) * score.abs() + 2.0 ** -17).all())
+    ops.check_status()
