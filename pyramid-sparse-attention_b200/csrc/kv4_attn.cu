@@ -115,19 +115,19 @@ __device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const 
   float x[N][NT][4], e[N][NT][4];
 #pragma unroll
   for (int n = 0; n < N; ++n) score<T, D, G, NT>(x[n], s, slice[n]);
-  // ---- the largest step of the values: a lane looks at one group of its two rows
+  // ---- the largest step of the values (or what stands for one): a lane looks at one group of its two rows
   float widest = 0.f, most = -INFINITY;
   int token[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     token[n] = t0[n] + (r >> 1) + 4 * (r & 1);
     const uint8_t* p = slice[n] + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
-    float s0 = param<T>(lds<1>(p + r * NG * 4).w[0]).x, s1 = param<T>(lds<1>(p + (r + 8) * NG * 4).w[0]).x;
+    uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
     if (MASKED) {   // what lies behind the last key may be anything
-      s0 = token[n] < s.last ? s0 : 0.f;
-      s1 = token[n] + 8 < s.last ? s1 : 0.f;
+      w0 = token[n] < s.last ? w0 : 0u;
+      w1 = token[n] + 8 < s.last ? w1 : 0u;
     }
-    widest = fmaxf(widest, fmaxf(s0, s1));
+    widest = fmaxf(widest, wanted<T>(w0, w1));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -161,15 +161,15 @@ __device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const 
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
         m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
         // largest score so far, or what the reference stood for
-        const float ref = fmaxf(m, s.ref[nt][j] - old + kHead) + (up - kHead), fade = ex2(s.ref[nt][j] - ref);
+        const float ref = fmaxf(m, s.ref[nt][j] - old + kHead) + (up - kHead), fade = half_of(s.ref[nt][j] - ref);
         s.ref[nt][j] = ref;
-        s.sum[nt][j] *= fade;
+        s.sum[nt][j] = faded(s.sum[nt][j], fade);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) s.mid[nt][g][j] *= fade;
+        for (int g = 0; g < NG; ++g) s.mid[nt][g][j] = faded(s.mid[nt][g][j], fade);
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
-          s.out[nt][i][j] *= fade;
-          s.out[nt][i][2 + j] *= fade;
+          s.out[nt][i][j] = faded(s.out[nt][i][j], fade);
+          s.out[nt][i][2 + j] = faded(s.out[nt][i][2 + j], fade);
         }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -390,20 +390,22 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(~0u, sum, d);
             const int row = 8 * nt + 2 * c + j;
+            const float size = size_of(sum), shrink = ex2(-size), even = shrink * 16777216.f, odd = shrink * 1048576.f;
             if (r == 0) {
-              stats_s[(warp * kRows + row) * 2] = s.ref[nt][j];
-              stats_s[(warp * kRows + row) * 2 + 1] = sum;
+              stats_s[(warp * kRows + row) * 2] = s.ref[nt][j] + size;
+              stats_s[(warp * kRows + row) * 2 + 1] = sum * shrink;
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               float mid = s.mid[nt][g][j];
 #pragma unroll
               for (int d = 4; d < 32; d *= 2) mid += __shfl_xor_sync(~0u, mid, d);
+              mid *= shrink;
 #pragma unroll
               for (int i = g * (G / 32); i < (g + 1) * (G / 32); ++i)
                 *reinterpret_cast<float4*>(mine + row * S::kOutRow + 32 * i + 4 * r) =
-                    make_float4(fmaf(s.out[nt][2 * i][j], 16777216.f, mid), fmaf(s.out[nt][2 * i][2 + j], 1048576.f, mid),
-                                fmaf(s.out[nt][2 * i + 1][j], 16777216.f, mid), fmaf(s.out[nt][2 * i + 1][2 + j], 1048576.f, mid));
+                    make_float4(fmaf(s.out[nt][2 * i][j], even, mid), fmaf(s.out[nt][2 * i][2 + j], odd, mid),
+                                fmaf(s.out[nt][2 * i + 1][j], even, mid), fmaf(s.out[nt][2 * i + 1][2 + j], odd, mid));
             }
           }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");

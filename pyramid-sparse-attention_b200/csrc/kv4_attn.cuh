@@ -45,8 +45,9 @@ constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has se
 // 2^kHead, and move when a weight times a step could be 2^kLazy times that: f16 has its full precision from 2^-14 to 2^16, so a
 // weight 2^-21 of the largest is still rounded to 11 bits.
 constexpr float kHead = 7.f, kLazy = 8.f;
-// Steps from 2^-80 on keep that precision (weights of 2^17 keys times 2^95 still fit 32 bits), and up to 2^100 (below 2^-126 weights are 0).
-constexpr float kLeastCapLog2 = -80.f, kLeastCap = 8.271806125530277e-25f;
+// Steps from 2^-80 on keep that precision, and up to 2^100 (below 2^-126 weights are 0): weights are up to 2^95, and 2^31 of them fit 32 bits.
+// Groups of one value have no step: 2^-64 of their size counts as one, so that weights times lowest values are up to 2^79.
+constexpr float kLeastCapLog2 = -80.f, kLeastCap = 8.271806125530277e-25f, kLowestShare = 5.421010862427522e-20f;
 // The smallest power of two that is not below x, or `least` if that is larger.
 __device__ __forceinline__ float power_above(float least, float x) {
   return x > least ? __uint_as_float((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u) : least;
@@ -227,6 +228,13 @@ __device__ __forceinline__ void mma_new(float (&c)[4], const uint32_t (&a)[4], c
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
+// What lies between two references of a row may be below the least number of 32 bits while what a weight becomes of it is not (rows of
+// zeros, then of 10^15: weights of 2^87 become such of 2^-46), so it is applied in two halves.  The half of 2^x; y times 2^x.
+__device__ __forceinline__ float half_of(float x) { return ex2(0.5f * x); }
+__device__ __forceinline__ float faded(float y, float half) { return y * half * half; }
+// Before parts of a row meet, each takes the size of its sum (a power of two) into its reference: what lies between those is what the parts
+// count for, and below the least number of 32 bits is nothing.  2^-100 at least: 2^24 times what shrinks the sum is a number.
+__device__ __forceinline__ float size_of(float sum) { return sum > 0.f ? (float)max((int)(__float_as_uint(sum) >> 23) - 127, -100) : 0.f; }
 __device__ __forceinline__ uint32_t to_tf32(float x) {
   uint32_t y;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
@@ -252,6 +260,18 @@ template <> __device__ __forceinline__ float2 param<__nv_bfloat16>(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 template <> __device__ __forceinline__ float2 param<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// What a group's values want of the references: two parameter words -> the larger step, or 2^-64 of the larger lowest value's size.
+template <typename T> __device__ __forceinline__ float wanted(uint32_t w0, uint32_t w1);
+template <> __device__ __forceinline__ float wanted<__nv_bfloat16>(uint32_t w0, uint32_t w1) {
+  const __nv_bfloat162 x = __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&w0)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w1)));
+  const float2 p = param<__nv_bfloat16>(*reinterpret_cast<const uint32_t*>(&x));
+  return fmaxf(p.x, p.y * kLowestShare);
+}
+template <> __device__ __forceinline__ float wanted<__half>(uint32_t w0, uint32_t w1) {
+  const float2 p = __half22float2(__hmax2(__habs2(*reinterpret_cast<const __half2*>(&w0)), __habs2(*reinterpret_cast<const __half2*>(&w1))));
+  return fmaxf(p.x, p.y * kLowestShare);
+}
 
 template <int N> struct Words { uint32_t w[N]; };
 template <int N> __device__ __forceinline__ Words<N> lds(const uint8_t* p) {

@@ -188,16 +188,16 @@ __device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const float4* columns = reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c;   // of rows 2 c and 2 c + 1
   score<T, D, G, NT, HALVES>(e, tile0, smem, slice);
-  // the largest step of the values: a lane looks at one group of its two rows
+  // the largest step of the values (or what stands for one): a lane looks at one group of its two rows
   float widest, most = -INFINITY;
   {
     const uint8_t* p = slice + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
-    float s0 = param<T>(lds<1>(p + r * NG * 4).w[0]).x, s1 = param<T>(lds<1>(p + (r + 8) * NG * 4).w[0]).x;
+    uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
     if (MASKED) {   // what lies behind the last key may be anything
-      s0 = token < length ? s0 : 0.f;
-      s1 = token + 8 < length ? s1 : 0.f;
+      w0 = token < length ? w0 : 0u;
+      w1 = token + 8 < length ? w1 : 0u;
     }
-    widest = fmaxf(s0, s1);
+    widest = wanted<T>(w0, w1);
   }
   float t[NT][4];   // to the references
 #pragma unroll
@@ -267,18 +267,22 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, rise[w * S::kRows + 8 * nt + 2 * c + j]);
       // largest score so far, or what the reference stood for
       float& was = j ? s.ref[nt].y : s.ref[nt].x;
-      const float ref = fmaxf(m, kHead - was - old) + (up - kHead), fade = ex2(-was - ref);
+      const float ref = fmaxf(m, kHead - was - old) + (up - kHead), fade = half_of(-was - ref);
       was = -ref;
-      (j ? s.sum[nt].y : s.sum[nt].x) *= fade;
+      float& sum = j ? s.sum[nt].y : s.sum[nt].x;
+      sum = faded(sum, fade);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) (j ? s.mid[nt][g].y : s.mid[nt][g].x) *= fade;
+      for (int g = 0; g < NG; ++g) {
+        float& mid = j ? s.mid[nt][g].y : s.mid[nt][g].x;
+        mid = faded(mid, fade);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s.out[nt][h][j] *= fade;
-        s.out[nt][h][2 + j] *= fade;
+        s.out[nt][h][j] = faded(s.out[nt][h][j], fade);
+        s.out[nt][h][2 + j] = faded(s.out[nt][h][2 + j], fade);
       }
-      e[nt][j] = rises ? ex2(e[nt][j] - ref) : e[nt][j] * fade;
-      e[nt][2 + j] = rises ? ex2(e[nt][2 + j] - ref) : e[nt][2 + j] * fade;
+      e[nt][j] = rises ? ex2(e[nt][j] - ref) : faded(e[nt][j], fade);
+      e[nt][2 + j] = rises ? ex2(e[nt][2 + j] - ref) : faded(e[nt][2 + j], fade);
     }
   weigh<T, D, G, NT, HALVES, true>(s, e, rises, reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c, slice, token, to);
   __syncthreads();
@@ -497,8 +501,9 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
       if (whole) {
         write_row<T>(a, p.b, p.head * group + (p.row0 + row) % group, (p.row0 + row) / group, d, o, refs[row], sum);
       } else {
-        *reinterpret_cast<float4*>(part + row * D + d) = o;
-        if (d == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * row) = make_float2(refs[row], sum);
+        const float size = size_of(sum), shrink = ex2(-size);
+        *reinterpret_cast<float4*>(part + row * D + d) = make_float4(o.x * shrink, o.y * shrink, o.z * shrink, o.w * shrink);
+        if (d == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * row) = make_float2(refs[row] + size, sum * shrink);
       }
     }
     if (starts && threadIdx.x == 0)   // whose parts the unit is made of: from this block to the one that holds its last tile

@@ -47,3 +47,47 @@ def test_attention_sums_of_q_keep_their_bits(ops, dtype, D, group, H, n):
         # change of its base 8 roundings of 2^-24; exponential and logarithm 2^-17 (as in `attention`)
         assert bool(((lse.double() - exact).abs() <= (2.0 ** -22 + 2.0 ** -23 + 2.0 ** -21) * score.abs() + 2.0 ** -17).all())
     ops.check_status()
+
+
+def put_values(ops, c, v):
+    """v [B, Hk, L, D] in the place of a filled cache's values."""
+    c.v = v.to(c.dtype)
+    ops.kv4_append(c.data, c.k, c.v, c.slots, c.group)
+
+
+@pytest.mark.parametrize("H,n", ROWS)
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, 1e13), (torch.bfloat16, -1e30), (torch.bfloat16, 1e-20), (torch.float16, 65504.0), (torch.float16, 6e-8)], **names)
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32)])
+def test_attention_of_constant_values(ops, dtype, value, D, group, H, n):
+    """Groups of one value have no step: the references take the value itself along."""
+    g = gen(70)
+    c = Filled(ops, g, [n, 500, 3000], 1, D, group, dtype, 64)
+    put_values(ops, c, torch.full_like(c.v, value, dtype=torch.float32))
+    got = check_attention(ops, randn(g, 3, H, n, D, dtype=dtype), c)
+    assert bool((got == torch.tensor(value, dtype=dtype)).all())
+
+
+@pytest.mark.parametrize("H,n", [(7, 1), (10, 3)])
+@pytest.mark.parametrize("order", ["zeros first", "zeros last", "in turn"])
+@pytest.mark.parametrize("value", [1e15, 1e30])
+def test_attention_of_values_of_different_sizes(ops, value, order, H, n):
+    """Rows of zeros before, behind and between large ones count as keys, within a warp, between warps and between blocks."""
+    g = gen(71)
+    lengths = [700, 40000, 90]
+    c = Filled(ops, g, lengths, 1, 128, 64, torch.bfloat16, 64, k_scale=0.3)
+    at = torch.arange(c.v.shape[2], device=DEV)[None, :]
+    half = torch.tensor(lengths, device=DEV)[:, None] // 2
+    zero = {"zeros first": at < half, "zeros last": at >= half, "in turn": at // 5 % 2 == 0}[order][:, None, :, None]
+    for v in (torch.full_like(c.v, value, dtype=torch.float32), c.v.float() * value, torch.where(at[..., None, None].transpose(1, 2) % 2 == 0, value, 1e-20).expand_as(c.v)):
+        put_values(ops, c, torch.where(zero, 0.0, v))
+        check_attention(ops, randn(g, 3, H, n, 128, dtype=torch.bfloat16), c)
+
+
+@pytest.mark.parametrize("H", [4, 12])
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, 1e30), (torch.float16, 60000.0)], **names)
+def test_attention_of_constant_values_over_a_long_context(ops, dtype, value, H):
+    g = gen(72)
+    c = Filled(ops, g, [131071], 1, 64, 32, dtype, 64)
+    put_values(ops, c, torch.full_like(c.v, value, dtype=torch.float32))
+    got = check_attention(ops, randn(g, 1, H, 2, 64, dtype=dtype), c)
+    assert bool((got == torch.tensor(value, dtype=dtype)).all())
