@@ -91,3 +91,32 @@ def test_attention_of_constant_values_over_a_long_context(ops, dtype, value, H):
     put_values(ops, c, torch.full_like(c.v, value, dtype=torch.float32))
     got = check_attention(ops, randn(g, 1, H, 2, 64, dtype=dtype), c)
     assert bool((got == torch.tensor(value, dtype=dtype)).all())
+
+
+def test_cache_offsets_beyond_32_bits_within_a_page(ops):
+    """One page of 2^24 tokens, 2.7 GB: rows at its start, on both sides of byte 2^31 and at its end, written, read and attended to."""
+    D, group, page, g = 128, 32, 1 << 24, gen(73)
+    data = torch.zeros_like(ops.kv4_empty(1, 1, page, D, group, DEV))
+    slice_bytes = data.shape[3]
+    border = (1 << 31) // slice_bytes * 16
+    at = torch.cat([torch.arange(s, s + 16) for s in (0, border - 16, border, border + 16, page - 16)])[None]
+    slots = at.to(torch.int32).to(DEV)
+    q = randn(g, 1, 4, 1, D, dtype=torch.bfloat16)
+    # keys in line with the queries' sum: what the other 2^24 tokens - zeros - count for stays small
+    k = (2 * q.sum(1, keepdim=True).expand(1, 1, at.shape[1], D) + 0.1 * randn(g, 1, 1, at.shape[1], D)).to(torch.bfloat16)
+    v = randn(g, 1, 1, at.shape[1], D, dtype=torch.bfloat16)
+    ops.kv4_append(data, k, v, slots, group)
+    for x, y in zip((k, v), ops.kv4_read(data, slots, D, group, torch.bfloat16)):
+        want = stands_for(x, group)
+        assert bool(((y.double() - want).abs() <= HALF[x.dtype] * 1.001 * want.abs() + TINY[x.dtype]).all())
+    written = data.flatten(0, 2).any(-1).nonzero().flatten()                       # slices of 16 tokens
+    assert written.tolist() == sorted({int(t) // 16 for t in at[0]})
+    got = ops.kv4_attention(q, data, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([page], dtype=torch.int32, device=DEV), group)
+    kk, vv = (stands_for(x, group)[0, 0] for x in (k, v))
+    s = q[0, :, 0].double() @ kk.T * D ** -0.5
+    top = s.amax(-1, keepdim=True).clamp(min=0)
+    p = torch.exp(s - top)
+    want = p @ vv / (p.sum(-1, keepdim=True) + (page - at.shape[1]) * torch.exp(-top))
+    # bf16's half step, a weight's 2^-11 on codes of 15 steps at most, scores and the sum of 2^24 numbers to 2^-10
+    assert bool(((got[0, :, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * vv.abs().amax()).all())
+    ops.check_status()
