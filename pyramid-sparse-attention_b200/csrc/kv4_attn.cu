@@ -276,8 +276,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
   if ((int)blockIdx.x >= shares.blocks) return;
   const int group = a.group;
   const bool whole_tiles = a.page % kTile == 0;
-  int pair = 0;
-  uint32_t phase = 0;
+  Ring<S::kPairs> ring = {0, 0};   // the copying warp's barriers; a computing warp's, which it waits for
   bool dead = false;   // a wait ran out: nothing is copied or handed back any more, and what is computed does not count
   Walk walk = {request, base, shares.first(blockIdx.x), shares.first(blockIdx.x + 1)};
   while (true) {
@@ -288,19 +287,19 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         const int last_slice = min((p.length + 15) / 16, (p.tile0 + p.tiles) * kWarps);
         Lookup found;
         for (int i = 0; i < p.tiles; i += 2) {
-          if (!dead && !__all_sync(~0u, tc::mbar_wait(empty + pair, phase ^ 1, abort_flag))) dead = true;
+          if (!dead && !__all_sync(~0u, tc::mbar_wait(empty + ring.at, ring.phase ^ 1, abort_flag))) dead = true;
+          if (dead) break;
           for (int k = 0; k < 2; ++k) {
-            const int t = i + k, at = 2 * pair + k;
+            const int t = i + k, at = 2 * ring.at + k;
             if (t < p.tiles && (t & (whole_tiles ? 31 : 7)) == 0) found.look(a, p, t, whole_tiles, last_slice);
-            if (dead) continue;
             if (t < p.tiles) {
-              found.copy<L::kSlice>(a, t, whole_tiles, last_slice - (p.tile0 + t) * kWarps, smem + at * kWarps * L::kSlice, full + pair, valid + at);
+              found.copy<L::kSlice>(a, t, whole_tiles, last_slice - (p.tile0 + t) * kWarps, smem + at * kWarps * L::kSlice, full + ring.at, valid + at);
             } else if (lane == 0) {
               valid[at] = 0;
-              tc::mbar_arrive(full + pair);
+              tc::mbar_arrive(full + ring.at);
             }
           }
-          if (++pair == S::kPairs) pair = 0, phase ^= 1;
+          ring.advance();
         }
       } else {
         // ------------------------------------------------------------ products
@@ -340,19 +339,19 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         // tiles whose tokens every row sees, then the others
         const int first = p.tile0 * kTile + 16 * warp, plain = all_see - 16 >= first ? min((all_see - 16 - first) / kTile + 1, p.tiles) : 0;
         auto wait = [&]() {
-          if (!tc::mbar_try_wait(full + pair, phase) && !tc::mbar_wait(full + pair, phase, abort_flag)) dead = true;
+          if (!tc::mbar_try_wait(full + ring.at, ring.phase) && !tc::mbar_wait(full + ring.at, ring.phase, abort_flag)) dead = true;
           __syncwarp();
         };
         auto leave = [&]() {
           __syncwarp();
-          if (lane == 0 && !dead) tc::mbar_arrive(empty + pair);
-          if (++pair == S::kPairs) pair = 0, phase ^= 1;
+          if (lane == 0 && !dead) tc::mbar_arrive(empty + ring.at);
+          ring.advance();
         };
         int i = 0;
         for (; i + 1 < plain; i += 2) {
           wait();
-          const uint8_t* slice = smem + (2 * pair * kWarps + warp) * L::kSlice;
-          const uint32_t there = *reinterpret_cast<volatile const uint32_t*>(valid + 2 * pair) & 0x10001u << warp;   // the slices, a bit each
+          const uint8_t* slice = smem + (2 * ring.at * kWarps + warp) * L::kSlice;
+          const uint32_t there = *reinterpret_cast<volatile const uint32_t*>(valid + 2 * ring.at) & 0x10001u << warp;   // the slices, a bit each
           if (kJoint && there == 0x10001u << warp) {
             const uint8_t* const two[2] = {slice, slice + kWarps * L::kSlice};
             const int at[2] = {};
@@ -372,9 +371,8 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
           wait();
 #pragma unroll 1
           for (int k = 0; k < 2; ++k)
-            if (valid[2 * pair + k] & 1u << warp)
-{
-              const uint8_t* const one[1] = {smem + ((2 * pair + k) * kWarps + warp) * L::kSlice};
+            if (valid[2 * ring.at + k] & 1u << warp) {
+              const uint8_t* const one[1] = {smem + ((2 * ring.at + k) * kWarps + warp) * L::kSlice};
               const int at[1] = {first + (i + k) * kTile};
               take<T, D, G, NT, 1, true>(s, one, at);
             }
@@ -442,14 +440,10 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
       }
   }
-  if (*abort_flag) {
-    if (threadIdx.x == 0) *a.status = PSA_ERR_TIMEOUT;
-    // copies still in flight must have landed before the block's memory is another's
-    if (warp == kWarps && lane == 0)
-      for (int i = 0; i < S::kPairs; ++i) {
-        int unused = 0;
-        tc::mbar_wait(full + i, i < pair ? phase : phase ^ 1, &unused);
-      }
+  if (lane == 0 && *abort_flag) *a.status = PSA_ERR_TIMEOUT;
+  if (warp == kWarps && lane == 0) {   // what was copied must have landed before the block's memory is another's
+    int unused = 0;
+    for (int i = 0; i < S::kPairs; ++i) tc::mbar_wait(full + i, ring.last(i), &unused);
   }
 }
 

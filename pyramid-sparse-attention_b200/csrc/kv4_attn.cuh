@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "kv4.cuh"
+#include "kv4_ring.h"
 #include "mma_sync.cuh"
 #include "tc_common.cuh"
 
@@ -159,7 +160,8 @@ __device__ __forceinline__ int line_of(const AttnArgs& a, int rows_per_tile, int
 }
 
 // Lengths that another stream changes meanwhile give wrong outputs, but no wait without end and no access out of range: one warp reads
-// them for those that meet at barriers, requests and blocks are bounded by what there is, and waits for tiles run out.
+// them for those that meet at barriers, requests and blocks are bounded by what there is, waits for tiles run out, and a block ends when
+// all that it copied has landed - also tiles that those who compute, with lengths of another moment, did not wait for.
 //
 // What a block has of a unit: tiles tile0 .. tile0 + tiles - 1 of key head `head` for the rows from row0 on.
 struct Piece {

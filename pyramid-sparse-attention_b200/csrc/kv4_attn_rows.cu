@@ -331,6 +331,7 @@ struct Ahead {
   Walk walk;
   Piece piece;
   int next, last_slice;
+  int before;   // tiles copied of the pieces before this one
 };
 
 template <typename T, int D, int G, int NT, int HALVES>
@@ -373,6 +374,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
       __syncwarp();
       if (lane == 0) {
         ahead.walk = w;
+        ahead.before += ahead.next;
         ahead.piece = p;
         ahead.next = 0;
         ahead.last_slice = min((p.length + 15) / 16, (p.tile0 + p.tiles) * kWarps);
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
   if (warp == 0) {
     if (lane == 0) {
       ahead.walk = walk;
-      ahead.piece.tiles = ahead.next = 0;
+      ahead.piece.tiles = ahead.next = ahead.before = 0;
     }
     __syncwarp();
     for (int i = 0; i < kStages; ++i) copy_next(i);
@@ -510,13 +512,11 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
       a.owners[((int64_t)p.b * a.kv_heads + p.head) * a.row_tiles + p.row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(p.end - 1));
     __syncthreads();
   }
-  if (__syncthreads_or(dead) && threadIdx.x == 0) {
-    *a.status = PSA_ERR_TIMEOUT;
-    // copies still in flight must have landed before the block's memory is another's
-    for (int i = 0; i < kStages; ++i) {
-      int unused = 0;
-      tc::mbar_wait(full + i, i < stage ? phase ^ 1 : phase, &unused);
-    }
+  if (__syncthreads_or(dead) && threadIdx.x == 0) *a.status = PSA_ERR_TIMEOUT;
+  if (threadIdx.x == 0) {   // what was copied must have landed before the block's memory is another's
+    const auto ring = Ring<kStages>::after(ahead.before + ahead.next);
+    int unused = 0;
+    for (int i = 0; i < kStages; ++i) tc::mbar_wait(full + i, ring.last(i), &unused);
   }
 }
 

@@ -1,0 +1,61 @@
+"""CPU: bookkeeping and host-side ends of the operators around the causal attention of a prompt."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "pyramid-sparse-attention_b200", "csrc")
+
+RING = r"""
+#include <cstdio>
+#include "kv4_ring.h"
+// A barrier as the hardware has it: armed and landed phases; a wait for a parity passes when the phase it stands in has the other one.
+struct Barrier {
+  int armed = 0, landed = 0;
+  bool passes(unsigned parity) const { return (unsigned)(landed & 1) != parity; }
+};
+// `copied` tiles are copied, one barrier of N after the other, at most N ahead of what is waited for; `waited` are waited for (lengths of
+// another moment).  Every copy still in flight must hold the wait at the end up, and nothing else may.
+template <int N> int check(int copied, int waited) {
+  Barrier bars[N];
+  psa::Ring<N> ring = {0, 0};
+  int done = 0;
+  for (int i = 0; i < copied; ++i) {
+    if (i - N >= waited) break;                      // the copier gives up: no one hands its barrier back
+    Barrier& b = bars[ring.at];
+    for (; done <= i - N; ++done) bars[done % N].landed++;
+    if (ring.at != i % N || b.armed != b.landed) return 1;
+    b.armed++;
+    ring.advance();
+    const auto same = psa::Ring<N>::after(i + 1);
+    if (same.at != ring.at || same.phase != ring.phase) return 3;
+  }
+  for (int i = 0; i < N; ++i)
+    for (;;) {
+      const bool over = bars[i].armed == bars[i].landed;
+      if (bars[i].passes(ring.last(i)) != over) return 2;
+      if (over) break;
+      bars[i].landed++;
+    }
+  return 0;
+}
+int main() {
+  for (int copied = 0; copied < 40; ++copied)
+    for (int waited = 0; waited < 40; ++waited) {
+      int bad = check<2>(copied, waited) + check<3>(copied, waited) + check<4>(copied, waited) + check<5>(copied, waited) + check<6>(copied, waited);
+      if (bad) { std::printf("%d copied, %d waited for\n", copied, waited); return 1; }
+    }
+}
+"""
+
+
+def test_blocks_wait_for_all_that_they_copied(tmp_path):
+    """The copying side's ring says at the end which phase of each barrier was armed last, whatever the computing side waited for."""
+    src = tmp_path / "ring.cpp"
+    src.write_text(RING)
+    exe = str(tmp_path / "ring")
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", f"-I{CSRC}", str(src), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
