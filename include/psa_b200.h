@@ -429,7 +429,8 @@ int psa_fwd_images_scatter(const void* q, const void* kimg, const void* vimg, co
  * reference hands single tokens back to the model's own attention (qwen2.5-vl-example/src/attention/qwen2vl_attention.py), so
  * these have no counterpart there.  Row strides are in elements; channels are neighbours; every pointer is 16-byte aligned.
  * `status` is the int32 word described above: PSA_ERR_ARG is written into it where a page number, slot, length or count found
- * on the device is out of range (the access is skipped) or a request could not be given pages. */
+ * on the device is out of range (the access is skipped) or a request could not be given pages; a
+ * PSA_ERR_TIMEOUT that is already there stays. */
 
 /* Rotary positions with several axes.  n operands (1 or 2: queries, keys) src[i] -> dst[i], [batch][heads[i]][seq][head_dim]
  * with strides {batch, head, token} each (multiples of 16 bytes).  Channel pair p - (p, p + head_dim/2) if half, else (2p, 2p + 1) - of

@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
       }
   }
-  if (lane == 0 && *abort_flag) *a.status = PSA_ERR_TIMEOUT;
+  if (lane == 0 && *abort_flag) report(a.status, PSA_ERR_TIMEOUT);
   if (warp == kWarps && lane == 0) {   // what was copied must have landed before the block's memory is another's
     int unused = 0;
     for (int i = 0; i < S::kPairs; ++i) tc::mbar_wait(full + i, ring.last(i), &unused);
@@ -459,6 +459,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const __grid_con
   const int group = a.group, i = blockIdx.x, head = blockIdx.y, b = blockIdx.z, own = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   int length, count;
   const Span span = span_of(a, b, rows_per_tile, length, count);
+  if (span.bad && threadIdx.x == 0) report(a.status, PSA_ERR_ARG);
   const int row = i * group + head % group, r = row % rows_per_tile;
   int2 owners = make_int2(0, -1);
   asm volatile("griddepcontrol.wait;" ::: "memory");

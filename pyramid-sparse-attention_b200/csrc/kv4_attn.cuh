@@ -66,17 +66,16 @@ template <typename T> constexpr float kSumScale = std::is_same<T, __half>::value
 // and after the tiles.
 struct Span {
   int rows, row_tiles, tiles, cells, work;
+  bool bad;   // a length or count out of range, and cut to it (the joining kernel reports it: here an atomic costs the start 0.2 us)
 };
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_tile, int& length, int& count) {
   length = a.lengths[b];
   count = a.counts ? a.counts[b] : a.tokens;
   const int most = a.width * a.page;
-  if (length < 0 || length > most || count < 0 || count > a.tokens) {
-    *a.status = PSA_ERR_ARG;
-    length = min(max(length, 0), most);
-    count = min(max(count, 0), a.tokens);
-  }
   Span s;
+  s.bad = length < 0 || length > most || count < 0 || count > a.tokens;
+  length = min(max(length, 0), most);
+  count = min(max(count, 0), a.tokens);
   s.rows = count * a.group;
   s.row_tiles = (s.rows + rows_per_tile - 1) / rows_per_tile;
   s.tiles = (length + kTile - 1) / kTile;
@@ -343,7 +342,7 @@ struct Lookup {
     if (s < last_slice) {
       const int in_page = s / per_page, page = a.table[(int64_t)p.b * a.width + in_page];
       if (page >= 0 && page < a.pages) from = (page * a.kv_heads + p.head) * per_page + s - in_page * per_page;
-      else *a.status = PSA_ERR_ARG;
+      else report(a.status, PSA_ERR_ARG);
     }
   }
   // Tile `tile` of the piece, of which `slices` slices are there, to `to`; valid: a bit for every slice that is.

@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
       a.owners[((int64_t)p.b * a.kv_heads + p.head) * a.row_tiles + p.row0 / kRows] = make_int2((int)blockIdx.x, shares.owner(p.end - 1));
     __syncthreads();
   }
-  if (__syncthreads_or(dead) && threadIdx.x == 0) *a.status = PSA_ERR_TIMEOUT;
+  if (__syncthreads_or(dead) && threadIdx.x == 0) report(a.status, PSA_ERR_TIMEOUT);
   if (threadIdx.x == 0) {   // what was copied must have landed before the block's memory is another's
     const auto ring = Ring<kStages>::after(ahead.before + ahead.next);
     int unused = 0;

@@ -67,7 +67,7 @@ struct Slot {
     in = row < (uint32_t)a.batch * (uint32_t)a.tokens;
     const int slot = a.slots[in ? row : 0];
     good = in && slot >= 0 && slot < a.slots_total;
-    if (in && !good && slot != -1) *a.status = PSA_ERR_ARG;
+    if (in && !good && slot != -1) report(a.status, PSA_ERR_ARG);
     const uint32_t of = good ? (uint32_t)slot : 0u, page = a.shift >= 0 ? of >> a.shift : of / (uint32_t)a.page, at = of - page * (uint32_t)a.page;
     slice = page * a.page_bytes + (int64_t)(at / 16) * slice_bytes;   // a page may be more than 2^31 bytes
     place = (int)(at & 15);

@@ -78,7 +78,7 @@ __device__ __forceinline__ Want want_of(const PlanArgs& a, int b) {
 }
 __device__ __forceinline__ Grant grant_of(const PlanArgs& a, const Want& w, int total, int available) {
   const bool served = w.need == 0 || total <= available;
-  if (!served || w.bad) *a.status = PSA_ERR_ARG;
+  if (!served || w.bad) report(a.status, PSA_ERR_ARG);
   return {w.held, served ? w.need : 0, total - w.need, served ? w.count : 0, w.length};
 }
 
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_kernel(const int32_t* ta
       for (int j = threadIdx.x & 31; j < held_of[i]; j += 32) {
         const int64_t at = (int64_t)top + end_of[i] - 1 - j;
         if (at < pool_size) pool[at] = row[j];
-        else *status = PSA_ERR_ARG;
+        else report(status, PSA_ERR_ARG);
       }
     }
     __syncthreads();

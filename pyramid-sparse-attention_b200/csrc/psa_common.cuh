@@ -57,6 +57,9 @@ template <> struct Elem<__nv_bfloat16> {
       return PSA_ERR_ARG;                                                   \
   }
 
+// A code into a status word that may hold one nobody has read yet: a wait that ran out (the largest) is not replaced by a number out of range.
+static __device__ __forceinline__ void report(int32_t* status, int code) { atomicMax(status, code); }
+
 static inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace psa

@@ -120,3 +120,30 @@ def test_cache_offsets_beyond_32_bits_within_a_page(ops):
     # bf16's half step, a weight's 2^-11 on codes of 15 steps at most, scores and the sum of 2^24 numbers to 2^-10
     assert bool(((got[0, :, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * vv.abs().amax()).all())
     ops.check_status()
+
+
+def test_an_expired_wait_is_not_replaced_by_a_number_out_of_range(ops):
+    """One status word a device: the code of a wait that ran out stays, whatever the calls behind it find."""
+    from psa_b200 import _lib
+    g = gen(74)
+    c = Filled(ops, g, [64, 64], 1, 64, 32, torch.bfloat16, 16)
+    word = ops.status_word(torch.device(DEV))
+    one = torch.ones(2, dtype=torch.int32, device=DEV)
+    bad = torch.full((2, 1), 2 ** 30, dtype=torch.int32, device=DEV)
+    row = randn(g, 2, 1, 1, 64, dtype=torch.bfloat16)
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def planned():
+        ops.plan_pages(torch.full_like(c.table, -1), one * 0, one, one, none, 16, 1)
+    calls = {"append": lambda: ops.kv4_append(c.data, row, row, bad, 32), "read": lambda: ops.kv4_read(c.data, bad, 64, 32, torch.bfloat16), "plan": planned,
+             "plan in place": lambda: ops.plan_pages(c.table.clone(), c.len.clone(), one * 99, one, none.clone(), 16, 1), "length": lambda: ops.kv4_attention(row, c.data, c.table, c.len + 999, 32),
+             "page": lambda: ops.kv4_attention(row, c.data, c.table + 10 ** 6, c.len, 32), "many rows": lambda: ops.kv4_attention(row.expand(2, 20, 1, 64), c.data, c.table + 10 ** 6, c.len, 32),
+             "release": lambda: ops.release_pages(c.table, c.len.clone(), one.bool(), one[:1].clone(), one[:1].clone(), 16)}
+    for name, call in calls.items():
+        for before, text in ((0, "out of range"), (_lib.PSA_ERR_TIMEOUT, "wait expired")):
+            word.fill_(before)
+            call()
+            with pytest.raises(RuntimeError, match=text):
+                ops.check_status()
+                pytest.fail(name)
+    ops.check_status()
