@@ -473,7 +473,8 @@ int psa_kv4_read(const void* data, void* k, void* v, const int64_t* strides, con
 /* Attention of the last counts[b] (null: tokens) tokens of every request over that cache: q, out [batch][heads][tokens][head_dim],
  * query i of request b stands at lengths[b] - counts[b] + i and sees the keys up to its own place; query head h reads key head
  * h / (heads / kv_heads).  Rows without a key, and rows from counts[b] on, give 0 (lse -inf).  lse: optional
- * [batch][heads][tokens], natural logarithm.  table [batch][width].  scratch needs no initialising. */
+ * [batch][heads][tokens], natural logarithm.  table [batch][width].  scratch needs no initialising (0 bytes: no rows, or numbers of
+ * requests, tokens or heads that psa_kv4_attention refuses). */
 size_t psa_kv4_attention_scratch_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim);
 int psa_kv4_attention(const void* q, const int64_t* q_strides, const void* data, const int32_t* table, const int32_t* lengths,
                       const int32_t* counts, void* out, const int64_t* out_strides, float* lse, void* scratch,

@@ -580,7 +580,7 @@ int launch(const AttnArgs& a, int rows, cudaStream_t st) {
 
 extern "C" size_t psa_kv4_attention_scratch_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim) {
   using namespace psa;
-  if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  if (batch <= 0 || batch >= 65536 || tokens <= 0 || tokens >= 65536 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
   const int64_t rows = tokens * (heads / kv_heads), r = rows_per_tile(rows);
   return owners_bytes(batch, kv_heads, cdiv64(rows, r)) + (size_t)kMostSms * blocks_of((int)r) * 2 * r * (head_dim + 2) * sizeof(float);
 }

@@ -1152,8 +1152,8 @@ def kv4_attention(q: torch.Tensor, data: torch.Tensor, table: torch.Tensor, leng
     with _on(q):
         out = _new_rows(q, like)
         lse = torch.empty((B, H, n), dtype=torch.float32, device=q.device) if return_lse else None
-        if nbytes:
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        if q.numel():
+            scratch = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
             rc = lib.psa_kv4_attention(_ptr(q), _row_strides(q), _ptr(data), _ptr(table), _ptr(lengths), _ptr(counts), _ptr(out), out_strides, _ptr(lse),
                                        _ptr(scratch), nbytes, data.shape[0], 16 * data.shape[2], table.shape[1], B, n, H, data.shape[1], D, group,
                                        D ** -0.5 if sm_scale is None else sm_scale, _DT[q.dtype], _ptr(status_word(q.device)), _stream(q))

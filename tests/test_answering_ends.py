@@ -59,3 +59,19 @@ def test_blocks_wait_for_all_that_they_copied(tmp_path):
     subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", f"-I{CSRC}", str(src), "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout
+
+
+@pytest.mark.parametrize("batch,tokens,heads,kv_heads", [(1, 1, 4, 8), (1, 1, 5, 2), (1, 2 ** 62, 4, 1), (65536, 1, 4, 4), (1, 65536, 4, 4), (1, 1, 4, 0), (0, 1, 4, 4)])
+def test_scratch_of_refused_sizes_is_none(batch, tokens, heads, kv_heads):
+    """A C caller asks for the scratch before it calls: numbers that the call refuses end neither the process (a division by zero) nor give bytes."""
+    from psa_b200._lib import LIB_PATH
+    code = (f"import ctypes as C; f = C.CDLL({LIB_PATH!r}).psa_kv4_attention_scratch_bytes; f.restype = C.c_size_t; "
+            f"print(f(C.c_int64({batch}), C.c_int64({tokens}), {heads}, {kv_heads}, 128))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.split()[-1] == "0", (r.returncode, r.stdout, r.stderr)
+
+
+def test_scratch_holds_the_parts():
+    from psa_b200._lib import lib
+    few, many = (lib.psa_kv4_attention_scratch_bytes(1, n, 4, 1, 128) for n in (1, 65535))
+    assert 0 < few < many
