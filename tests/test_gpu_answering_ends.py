@@ -151,6 +151,6 @@ def test_an_expired_wait_is_not_replaced_by_a_number_out_of_range(ops):
 
 def test_attention_of_more_tokens_than_it_takes_is_refused(ops):
     c = Filled(ops, gen(75), [20], 1, 64, 32, torch.bfloat16, 16)
-    with pytest.raises(RuntimeError, match="tokens"):
+    with pytest.raises(ValueError, match="tokens"):
         ops.kv4_attention(torch.zeros(1, 1, 65536, 64, dtype=torch.bfloat16, device=DEV), c.data, c.table, c.len, 32)
     ops.check_status()
