@@ -3,7 +3,7 @@
 // A single token's operators take 2 to 8 us on the device.  Looking at their tensors from Python, making outputs there and passing
 // twenty arguments through ctypes took 17 to 22 us a call; here it is 1 to 2 us beside the launch.  Each function returns its result
 // (tensors; a status code where the library refused the call), or None for whatever is out of the ordinary - a tensor on the CPU, rows
-// that are not whole words, a wrong shape, a gradient wanted - which the wrapper in ops.py then lays out or refuses with a reason.
+// that are not whole words, a wrong shape, a tangent - which the wrapper in ops.py then lays out or refuses with a reason.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -12,6 +12,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -87,6 +88,9 @@ bool integer(PyObject* o, int64_t& n) {
 }
 
 bool wants_gradient(const at::Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
+
+// Whether a derivative in forward mode is asked for: x has a tangent.
+bool wants_tangent(const at::Tensor& x) { return x._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode(); }
 
 PyObject* none() { Py_RETURN_NONE; }
 
@@ -228,7 +232,8 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   bool gradient = false;
   for (int i = 0; i < count; ++i) {
     int64_t unused[3];
-    if (!rotation.fits(*xs[i]) || !rows_of(*xs[i], unused) || xs[i]->scalar_type() != q->scalar_type() || xs[i]->size(0) != q->size(0)) return none();
+    if (!rotation.fits(*xs[i]) || !rows_of(*xs[i], unused) || xs[i]->scalar_type() != q->scalar_type() || xs[i]->size(0) != q->size(0) || wants_tangent(*xs[i]))
+      return none();
     gradient = gradient || wants_gradient(*xs[i]);
   }
   at::Tensor outs[2];

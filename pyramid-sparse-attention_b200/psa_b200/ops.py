@@ -9,6 +9,7 @@ from fractions import Fraction
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import PSA_FWD_BLOCKS_MAX, PSA_FWD_LIST_MAX, _calls, check, lib
@@ -928,14 +929,20 @@ def _rotate(xs, positions: torch.Tensor, plan, half: bool, inverse: bool):
 
 
 class _RotateAxes(torch.autograd.Function):
-    """The gradient of a rotation is the rotation back, through the same function: it can be differentiated again."""
+    """The gradient of a rotation is the rotation back, through the same function: it can be differentiated again.  Its derivative in forward
+    mode is the rotation of the tangents."""
 
     @staticmethod
     def forward(ctx, positions, plan, half, inverse, *xs):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.how = plan, half, inverse
         ctx.set_materialize_grads(False)
         return tuple(_rotate(xs, positions, plan, half, inverse))
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        return _RotateAxes.apply(ctx.saved_tensors[0], *ctx.how, *tangents[4:])
 
     @staticmethod
     def backward(ctx, *grads):
@@ -956,7 +963,7 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     by positions[axis of i] * frequency of i: theta^(-i / (D/2)), or with per_axis theta^(-j / n) for the j-th of an axis' n pairs;
     inv_freq: D/2 frequencies instead.  layout: "half" pairs channels (i, i + D/2), "pairs" (2i, 2i + 1).  A position of zero
     leaves a token as it is.  Angles are exact to 2^-24 turns at any position; values are computed in 32 bits and rounded once.
-    Returns the turned copies (q, or (q, k)), in the order of dimensions of their inputs; differentiable in q and k."""
+    Returns the turned copies (q, or (q, k)), in the order of dimensions of their inputs; differentiable in q and k, backward and in forward mode."""
     sections = tuple(map(int, sections))
     plan = _rotary_plan(q.size(-1), sections, float(theta), bool(per_axis), None if inv_freq is None else tuple(map(float, inv_freq)))
     half = layout == "half"
@@ -971,11 +978,13 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
         raise ValueError(f"rotate_axes: layout must be 'half' or 'pairs', got {layout!r}")
     if positions.dim() not in (2, 3) or positions.size(0) != len(sections):
         raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{len(sections)}, {q.size(0)}, {q.size(2)}]")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+    if any(forward_ad.unpack_dual(x).tangent is not None for x in xs):       # one by one: an operand may have none
+        outs = [_RotateAxes.apply(positions, plan, half, False, x)[0] for x in xs]
+    elif torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         outs = _RotateAxes.apply(positions, plan, half, False, *xs)
     else:
         outs = _rotate(xs, positions, plan, half, False)
-    return outs[0] if k is None else outs
+    return outs[0] if k is None else tuple(outs)
 
 
 def _state32(name: str, t: torch.Tensor, shape) -> None:

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_answering import DEV, HALF, SIZES, TINY, TYPES, Filled, attention, check_attention, gen, names, ops, randn, stands_for  # noqa: F401
+from test_gpu_answering import (DEV, HALF, SIZES, TINY, TYPES, Filled, angles, attention, check_attention, gen, names, near_turned, ops, randn,  # noqa: F401
+                                stands_for)
 
 pytestmark = pytest.mark.gpu
 # new tokens and query heads of one key head: rows for each of the five widths that the two attention kernels work in
@@ -153,4 +154,50 @@ def test_attention_of_more_tokens_than_it_takes_is_refused(ops):
     c = Filled(ops, gen(75), [20], 1, 64, 32, torch.bfloat16, 16)
     with pytest.raises(ValueError, match="tokens"):
         ops.kv4_attention(torch.zeros(1, 1, 65536, 64, dtype=torch.bfloat16, device=DEV), c.data, c.table, c.len, 32)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [*TYPES, torch.float32], **names)
+@pytest.mark.parametrize("layout", ["half", "pairs"])
+def test_rotary_axes_in_forward_mode(ops, dtype, layout):
+    """A tangent is turned as its operand is: of q, of k, of both, with a gradient wanted beside it, without gradients, of any layout."""
+    from torch.autograd import forward_ad
+    g = gen(76)
+    pos = torch.randint(0, 999, (2, 2, 9), generator=g, device=DEV)
+    ang = angles(pos, (12, 20), 1e4, False, 64)
+    q, tq = (randn(g, 2, 9, 3, 64, dtype=dtype).transpose(1, 2) for _ in range(2))
+    k, tk = randn(g, 2, 2, 9, 64, dtype=dtype), randn(g, 2, 1, 9, 1, dtype=dtype).expand(2, 2, 9, 64)
+    plain = ops.rotate_axes(q, k, pos, (12, 20), layout=layout)
+
+    def check(duals, tangents):
+        outs = ops.rotate_axes(duals[0], duals[1], pos, (12, 20), layout=layout)
+        for out, want, t in zip(outs, plain, tangents):
+            primal, tangent = forward_ad.unpack_dual(out)
+            assert torch.equal(primal, want) and (tangent is None) == (t is None)
+            if t is not None:
+                near_turned(tangent.detach(), t, ang, layout)
+        return outs
+    with forward_ad.dual_level():
+        check((forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk)), (tq, tk))
+        check((forward_ad.make_dual(q, tq), k), (tq, None))
+        check((q, forward_ad.make_dual(k, tk)), (None, tk))
+        check((q, k), (None, None))
+        with torch.no_grad():
+            check((forward_ad.make_dual(q, tq), k), (tq, None))
+        alone = forward_ad.unpack_dual(ops.rotate_axes(forward_ad.make_dual(q, tq), None, pos, (12, 20), layout=layout))
+        near_turned(alone.tangent, tq, ang, layout)
+        leaf = q.detach().clone().requires_grad_()
+        outs = check((forward_ad.make_dual(leaf, tq), k), (tq, None))
+        (back,) = torch.autograd.grad(forward_ad.unpack_dual(outs[0]).primal, leaf, tq)
+        near_turned(back, tq, -ang, layout)
+        # a tangent that comes to the gradient of the ordinary path is not dropped either
+        leaf = q.detach().clone().requires_grad_()
+        out = ops.rotate_axes(leaf, None, pos, (12, 20), layout=layout)
+        try:
+            (back,) = torch.autograd.grad(out, leaf, forward_ad.make_dual(q, tq))
+        except RuntimeError as e:
+            assert "jvp" in str(e)
+        else:
+            near_turned(forward_ad.unpack_dual(back).tangent, tq, -ang, layout)
+    assert all(torch.equal(a, b) for a, b in zip(ops.rotate_axes(q, k, pos, (12, 20), layout=layout), plain))
     ops.check_status()
