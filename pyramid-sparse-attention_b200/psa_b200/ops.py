@@ -5,6 +5,7 @@ import contextlib
 import ctypes as C
 import functools
 import math
+import threading
 from fractions import Fraction
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -62,15 +63,23 @@ def _mask32(mask: torch.Tensor) -> torch.Tensor:
 # the device is out of range) and nothing ever clears it except check_status().  Calls stay
 # free of host synchronisation; a run asks once, at the end (PSAAttention.check_status, close_logger).
 _STATUS: Dict[int, torch.Tensor] = {}
+_STATUS_LOCK = threading.Lock()
 
 
 def status_word(device) -> torch.Tensor:
     dev = torch.device(device)
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    if idx not in _STATUS:
-        _STATUS[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _calls.status(idx, _STATUS[idx].data_ptr())
-    return _STATUS[idx]
+    word = _STATUS.get(idx)
+    if word is None:
+        with _STATUS_LOCK:      # one word a device for good: kernels of every thread hold its address
+            word = _STATUS.get(idx)
+            if word is None:
+                word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(idx).synchronize()        # zero before another thread's stream writes into it
+                _calls.status(idx, word.data_ptr())
+                _STATUS[idx] = word
+    return word
 
 
 def check_status(device=None, reset: bool = True) -> None:

@@ -75,3 +75,36 @@ def test_scratch_holds_the_parts():
     from psa_b200._lib import lib
     few, many = (lib.psa_kv4_attention_scratch_bytes(1, n, 4, 1, 128) for n in (1, 65535))
     assert 0 < few < many
+
+
+def test_threads_make_one_status_word(monkeypatch):
+    """Whoever comes first makes the word of a device; nobody is given, or stores, the address of another."""
+    import threading
+    import time
+    from types import SimpleNamespace
+
+    import torch
+
+    from psa_b200 import ops
+    made, stored, got, real = [], [], [], torch.zeros
+
+    def zeros(*shape, dtype=None, device=None):
+        time.sleep(0.05)
+        made.append(real(*shape, dtype=dtype))
+        return made[-1]
+    monkeypatch.setattr(ops, "_STATUS", {})
+    monkeypatch.setattr(ops, "_calls", SimpleNamespace(status=lambda index, address: stored.append((index, address))))
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: SimpleNamespace(synchronize=lambda: None))
+    start = threading.Barrier(4)
+
+    def work():
+        start.wait()
+        got.append(ops.status_word("cuda:7"))
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and stored == [(7, made[0].data_ptr())] and all(w is made[0] for w in got) and len(got) == 4
