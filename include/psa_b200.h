@@ -446,7 +446,8 @@ int psa_rotate_axes(const void* const* src, const int64_t* src_strides, void* co
  * pool of free page numbers and how many of them are free (free_in[0], taken from the top) -> the same after the call, and
  * slots [requests][tokens] = page * page_size + place of each new token, -1 behind the last one.  Requests that need pages are served in
  * order while the running total of all needs fits the pool; one that is not served, would outgrow its row or has a count or
- * length out of range is given nothing.  Outputs may be their own inputs' memory (table, lengths, free).  page_size: a multiple of 16.
+ * length out of range is given nothing.  A token whose page has a number that no slot can have gets -1, and the status word says so.
+ * Outputs may be their own inputs' memory (table, lengths, free).  page_size: a multiple of 16.
  * scratch is not needed where all outputs lie beside the inputs and there are 1024 requests at most. */
 size_t psa_plan_pages_scratch_bytes(int64_t requests);
 int psa_plan_pages(const int32_t* table, const int32_t* lengths, const int32_t* counts, const int32_t* pool, const int32_t* free_in,

@@ -114,8 +114,12 @@ __device__ __forceinline__ void fill_row(const PlanArgs& a, int b, const Grant& 
     if (k != last) {
       last = k;
       page = k < g.held ? table[k] : a.pool[top - (k - g.held)];
+      if ((uint32_t)page >= (uint32_t)most_pages) {   // no slot has such a number
+        page = -1;
+        report(a.status, PSA_ERR_ARG);
+      }
     }
-    return page >= 0 && page < most_pages ? page * a.page + (at - k * a.page) : -1;
+    return page >= 0 ? page * a.page + (at - k * a.page) : -1;
   });
 }
 

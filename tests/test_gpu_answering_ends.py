@@ -201,3 +201,36 @@ def test_rotary_axes_in_forward_mode(ops, dtype, layout):
             near_turned(forward_ad.unpack_dual(back).tangent, tq, -ang, layout)
     assert all(torch.equal(a, b) for a, b in zip(ops.rotate_axes(q, k, pos, (12, 20), layout=layout), plain))
     ops.check_status()
+
+
+@pytest.mark.parametrize("requests,tokens", [(3, 20), (1100, 20), (3, 20000)])
+@pytest.mark.parametrize("where", ["beside", "in place"])
+def test_pages_of_no_slot_are_reported(ops, where, requests, tokens):
+    """A request's page that is none, and one that the pool names: their tokens have no slot, and the status word says so."""
+    def state(table_page, pool_page):
+        width = tokens // 16 + 2
+        table = torch.full((requests, width), -1, dtype=torch.int32, device=DEV)
+        table[:, 0] = torch.arange(requests, device=DEV)
+        table[1, 0] = table_page
+        pool = torch.arange(requests, 2 * requests * width, dtype=torch.int32, device=DEV)
+        pool[-1] = pool_page                             # the first page that is given away: request 0's
+        return table, torch.full((requests,), 5, dtype=torch.int32, device=DEV), pool, torch.tensor([pool.numel()], dtype=torch.int32, device=DEV)
+
+    def planned(*pages):
+        table, lengths, pool, free = state(*pages)
+        out = (table, lengths, free) if where == "in place" else None
+        return ops.plan_pages(table, lengths, torch.full_like(lengths, tokens), pool, free, 16, tokens, out=out)[3]
+    good = planned(1, 2 * requests * (tokens // 16 + 2))
+    ops.check_status()
+    assert bool((good >= 0).all())
+    for pages in ((-1, 7), (1, -9), (2 ** 27, 7), (1, 2 ** 31 - 1)):
+        slots = planned(*pages)
+        with pytest.raises(RuntimeError, match="out of range"):
+            ops.check_status()
+        gone = torch.zeros_like(slots, dtype=torch.bool)
+        if pages[0] != 1:
+            gone[1, :11] = True                          # places 5 .. 15 of its first page
+        else:
+            gone[0, 11:27] = True                        # its second page
+        assert torch.equal(slots < 0, gone)
+    ops.check_status()
