@@ -455,7 +455,8 @@ int psa_plan_pages(const int32_t* table, const int32_t* lengths, const int32_t* 
                    size_t scratch_bytes, int64_t requests, int64_t width, int64_t pool_size, int page_size, int64_t tokens,
                    int32_t* status, void* stream);
 /* The pages of the requests with which[b] != 0 go back on top of the pool, in an order that undoes psa_plan_pages; their lengths
- * become 0. */
+ * become 0.  Numbers that no slot can have (negative ones among them) do not: the pool takes the others, and the status word says so, as
+ * it does of lengths out of range and of pages that the pool has no room for. */
 int psa_release_pages(const int32_t* table, int32_t* lengths, const uint8_t* which, int32_t* pool, int32_t* free_count,
                       int64_t requests, int64_t width, int64_t pool_size, int page_size, int32_t* status, void* stream);
 

@@ -196,29 +196,66 @@ __global__ void __launch_bounds__(kRowThreads) fill_kernel(const PlanArgs a) {
 }
 
 // Pages of the requests marked in `which` go back on top of the pool, the last request's last page first: a request that is given
-// room and released at once leaves the pool as it was.
+// room and released at once leaves the pool as it was.  64 requests of 126 pages 4.1 us, 250 of 128 9.8.  Entries with numbers that no slot
+// can have stay away and leave no gap: where a round of requests has some, it is done again by the numbers of good entries.  (To count
+// those first took 5.3 and 14.3 us.)
 __global__ void __launch_bounds__(kPlanThreads) release_kernel(const int32_t* table, int32_t* lengths, const uint8_t* which, int32_t* pool,
                                                                int32_t* free_count, int requests, int width, int pool_size, int page,
                                                                int32_t* status) {
   __shared__ int warp_sums[32], held_of[kPlanThreads], end_of[kPlanThreads];
-  const int top = min(max(free_count[0], 0), pool_size);
+  const int top = min(max(free_count[0], 0), pool_size), lane = threadIdx.x & 31, most = width * page;
+  const uint32_t most_pages = 0x7fffffffu / page;
   int before = 0;
   for (int b0 = 0; b0 < requests; b0 += kPlanThreads) {
     const int b = requests - 1 - (b0 + (int)threadIdx.x);
     int held = 0;
-    if (b >= 0 && which[b]) held = pages_of(min(max(lengths[b], 0), width * page), page, -1);
+    if (b >= 0 && which[b]) {
+      const int length = lengths[b];
+      if (length < 0 || length > most) report(status, PSA_ERR_ARG);
+      held = pages_of(min(max(length, 0), most), page, -1);
+      lengths[b] = 0;
+    }
     held_of[threadIdx.x] = held;
     end_of[threadIdx.x] = before + block_scan(held, warp_sums);
-    if (held) lengths[b] = 0;
-    before += warp_sums[31];
+    const int all = warp_sums[31];
     __syncthreads();
     const int n = min(kPlanThreads, requests - b0);
+    bool stays = false;
     for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {   // a warp moves a request's pages
       const int32_t* row = table + (int64_t)(requests - 1 - (b0 + i)) * width;
-      for (int j = threadIdx.x & 31; j < held_of[i]; j += 32) {
+      for (int j = lane; j < held_of[i]; j += 32) {
         const int64_t at = (int64_t)top + end_of[i] - 1 - j;
-        if (at < pool_size) pool[at] = row[j];
-        else report(status, PSA_ERR_ARG);
+        const int number = row[j];
+        if ((uint32_t)number < most_pages && at < pool_size) pool[at] = number;
+        else stays = true;
+      }
+    }
+    if (!__syncthreads_or(stays)) {
+      before += all;
+      continue;
+    }
+    if (threadIdx.x == 0) report(status, PSA_ERR_ARG);
+    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {   // how many go back
+      const int32_t* row = table + (int64_t)(requests - 1 - (b0 + i)) * width;
+      int good = 0;
+      for (int j = lane; j < held_of[i]; j += 32) good += (uint32_t)row[j] < most_pages;
+      good = __reduce_add_sync(~0u, good);
+      if (lane == 0) end_of[i] = good;
+    }
+    __syncthreads();
+    const int end = before + block_scan((int)threadIdx.x < n ? end_of[threadIdx.x] : 0, warp_sums);
+    end_of[threadIdx.x] = end;
+    before += warp_sums[31];
+    __syncthreads();
+    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+      const int32_t* row = table + (int64_t)(requests - 1 - (b0 + i)) * width;
+      int64_t at = (int64_t)top + end_of[i] - 1;   // of the first page of 32
+      for (int j0 = 0; j0 < held_of[i]; j0 += 32) {
+        const int number = j0 + lane < held_of[i] ? row[j0 + lane] : -1;
+        const uint32_t mask = __ballot_sync(~0u, (uint32_t)number < most_pages);
+        const int64_t to = at - __popc(mask & ((1u << lane) - 1));
+        if ((uint32_t)number < most_pages && to < pool_size) pool[to] = number;
+        at -= __popc(mask);
       }
     }
     __syncthreads();

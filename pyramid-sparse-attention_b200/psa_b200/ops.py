@@ -1046,7 +1046,7 @@ def plan_pages(table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
 
 def release_pages(table: torch.Tensor, lengths: torch.Tensor, which: torch.Tensor, pool: torch.Tensor, free: torch.Tensor, page_size: int) -> None:
     """The pages of the requests marked in which (bool [requests]) go back to the pool and their lengths become 0, in place; an
-    order that undoes plan_pages."""
+    order that undoes plan_pages.  Entries of the table that no page has (-1) do not; check_status() says so."""
     if table.dim() != 2 or pool.dim() != 1 or which.dtype != torch.bool or which.shape != table.shape[:1]:
         raise ValueError("release_pages: table [requests, width], which bool [requests], pool [n]")
     if page_size < 16 or page_size % 16:

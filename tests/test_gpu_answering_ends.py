@@ -234,3 +234,44 @@ def test_pages_of_no_slot_are_reported(ops, where, requests, tokens):
             gone[0, 11:27] = True                        # its second page
         assert torch.equal(slots < 0, gone)
     ops.check_status()
+
+
+@pytest.mark.parametrize("requests", [3, 70, 1500])
+def test_release_puts_only_pages_into_the_pool(ops, requests):
+    """Entries that are no page of any cache stay out of the pool, without a gap in it; lengths out of range end at 0 and are reported."""
+    g = torch.Generator().manual_seed(requests)
+    width, page = 70, 16
+    table = torch.randperm(requests * width, generator=g).view(requests, width).to(torch.int32)
+    lengths = torch.randint(0, width * page + 1, (requests,), generator=g).to(torch.int32)
+    lengths[0] = width * page
+    bad = torch.rand(requests, width, generator=g) < 0.1
+    bad[1] = True
+    bad[2] = False
+    wrong = torch.tensor([-1, -2 ** 31, 2 ** 31 - 1, 2 ** 31 // page]).to(torch.int32)
+    table[bad] = wrong[torch.arange(int(bad.sum())) % 4]
+    which = torch.rand(requests, generator=g) < 0.7
+    which[:3] = True
+    room = requests * width + 5
+    pool = torch.full((room,), -7, dtype=torch.int32)
+    want = []
+    for b in reversed(range(requests)):
+        if which[b]:
+            held = table[b, :-(-int(lengths[b]) // page)].tolist()
+            want += [p for p in reversed(held) if 0 <= p < 2 ** 31 // page]
+    state = [t.to(DEV) for t in (table, lengths, which, pool, torch.tensor([4], dtype=torch.int32))]
+    ops.release_pages(*state, page)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    assert state[4].item() == 4 + len(want) and state[3][4:4 + len(want)].tolist() == want
+    assert bool((state[3][:4] == -7).all())                       # what lies behind the free ones is nobody's
+    assert torch.equal(state[1].cpu(), torch.where(which, 0, lengths)) and torch.equal(state[0].cpu(), table)
+    # lengths out of range: nothing below zero, a whole row above its end
+    far = torch.tensor([-5, width * page + 1, 3], dtype=torch.int32, device=DEV)
+    rows = torch.arange(3 * width, dtype=torch.int32, device=DEV).view(3, width)
+    pool, free = torch.full((3 * width,), -7, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.release_pages(rows, far, torch.ones(3, dtype=torch.bool, device=DEV), pool, free, page)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    assert far.tolist() == [0, 0, 0] and free.item() == 1 + width
+    assert pool[:1 + width].tolist() == [2 * width] + list(reversed(range(width, 2 * width))) and bool((pool[1 + width:] == -7).all())
+    ops.check_status()
