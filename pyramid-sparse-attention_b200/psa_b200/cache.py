@@ -4,11 +4,12 @@
     layers = [KV4Cache(table, kv_heads=4, head_dim=128, dtype=torch.bfloat16) for _ in range(28)]
     # every step: room for the new tokens once, then in each layer
     slots = table.reserve(counts, tokens)
+    counts = table.granted(counts, slots)
     cache.append(k, v, slots)
     out = cache.attend(q, counts)
 
 Nothing here reads a length back to the host, so a step can be captured in a CUDA graph and replayed; ops.check_status() says
-afterwards whether a request ran out of pages."""
+afterwards whether a request ran out of pages, and `granted` which: its rows come out as zeros."""
 from __future__ import annotations
 
 from typing import Optional
@@ -37,9 +38,15 @@ class PageTable:
         return self.pool.numel()
 
     def reserve(self, counts: torch.Tensor, tokens: int) -> torch.Tensor:
-        """Room for counts[b] <= tokens more tokens of every request -> slots int32 [requests, tokens] (ops.plan_pages, in place)."""
+        """Room for counts[b] <= tokens more tokens of every request -> slots int32 [requests, tokens] (ops.plan_pages, in place).  A request
+        that the pool or its row of the table has no room for gets none (see granted)."""
         state = self.table, self.lengths, self.free
         return ops.plan_pages(self.table, self.lengths, counts, self.pool, self.free, self.page_size, tokens, out=state)[3]
+
+    def granted(self, counts: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+        """How many new tokens each request has after reserve(counts, tokens) -> slots: counts, and 0 where it was refused (int32 [requests], on
+        the device).  With its own count a refused request's queries would stand at the tokens that it had before."""
+        return torch.where(slots[:, 0] >= 0, counts, 0).to(torch.int32)
 
     def release(self, which: torch.Tensor) -> None:
         """Ends the requests marked in which (bool [requests]): their pages are free again, their lengths 0."""
@@ -70,6 +77,7 @@ class KV4Cache:
         return ops.kv4_read(self.data, slots, self.head_dim, self.group, self.dtype)
 
     def attend(self, q: torch.Tensor, counts: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None, return_lse: bool = False):
-        """Attention of the newest tokens q [requests, heads, tokens, head_dim], their keys appended before (ops.kv4_attention)."""
+        """Attention of the newest tokens q [requests, heads, tokens, head_dim], their keys appended before (ops.kv4_attention); counts: as
+        PageTable.granted gives them."""
         self._own(q)
         return ops.kv4_attention(q, self.data, self.table.table, self.table.lengths, self.group, counts, sm_scale, return_lse)

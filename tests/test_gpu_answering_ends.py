@@ -275,3 +275,45 @@ def test_release_puts_only_pages_into_the_pool(ops, requests):
     assert far.tolist() == [0, 0, 0] and free.item() == 1 + width
     assert pool[:1 + width].tolist() == [2 * width] + list(reversed(range(width, 2 * width))) and bool((pool[1 + width:] == -7).all())
     ops.check_status()
+
+
+@pytest.mark.parametrize("counts_dtype", [torch.int32, torch.int64], **names)
+def test_refused_requests_answer_nothing(ops, counts_dtype):
+    """Of three requests one fills its row and one finds the pool empty: `granted` says so on the device, their rows are zeros, the others'
+    are as without them; in a captured step too."""
+    from psa_b200.cache import KV4Cache, PageTable
+    g = gen(77)
+    B, H, D, n = 4, 4, 64, 3
+    table = PageTable(B, 64, 9, 16, DEV)
+    cache = KV4Cache(table, 1, D, torch.bfloat16)
+    held = torch.tensor([20, 62, 48, 0], device=DEV)
+    # pages: 2, 4 and 3 of 9; the first step needs none for request 0, one that the pool does not have for 2 and for 3, and 1's row is full
+    rows = [randn(g, B, 1, 62, D, dtype=torch.bfloat16) for _ in range(2)]
+    cache.append(*rows, table.reserve(held, 62))
+    ops.check_status()
+    want_counts = torch.tensor([n, 0, 0, 0], device=DEV)
+    k, v = (randn(g, B, 1, n, D, dtype=torch.bfloat16) for _ in range(2))
+    q = randn(g, B, H, n, D, dtype=torch.bfloat16)
+    counts = torch.full((B,), n, dtype=counts_dtype, device=DEV)
+
+    def step():
+        slots = table.reserve(counts, n)
+        ok = table.granted(counts, slots)
+        cache.append(k, v, slots)
+        return ok, cache.attend(q, ok)
+    ok, out = step()
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    assert ok.dtype == torch.int32 and torch.equal(ok.long(), want_counts)
+    assert table.lengths.tolist() == [23, 62, 48, 0] and not bool(out[1:].any()) and bool(out[0].any(-1).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ok, out = step()
+    graph.replay()
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    assert torch.equal(ok.long(), want_counts) and table.lengths.tolist() == [26, 62, 48, 0] and not bool(out[1:].any())
+    table.release(torch.tensor([False, True, False, False], device=DEV))
+    ok, out = step()
+    ops.check_status()
+    assert ok.tolist() == [n] * B and bool(out.any(-1).all()) and table.lengths.tolist() == [29, 3, 51, 3]
