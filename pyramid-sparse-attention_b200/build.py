@@ -5,11 +5,13 @@
 Each csrc/*.cu is compiled to build/*.o in parallel with
 ``nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` and linked into
 psa_b200/libpsa_b200.so; csrc/calls.cpp, the Python entry to some of its calls, is compiled with the host compiler
-against torch's headers and linked with that library into psa_b200/_calls.so.  Objects are reused when they are newer than every source and header.
+against torch's headers and linked with that library into a module whose name says which torch and which Python it is for
+(calls_name.py).  Objects are reused when they are newer than every source and header.
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -21,7 +23,6 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "psa_b200", "libpsa_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-CALLS = os.path.join(HERE, "psa_b200", "_calls.so")
 CXX = os.environ.get("CXX", "g++")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
@@ -68,17 +69,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def calls_path() -> str:
+    spec = importlib.util.spec_from_file_location("calls_name", os.path.join(HERE, "psa_b200", "calls_name.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return os.path.join(HERE, "psa_b200", mod.calls_name())
+
+
 def build_calls(force: bool, hdr_t: float) -> None:
-    import torch
-    src = os.path.join(CSRC, "calls.cpp")
-    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), hdr_t):
+    try:
+        import torch
+    except ImportError:
+        print("no torch: the C library alone")
+        return
+    src, out = os.path.join(CSRC, "calls.cpp"), calls_path()
+    for old in glob.glob(os.path.join(HERE, "psa_b200", "_calls*.so")):
+        if old != out:
+            os.remove(old)       # of another torch or Python
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), hdr_t):
         return
     at = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(NVCC)) or "/usr/local/cuda"
     include = [os.path.join(HERE, "..", "include"), os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     abi = f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
-    r = subprocess.run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", abi, *[f"-I{i}" for i in include], src, "-o", CALLS,
+    r = subprocess.run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", abi, *[f"-I{i}" for i in include], src, "-o", out,
                         f"-L{os.path.dirname(LIB)}", f"-l:{os.path.basename(LIB)}", "-Wl,-rpath,$ORIGIN", f"-L{os.path.join(at, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"],
                        capture_output=True, text=True)
     if r.returncode != 0:

@@ -6,7 +6,12 @@ this module raises, and every op raises if its tensors are not CUDA tensors.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
+import sys
+import warnings
+
+from .calls_name import calls_name
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpsa_b200.so")
@@ -24,9 +29,41 @@ if not os.path.exists(LIB_PATH):
 
 lib = C.CDLL(LIB_PATH)
 
-import torch  # noqa: E402,F401  (_calls links against its libraries)
 
-from . import _calls  # noqa: E402,F401  (built beside the library: the answering operators' ordinary calls in one step)
+class NoCalls:
+    """Stands for _calls where that is not there: every call is out of the ordinary and laid out by its wrapper in ops.py, with the
+    same kernels and results, 8 to 13 us of the host more each."""
+
+    @staticmethod
+    def status(index, address):
+        pass
+
+    @staticmethod
+    def _none(*args):
+        return None
+
+    rotate = plan_pages = append = read = attend = _none
+
+
+def load_calls(path: str):
+    """The module of the ordinary calls at path, or NoCalls and a warning."""
+    why = "is not there"
+    if os.path.exists(path):
+        try:
+            spec = importlib.util.spec_from_file_location(f"{__package__}._calls", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            return module
+        except ImportError as e:
+            why = f"does not load ({e})"
+    warnings.warn(f"{path} {why}: single-token calls take longer on the host. "
+                  "`python pyramid-sparse-attention_b200/build.py` builds it for this torch and Python.", RuntimeWarning, stacklevel=2)
+    return NoCalls
+
+
+_calls = load_calls(os.path.join(_HERE, calls_name()))
+if _calls is not NoCalls:
+    sys.modules[f"{__package__}._calls"] = _calls
 
 _p, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 

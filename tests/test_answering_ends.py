@@ -108,3 +108,27 @@ def test_threads_make_one_status_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(made) == 1 and stored == [(7, made[0].data_ptr())] and all(w is made[0] for w in got) and len(got) == 4
+
+
+def test_native_calls_of_other_versions_are_not_loaded(monkeypatch, tmp_path):
+    """The module's name says what it was compiled against; without one of the running versions, and with one that does not load, importing
+    warns and every call is laid out by its wrapper."""
+    import torch
+
+    from psa_b200 import _lib
+    from psa_b200.calls_name import calls_name
+    here = os.path.dirname(_lib.__file__)
+    now = calls_name()
+    assert torch.__version__ in now and os.path.exists(os.path.join(here, now)) and _lib._calls is not _lib.NoCalls
+    assert [f for f in os.listdir(here) if f.startswith("_calls") and f.endswith(".so")] == [now]
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    assert calls_name() != now
+    with pytest.warns(RuntimeWarning, match="is not there"):
+        assert _lib.load_calls(os.path.join(here, calls_name())) is _lib.NoCalls
+    broken = tmp_path / "_calls-broken.so"
+    broken.write_bytes(b"not a library")
+    with pytest.warns(RuntimeWarning, match="does not load"):
+        assert _lib.load_calls(str(broken)) is _lib.NoCalls
+    names = [n for n in dir(_lib._calls) if not n.startswith("_")]
+    assert sorted(names) == ["append", "attend", "plan_pages", "read", "rotate", "status"]
+    assert all(getattr(_lib.NoCalls, n)(0, 0) is None for n in names)

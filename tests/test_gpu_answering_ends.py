@@ -317,3 +317,33 @@ def test_refused_requests_answer_nothing(ops, counts_dtype):
     ok, out = step()
     ops.check_status()
     assert ok.tolist() == [n] * B and bool(out.any(-1).all()) and table.lengths.tolist() == [29, 3, 51, 3]
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+def test_calls_without_the_native_module(ops, monkeypatch, dtype):
+    """Laid out in Python, every operator gives the same bits."""
+    from psa_b200 import _lib
+    from psa_b200.cache import KV4Cache, PageTable
+
+    def everything():
+        g = gen(78)
+        table = PageTable(3, 200, 40, 16, DEV)
+        cache = KV4Cache(table, 2, 64, dtype)
+        got = []
+        for n, counts in ((90, [90, 3, 0]), (1, [1, 1, 1]), (4, [4, 0, 3])):
+            q, k, v = (randn(g, 3, n, h, 64, dtype=dtype).transpose(1, 2).requires_grad_() for h in (4, 2, 2))
+            count = torch.tensor(counts, dtype=torch.int32, device=DEV)
+            pos = (table.lengths[:, None] + torch.arange(n, dtype=torch.int32, device=DEV)).expand(3, 3, n)
+            beside = ops.plan_pages(table.table, table.lengths, count, table.pool, table.free, 16, n)
+            slots = table.reserve(count, n)
+            turned = ops.rotate_axes(q, k, pos, (8, 12, 12))
+            got += [*turned, *torch.autograd.grad(turned, (q, k), [torch.ones_like(t) for t in turned]), ops.rotate_axes(q.detach(), None, pos, (32, 0, 0), layout="pairs")]
+            cache.append(turned[1].detach(), v.detach(), slots)
+            got += [*beside, slots, cache.attend(turned[0].detach(), count), *cache.read(slots)]
+            got += ops.kv4_attention(turned[0].detach(), cache.data, table.table, table.lengths, 32, count, 0.3, return_lse=True)
+        ops.check_status()
+        return got
+    native = everything()
+    monkeypatch.setattr(ops, "_calls", _lib.NoCalls)
+    for a, b in zip(native, everything()):
+        assert torch.equal(a, b) and a.stride() == b.stride()
