@@ -78,7 +78,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int rows_per_t
   count = min(max(count, 0), a.tokens);
   s.rows = count * a.group;
   s.row_tiles = (s.rows + rows_per_tile - 1) / rows_per_tile;
-  s.tiles = (length + kTile - 1) / kTile;
+  s.tiles = (int)(((uint32_t)length + kTile - 1) / kTile);   // lengths up to 2^31 - 16
   s.cells = s.tiles ? s.tiles + a.unit_cells : 0;
   s.work = s.cells * s.row_tiles * a.kv_heads;   // the entry point sees to it that the sum over all requests fits 32 bits
   return s;

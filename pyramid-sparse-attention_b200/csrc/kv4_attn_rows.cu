@@ -442,12 +442,12 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
     const int all_see = p.length - p.count + p.row0 / group + 1;   // keys that every row of the unit sees
     const uint32_t area_at = tc::smem_u32(area);
     int t0 = p.tile0 * kTile + 16 * own;
-    for (int i = 0; i < p.tiles; ++i, t0 += kTile) {
+    for (int i = 0; i < p.tiles; ++i, t0 = (int)((uint32_t)t0 + kTile)) {
       if (!dead && !__all_sync(~0u, tc::mbar_try_wait(full + stage, phase))) dead = !__all_sync(~0u, tc::mbar_wait(full + stage, phase, abort_flag));
       const uint8_t* tile = smem + stage * S::kTileBytes;
       const uint8_t* slice = tile + own * L::kSlice;
       const bool there = valid[stage] >> own & 1;
-      const int token = (there ? t0 : 1 << 30) + (r >> 1) + 4 * (r & 1);   // a slice that is not there lies behind every key
+      const int token = (there ? t0 : 0x7ffffff0) + (r >> 1) + 4 * (r & 1);   // a slice that is not there lies behind every key
       const uint32_t weights = area_at + (S::kBuffers == 2 && (i & 1) ? S::kWeights : 0) + tile0 * 256, to = weights + own * (S::kTiles * 256);
       float e[NT][4];
       if (S::kBuffers == 1 && i) __syncthreads();                          // the weights before have been used

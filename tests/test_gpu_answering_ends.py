@@ -347,3 +347,31 @@ def test_calls_without_the_native_module(ops, monkeypatch, dtype):
     monkeypatch.setattr(ops, "_calls", _lib.NoCalls)
     for a, b in zip(native, everything()):
         assert torch.equal(a, b) and a.stride() == b.stride()
+
+
+@pytest.mark.parametrize("H", [2, 20])
+def test_attention_of_the_longest_row_of_a_table(ops, H):
+    """2^31 - 16 tokens, all on one page of 16: the number of tiles, and places beyond 2^30, fit their 32 bits; so do places of pages that are
+    not there."""
+    page, width = 16, (1 << 27) - 1
+    data = ops.kv4_empty(1, 1, page, 64, 64, DEV)
+    g = gen(79)
+    row = randn(g, 1, 1, 1, 64, dtype=torch.bfloat16).expand(1, 1, page, 64)
+    ops.kv4_append(data, row, row, torch.arange(page, device=DEV)[None], 64)
+    q = randn(g, 1, H, 1, 64, dtype=torch.bfloat16)
+    table = torch.zeros(1, width, dtype=torch.int32, device=DEV)
+    length = torch.tensor([width * page], dtype=torch.int32, device=DEV)
+    k = stands_for(row, 64)[0, 0, 0]
+    score = (q[0, :, 0].double() @ k) / 8
+    for tokens in (width * page, 1 << 30):
+        table[0, tokens // page:] = -1
+        out, lse = ops.kv4_attention(q, data, table, length, 64, return_lse=True)
+        if tokens < width * page:
+            with pytest.raises(RuntimeError, match="out of range"):
+                ops.check_status()
+        # a lane adds two weights a slice, of 2^27 slices in 148 x 2 blocks' 4 warps or more: 2^-24 of the sum each
+        adds = 2 * 2 ** 27 / (148 * 2 * 4)
+        assert bool(((lse[0, :, 0].double() - score - math.log(tokens)).abs() <= adds * 2.0 ** -24 + 2.0 ** -10).all())
+        # every value is the same, so is every output: weights and their products with it are rounded alike but for what sums lose
+        assert bool(((out[0, :, 0].double() - k).abs() <= 2.0 ** -8 * k.abs() + (2 * adds * 2.0 ** -24 + 2.0 ** -11) * 15 * k.abs().amax()).all())
+    ops.check_status()
