@@ -1005,7 +1005,9 @@ def _ints32(name: str, t: torch.Tensor, shape) -> torch.Tensor:
     """Numbers made for the call, which may be int64 or strided."""
     if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be an int32 or int64 tensor of shape {tuple(shape)}")
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:       # a number beyond 32 bits stays out of range
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def plan_pages(table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, pool: torch.Tensor, free: torch.Tensor, page_size: int,

@@ -132,3 +132,14 @@ def test_native_calls_of_other_versions_are_not_loaded(monkeypatch, tmp_path):
     names = [n for n in dir(_lib._calls) if not n.startswith("_")]
     assert sorted(names) == ["append", "attend", "plan_pages", "read", "rotate", "status"]
     assert all(getattr(_lib.NoCalls, n)(0, 0) is None for n in names)
+
+
+def test_numbers_of_64_bits_keep_their_side_of_the_range():
+    import torch
+
+    from psa_b200 import ops
+    far = torch.tensor([5, -1, 2 ** 32 + 5, -2 ** 32, 2 ** 31, -2 ** 31 - 1, 2 ** 62], dtype=torch.int64)
+    got = ops._ints32("slots", far, (7,))
+    assert got.dtype == torch.int32 and got.tolist() == [5, -1] + [2 ** 31 - 1, -2 ** 31] * 2 + [2 ** 31 - 1]
+    strided = torch.arange(8, dtype=torch.int32)[::2]
+    assert ops._ints32("counts", strided, (4,)).is_contiguous() and ops._ints32("counts", strided, (4,)).tolist() == [0, 2, 4, 6]

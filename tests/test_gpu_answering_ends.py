@@ -375,3 +375,30 @@ def test_attention_of_the_longest_row_of_a_table(ops, H):
         # every value is the same, so is every output: weights and their products with it are rounded alike but for what sums lose
         assert bool(((out[0, :, 0].double() - k).abs() <= 2.0 ** -8 * k.abs() + (2 * adds * 2.0 ** -24 + 2.0 ** -11) * 15 * k.abs().amax()).all())
     ops.check_status()
+
+
+def test_numbers_beyond_32_bits_are_out_of_range(ops):
+    """Slots and counts of 64 bits whose lower halves would do: skipped, refused or cut, and reported."""
+    g = gen(80)
+    far = 2 ** 32
+    data = torch.zeros_like(ops.kv4_empty(1, 1, 16, 64, 32, DEV))
+    row = randn(g, 1, 1, 3, 64, dtype=torch.bfloat16)
+
+    def reported():
+        with pytest.raises(RuntimeError, match="out of range"):
+            ops.check_status()
+    ops.kv4_append(data, row, row, torch.tensor([[far, far + 5, -far + 7]], device=DEV), 32)
+    reported()
+    assert not bool(data.any())
+    ops.kv4_append(data, row, row, torch.tensor([[0, 1, 2]], device=DEV), 32)
+    ops.check_status()
+    assert not bool(ops.kv4_read(data, torch.tensor([[far, far + 1]], device=DEV), 64, 32, torch.bfloat16)[0].any())
+    reported()
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([3], dtype=torch.int32, device=DEV)
+    pool, free = torch.zeros(1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    _, after, _, slots = ops.plan_pages(table, lengths, torch.tensor([far + 1], device=DEV), pool, free, 16, 2)
+    reported()
+    assert after.tolist() == [3] and slots.tolist() == [[-1, -1]]
+    q = randn(g, 1, 2, 2, 64, dtype=torch.bfloat16)
+    assert not bool(ops.kv4_attention(q, data, table, lengths, 32, torch.tensor([-far + 2], device=DEV)).any())
+    reported()
