@@ -427,7 +427,8 @@ int psa_fwd_images_scatter(const void* q, const void* kimg, const void* vimg, co
 /* ---------------------------------------------------------------------------------------------------------------------
  * The answering side of the vision-language call site: what a decoder needs around the causal attention of the prompt.  The
  * reference hands single tokens back to the model's own attention (qwen2.5-vl-example/src/attention/qwen2vl_attention.py), so
- * these have no counterpart there.  Row strides are in elements; channels are neighbours; every pointer is 16-byte aligned.
+ * these have no counterpart there.  Row strides are in elements; channels are neighbours; rows, the
+ * cache and the scratch are 16-byte aligned, numbers as their type is.
  * `status` is the int32 word described above: PSA_ERR_ARG is written into it where a page number, slot, length or count found
  * on the device is out of range (the access is skipped) or a request could not be given pages; a
  * PSA_ERR_TIMEOUT that is already there stays. */

@@ -12,7 +12,7 @@
 // accumulators near zero.  Sums of codes alone would grow with the context, the tensor cores cut their sums off, and what is cut off
 // adds up (0.1 % of an output of 131072 evenly weighted keys).
 //
-// Work: one tile is 64 tokens of one key head, for up to R query rows (new tokens x query heads of that key head; 8 or 16 here, 32 or 48 in
+// Work: one tile is 64 tokens of one key head, for up to R query rows (new tokens x query heads of that key head; 8 or 16 here, 24, 32 or 48 in
 // kv4_attn_rows.cu).  All tiles of all requests stand in one line, and every block takes an equal stretch of it, computed from the lengths
 // on the device: requests of any mix of lengths load the GPU evenly.  A row's tiles may lie in several blocks; their parts (running
 // maximum, sum, output) are joined in order by a second kernel.  A block: one warp copies tiles into a ring (one copy where pages hold
@@ -22,8 +22,8 @@
 //
 // The floor is the cache's bytes (160 a token and key head at head_dim 128, groups of 32).  mma.sync and not tcgen05: 8 query rows
 // against 128 rows of a tcgen05 tile, and operands that are made in registers; the products take a fifth of a warp's issue slots.  8 requests
-// of 131071 tokens, 28 heads on 4, bf16: 134-139 us (5.0 TB/s; 103 us at copy speed).  The copies alone take 104: what bounds it is issue
-// slots, 358 instructions a slice - 88 take the codes apart, 17 are products - at two thirds of a slot a cycle.  Waiting for tiles one by
+// of 131071 tokens, 28 heads on 4, bf16: 135-137 us (4.9-5.0 TB/s; 103 us at copy speed).  The copies alone take 104: what bounds it is issue
+// slots, 340 instructions a slice - 88 take the codes apart, 17 are products - at two thirds of a slot a cycle.  Waiting for tiles one by
 // one cost 30 instructions more (149 us), a ring of its own for every warp 170 us, outputs split by channels as in kv4_attn_rows.cu 164.
 #include "kv4_attn.cuh"
 
@@ -532,7 +532,8 @@ int rows_per_tile(int64_t rows) {
   return most <= 8 ? 8 : most <= 16 ? 16 : most <= 24 ? 24 : most <= 32 ? 32 : 48;
 }
 // What a unit's beginning and end cost, in tiles (33 requests of 17 to 16384 tokens, 16 key heads of 64 channels: 87 us with 1, 62 with 2, 46
-// with 4, 41 with 8, 45 with 12; 4 key heads of 128 with 5 tokens: 74 us with 2, 64 with 3, 63 with 4).
+// with 4, 41 with 8, 45 with 12; the same requests, 4 key heads of 128 channels: 20.8 us with 4, 20.3 with 6, 20.8 with 8, 21.5 with 10, and 5
+// requests of 5000: 18.3, 16.6, 16.7, 16.8; 4 key heads of 128 with 5 tokens, more than 16 rows: 74 us with 2, 64 with 3, 63 with 4).
 int unit_cells(int head_dim, int rows) { return rows > 16 ? 4 : head_dim == 64 ? 8 : 6; }
 // The least cells of a block: few, which leaves a small call's tiles to many blocks (500 tokens, 4 key heads: 8.2 us with 2, 11.7 with 10).
 int least_cells(int rows) { return rows > 16 ? 1 : 2; }

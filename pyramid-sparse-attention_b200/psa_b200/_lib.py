@@ -32,7 +32,7 @@ lib = C.CDLL(LIB_PATH)
 
 class NoCalls:
     """Stands for _calls where that is not there: every call is out of the ordinary and laid out by its wrapper in ops.py, with the
-    same kernels and results, 8 to 13 us of the host more each."""
+    same kernels and results, 8 to 12 us of the host more each."""
 
     @staticmethod
     def status(index, address):
