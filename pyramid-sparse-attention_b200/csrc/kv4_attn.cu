@@ -63,7 +63,7 @@ struct Rows {
   float ref[NT][2], sum[NT][2];
   float out[NT][2 * NB][4]; // of channels 4 i, 4 i + 2: times 2^-24, of the others: times 2^-20
   float mid[NT][NG][2];
-  float cap, limit;         // at least the largest step of the values so far, and the exponent from which a weight is too large
+  float cap, limit;         // groups of 32: the largest need so far (a power of two), and the exponent from which a weight times it is too large
   int seen[NT][2];          // keys that a column's row sees
   int last;                 // keys of the request
 };
@@ -115,53 +115,77 @@ __device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const 
   float x[N][NT][4], e[N][NT][4];
 #pragma unroll
   for (int n = 0; n < N; ++n) score<T, D, G, NT>(x[n], s, slice[n]);
-  // ---- the largest step of the values (or what stands for one): a lane looks at one group of its two rows
-  float widest = 0.f, most = -INFINITY;
+  // ---- weights, and whether one times its token's need is too large.  To look token by token takes few instructions where a token has few
+  // groups.  With groups of 32 a warp keeps the largest need that it has met and looks only where a weight times that is too large: 8 x 131071
+  // tokens of 128 channels 134.5 us instead of 140-142, 16 x 65536 of 64 channels 44.5 instead of 45.9; groups of 64 the other way round: 33
+  // ragged requests of 64 channels 34.9 and 33.8, 2 new tokens of 5 x 20000 31.8 and 29.8.
+  constexpr bool kKept = G == 32;
   int token[N];
+  float need[N][2], widest = 0.f, most = kKept ? -INFINITY : 0.f;
+  auto look_up = [&](int n) {
+    const uint8_t* p = slice[n] + L::kHalf + L::kParams + r * NG * 4;
+    need[n][0] = need_of<T, NG>(lds<NG>(p));
+    need[n][1] = need_of<T, NG>(lds<NG>(p + 8 * NG * 4));
+  };
+  auto distance = [&](int n, int nt, int j) {   // to the reference; then, or at once, weights
+    const float t = fmaf(x[n][nt][j], s.factor[nt][j & 1], -s.ref[nt][j & 1]);
+    const float u = MASKED && token[n] + 8 * (j >> 1) >= s.seen[nt][j & 1] ? -INFINITY : t;
+    return kKept ? u : ex2(u);
+  };
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     token[n] = t0[n] + (r >> 1) + 4 * (r & 1);
-    const uint8_t* p = slice[n] + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
-    uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
-    if (MASKED) {   // what lies behind the last key may be anything
-      w0 = token[n] < s.last ? w0 : 0u;
-      w1 = token[n] + 8 < s.last ? w1 : 0u;
+    if constexpr (kKept) {
+      const uint8_t* p = slice[n] + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;   // a lane looks at one group of its two rows
+      Words<2> w = {lds<1>(p + r * NG * 4).w[0], lds<1>(p + (r + 8) * NG * 4).w[0]};
+      if (MASKED) {   // what lies behind the last key may be anything
+        w.w[0] = token[n] < s.last ? w.w[0] : 0u;
+        w.w[1] = token[n] + 8 < s.last ? w.w[1] : 0u;
+      }
+      widest = fmaxf(widest, need_of<T, 2>(w));
+    } else {
+      look_up(n);
     }
-    widest = fmaxf(widest, wanted<T>(w0, w1));
+    float top[2] = {most, most};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        e[n][nt][j] = fmaf(x[n][nt][j], s.factor[nt][j & 1], -s.ref[nt][j & 1]);
-        if (MASKED && token[n] + 8 * (j >> 1) >= s.seen[nt][j & 1]) e[n][nt][j] = -INFINITY;
-        most = fmaxf(most, e[n][nt][j]);
+        e[n][nt][j] = distance(n, nt, j);
+        top[j >> 1] = fmaxf(top[j >> 1], e[n][nt][j]);
       }
+    most = kKept ? fmaxf(top[0], top[1]) : 0.f;
+    if constexpr (!kKept) widest = fmaxf(widest, fmaxf(top[0] * need[n][0], top[1] * need[n][1]));
   }
-  // ---- the references move seldom: when a weight times a step could leave f16
-  if (__any_sync(~0u, widest > s.cap || most > s.limit)) {
+  // ---- the references move seldom
+  if (__any_sync(~0u, kKept ? widest > s.cap || most > s.limit : widest > kMost)) {
+    if constexpr (kKept) {
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
-    const float old = log2f(s.cap);
-    s.cap = power_above(s.cap, widest);
-    const float up = log2f(s.cap);
-    s.limit = kHead + kLazy - up;
+      for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
+      s.cap = power_above(s.cap, widest);
+      s.limit = kMostLog2 - log2_above(s.cap);
+#pragma unroll
+      for (int n = 0; n < N; ++n) look_up(n);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = -INFINITY;
+        float m = -INFINITY, over = 0.f;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            e[n][nt][2 * i + j] = MASKED && token[n] + 8 * i >= s.seen[nt][j] ? -INFINITY : x[n][nt][2 * i + j] * s.factor[nt][j];
-            m = fmaxf(m, e[n][nt][2 * i + j]);
+            const float w = e[n][nt][2 * i + j];
+            over = fmaxf(over, (kKept ? ex2(w) : w) * need[n][i]);
+            if (!MASKED || token[n] + 8 * i < s.seen[nt][j]) m = fmaxf(m, x[n][nt][2 * i + j] * s.factor[nt][j] + log2_above(need[n][i]));
           }
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-        // largest score so far, or what the reference stood for
-        const float ref = fmaxf(m, s.ref[nt][j] - old + kHead) + (up - kHead), fade = half_of(s.ref[nt][j] - ref);
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) {
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+          over = fmaxf(over, __shfl_xor_sync(~0u, over, d));
+        }
+        const float ref = over > kMost ? fmaxf(m - kHead, s.ref[nt][j]) : s.ref[nt][j], fade = half_of(s.ref[nt][j] - ref);
         s.ref[nt][j] = ref;
         s.sum[nt][j] = faded(s.sum[nt][j], fade);
 #pragma unroll
@@ -173,8 +197,8 @@ __device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const 
         }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          e[n][nt][j] -= ref;
-          e[n][nt][2 + j] -= ref;
+          e[n][nt][j] = distance(n, nt, j);
+          e[n][nt][2 + j] = distance(n, nt, 2 + j);
         }
       }
   }
@@ -184,7 +208,7 @@ __device__ __forceinline__ void take(Rows<T, D, G, NT>& s, const uint8_t* const 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        e[n][nt][j] = ex2(e[n][nt][j]);
+        if constexpr (kKept) e[n][nt][j] = ex2(e[n][nt][j]);
         s.sum[nt][j & 1] += e[n][nt][j];
       }
   // ---- outputs: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12); channels 32 b + 4 r + 0..3
@@ -332,8 +356,8 @@ __global__ void __launch_bounds__(kThreads, blocks_of(8 * NT)) kv4_attn_kernel(c
 #pragma unroll
           for (int i = 0; i < 2 * NB; ++i) s.out[nt][i][0] = s.out[nt][i][1] = s.out[nt][i][2] = s.out[nt][i][3] = 0.f;
         }
-        s.cap = kLeastCap;
-        s.limit = kHead + kLazy - kLeastCapLog2;
+        s.cap = kLeastNeed<T>;
+        s.limit = kMostLog2 - log2_above(s.cap);
         s.last = length;
         const int all_see = length - count + row0 / group + 1;   // keys that every row of the unit sees
         // tiles whose tokens every row sees, then the others

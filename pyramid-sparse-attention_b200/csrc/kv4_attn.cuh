@@ -42,13 +42,16 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int b, int head, in
 
 constexpr int kWarps = 4, kTile = 16 * kWarps;   // slices and tokens of a tile
 constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has seen nothing: exp2(-inf - kLowest) is 0
-// A weight is 2^(score - reference).  References are set so that the largest score so far, times the largest step of the values so far, gives
-// 2^kHead, and move when a weight times a step could be 2^kLazy times that: f16 has its full precision from 2^-14 to 2^16, so a
-// weight 2^-21 of the largest is still rounded to 11 bits.
-constexpr float kHead = 7.f, kLazy = 8.f;
-// Steps from 2^-80 on keep that precision, and up to 2^100 (below 2^-126 weights are 0): weights are up to 2^95, and 2^31 of them fit 32 bits.
-// Groups of one value have no step: 2^-64 of their size counts as one, so that weights times lowest values are up to 2^79.
-constexpr float kLeastCapLog2 = -80.f, kLeastCap = 8.271806125530277e-25f, kLowestShare = 5.421010862427522e-20f;
+// A weight is 2^(score - reference), and meets the steps of its token's values in f16.  A token's need is the largest of its steps; where its groups
+// are constant and have none, 2^-64 of its values' size; and kLeastNeed at least.  A row's reference moves when a weight times its token's need
+// is above 2^15, to where the largest of these products is 2^kHead: f16 has its full precision from 2^-14 to 2^16, so a product 2^-20 of the
+// largest is still rounded to 11 bits.  A row looks at its own tokens alone: what it does not see, and what other rows see, changes no
+// bit of it.
+// Weights are up to 2^95 (f16 tensors: 2^63), 2^31 of them fit 32 bits, and so do as many of up to 2^79 times a lowest value.  Steps may be up to
+// 2^100 (below 2^-126 weights are 0).
+constexpr float kHead = 7.f, kMostLog2 = 15.f, kMost = 32768.f, kLowestShare = 5.421010862427522e-20f;
+// f16: 2^-64 of the largest number; a step is 2^-24 or more.
+template <typename T> constexpr float kLeastNeed = std::is_same<T, __half>::value ? 3.552713678800501e-15f : 8.271806125530277e-25f;   // 2^-48, 2^-80
 // The smallest power of two that is not below x, or `least` if that is larger.
 __device__ __forceinline__ float power_above(float least, float x) {
   return x > least ? __uint_as_float((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u) : least;
@@ -262,18 +265,6 @@ template <> __device__ __forceinline__ float2 param<__nv_bfloat16>(uint32_t w) {
 }
 template <> __device__ __forceinline__ float2 param<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// What a group's values want of the references: two parameter words -> the larger step, or 2^-64 of the larger lowest value's size.
-template <typename T> __device__ __forceinline__ float wanted(uint32_t w0, uint32_t w1);
-template <> __device__ __forceinline__ float wanted<__nv_bfloat16>(uint32_t w0, uint32_t w1) {
-  const __nv_bfloat162 x = __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&w0)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w1)));
-  const float2 p = param<__nv_bfloat16>(*reinterpret_cast<const uint32_t*>(&x));
-  return fmaxf(p.x, p.y * kLowestShare);
-}
-template <> __device__ __forceinline__ float wanted<__half>(uint32_t w0, uint32_t w1) {
-  const float2 p = __half22float2(__hmax2(__habs2(*reinterpret_cast<const __half2*>(&w0)), __habs2(*reinterpret_cast<const __half2*>(&w1))));
-  return fmaxf(p.x, p.y * kLowestShare);
-}
-
 template <int N> struct Words { uint32_t w[N]; };
 template <int N> __device__ __forceinline__ Words<N> lds(const uint8_t* p) {
   Words<N> r;
@@ -282,6 +273,24 @@ template <int N> __device__ __forceinline__ Words<N> lds(const uint8_t* p) {
   else r.w[0] = *reinterpret_cast<const uint32_t*>(p);
   return r;
 }
+
+// The need that parameter words stand for: of a token's groups, or of tokens.
+template <typename T, int N> __device__ __forceinline__ float need_of(const Words<N>& p) {
+  if constexpr (std::is_same<T, __half>::value) {
+    __half2 most = *reinterpret_cast<const __half2*>(&p.w[0]);
+#pragma unroll
+    for (int g = 1; g < N; ++g) most = __hmax2(most, *reinterpret_cast<const __half2*>(&p.w[g]));
+    return fmaxf(__low2float(most), kLeastNeed<T>);
+  } else {
+    __nv_bfloat162 most = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p.w[0]));
+#pragma unroll
+    for (int g = 1; g < N; ++g) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p.w[g])));
+    const float2 m = param<T>(*reinterpret_cast<const uint32_t*>(&most));
+    return fmaxf(fmaxf(m.x, kLeastNeed<T>), m.y * kLowestShare);
+  }
+}
+// log2 of the smallest power of two that is not below a need.
+__device__ __forceinline__ float log2_above(float need) { return (float)((int)(__float_as_uint(need) + 0x7fffffu >> 23) - 127); }
 
 // A lane's operands of a row of q (lane 4 r + c: row r of eight), from its row's start plus 8 c channels, or of no row: q as f16, times the
 // power of two that brings the row's largest value to 2^14 - exact for all that matters to a score; channels 4 i + 1 and 4 i + 3 meet

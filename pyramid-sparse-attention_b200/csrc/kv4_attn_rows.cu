@@ -37,8 +37,7 @@ struct Shape {
   static constexpr int kQSum = kQ + kTiles * L::kBlocks * 512;                     // [kTiles][lanes] operands of its sums, 8 bytes
   static constexpr int kColumns = kQSum + kTiles * 256;                            // [row pairs] {factors to log2, keys that the rows see}
   static constexpr int kRise = kColumns + kRows * 8;                               // [slices][rows] scores that ask for a higher reference
-  static constexpr int kWide = kRise + kWarps * kRows * 4;                         // [warps] steps that do
-  static constexpr int kBars = kWide + kWarps * kHalves * 4;                       // full
+  static constexpr int kBars = kRise + kWarps * kRows * 4;                         // full
   static constexpr int kMore = kBars + kStages * 8;                                // scan[10], abort, valid[stages]
   static constexpr int kBytes = kMore + (11 + kStages) * 4;
   static constexpr int64_t kPart = (int64_t)kRows * (D + 2);                       // scratch: output rows, and {reference, sum} of each
@@ -67,7 +66,6 @@ struct Rows {
   float2 sum[NT];
   float2 mid[NT][D / G];        // the share of the output that the groups' middle values give
   float out[NT][2][4];          // of channels 4 i, 4 i + 2 (first) and 4 i + 1, 4 i + 3: times 2^-24 and 2^-20
-  float cap, limit;             // at least the largest step of the values so far, and the exponent from which a weight is too large
 };
 
 // Scores of a slice's 16 tokens and the warp's rows, from 8-row tile `tile0` on: rows of x are the tokens r/2 + 4 (r % 2) and that + 8.
@@ -179,66 +177,68 @@ __device__ __forceinline__ void weigh(Rows<T, D, G, NT>& s, const float (&e)[NT]
   }
 }
 
-// Scores and weights of the warp's 16 tokens of a tile; true, and scores times factors in e, where a weight times a step could leave f16 and
-// the references have to move first - which is seldom.
+// Scores (times factors, less references) to weights, and nothing for what a row does not see.
+template <bool MASKED, int NT>
+__device__ __forceinline__ void weights(float (&e)[NT][4], const float (&x)[NT][4], const float2 (&ref)[NT], const float4* columns, int token) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float4 w = columns[4 * nt];
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const float2 y = fma2(make_float2(x[nt][j], x[nt][j + 1]), make_float2(w.x, w.y), ref[nt]);
+      e[nt][j] = ex2(MASKED && token + 4 * j >= __float_as_int(w.z) ? -INFINITY : y.x);
+      e[nt][j + 1] = ex2(MASKED && token + 4 * j >= __float_as_int(w.w) ? -INFINITY : y.y);
+    }
+  }
+}
+
+// Scores and weights of the warp's 16 tokens of a tile; true, and scores in e, where a weight times a step could leave f16 and the references
+// have to move first - which is seldom.
 template <typename T, int D, int G, int NT, int HALVES, bool MASKED>
-__device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4], int tile0, uint8_t* smem, const uint8_t* slice, int token, int length,
-                                          uint32_t to) {
+__device__ __forceinline__ bool first_try(Rows<T, D, G, NT>& s, float (&e)[NT][4], int tile0, uint8_t* smem, const uint8_t* slice, int token, uint32_t to) {
   using L = Kv4<D, G>;
   using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = L::kGroups;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const float4* columns = reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c;   // of rows 2 c and 2 c + 1
   score<T, D, G, NT, HALVES>(e, tile0, smem, slice);
-  // the largest step of the values (or what stands for one): a lane looks at one group of its two rows
-  float widest, most = -INFINITY;
-  {
-    const uint8_t* p = slice + L::kHalf + L::kParams + (c < NG ? c : 0) * 4;
-    uint32_t w0 = lds<1>(p + r * NG * 4).w[0], w1 = lds<1>(p + (r + 8) * NG * 4).w[0];
-    if (MASKED) {   // what lies behind the last key may be anything
-      w0 = token < length ? w0 : 0u;
-      w1 = token + 8 < length ? w1 : 0u;
-    }
-    widest = wanted<T>(w0, w1);
-  }
-  float t[NT][4];   // to the references
+  // token by token, in the other kernel's words (the largest need kept: 3 new tokens of 5 x 20000 39 us instead of 38, groups of 32 43.6 instead of 41.2)
+  const uint8_t* p = slice + L::kHalf + L::kParams + r * NG * 4;
+  const float need[2] = {need_of<T, NG>(lds<NG>(p)), need_of<T, NG>(lds<NG>(p + 8 * NG * 4))};
+  float w[NT][4], top[2] = {0.f, 0.f};
+  weights<MASKED, NT>(w, e, s.ref, columns, token);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float4 w = columns[4 * nt];
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      const float2 y = fma2(make_float2(e[nt][j], e[nt][j + 1]), make_float2(w.x, w.y), s.ref[nt]);
-      t[nt][j] = MASKED && token + 4 * j >= __float_as_int(w.z) ? -INFINITY : y.x;
-      t[nt][j + 1] = MASKED && token + 4 * j >= __float_as_int(w.w) ? -INFINITY : y.y;
-      most = fmaxf(most, fmaxf(t[nt][j], t[nt][j + 1]));
-    }
-  }
-  const bool rises = __any_sync(~0u, widest > s.cap || most > s.limit);
+    for (int j = 0; j < 4; ++j) top[j >> 1] = fmaxf(top[j >> 1], w[nt][j]);
+  const bool rises = __any_sync(~0u, fmaxf(top[0] * need[0], top[1] * need[1]) > kMost);
   if (rises) {
+    float* rise = reinterpret_cast<float*>(smem + S::kRise) + warp % kWarps * S::kRows + 8 * tile0;
+    const float up[2] = {log2_above(need[0]), log2_above(need[1])};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float4 w = columns[4 * nt];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) e[nt][j] = MASKED && token + 8 * (j >> 1) >= __float_as_int(j & 1 ? w.w : w.z) ? -INFINITY : e[nt][j] * (j & 1 ? w.y : w.x);
-    }
-    float* rise = reinterpret_cast<float*>(smem + S::kRise) + warp % kWarps * S::kRows + 8 * tile0;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) widest = fmaxf(widest, __shfl_xor_sync(~0u, widest, d));
-    if (lane == 0) reinterpret_cast<float*>(smem + S::kWide)[warp] = widest;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      const float4 of = columns[4 * nt];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = fmaxf(e[nt][j], e[nt][2 + j]);
+        float m = -INFINITY, over = 0.f;
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-        if (r == 0) rise[8 * nt + 2 * c + j] = m;
+        for (int i = 0; i < 2; ++i) {
+          over = fmaxf(over, w[nt][2 * i + j] * need[i]);
+          if (!MASKED || token + 8 * i < __float_as_int(j ? of.w : of.z)) m = fmaxf(m, e[nt][2 * i + j] * (j ? of.y : of.x) + up[i]);
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) {
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+          over = fmaxf(over, __shfl_xor_sync(~0u, over, d));
+        }
+        if (r == 0) rise[8 * nt + 2 * c + j] = over > kMost ? m : -INFINITY;
       }
+    }
   } else {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[nt][j] = ex2(t[nt][j]);
+      for (int j = 0; j < 4; ++j) e[nt][j] = w[nt][j];
     weigh<T, D, G, NT, HALVES, MASKED>(s, e, true, columns, slice, token, to);
   }
   return rises;
@@ -251,15 +251,8 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
   using S = Shape<T, D, G, NT, HALVES>;
   constexpr int NG = D / G;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
+  const float4* columns = reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c;
   float* rise = reinterpret_cast<float*>(smem + S::kRise) + 8 * tile0;
-  float* wide = reinterpret_cast<float*>(smem + S::kWide);
-  float widest = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps * HALVES; ++w) widest = fmaxf(widest, wide[w]);
-  const float old = log2f(s.cap);
-  s.cap = power_above(s.cap, widest);
-  const float up = log2f(s.cap);
-  s.limit = kHead + kLazy - up;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -267,9 +260,8 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
       float m = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, rise[w * S::kRows + 8 * nt + 2 * c + j]);
-      // largest score so far, or what the reference stood for
       float& was = j ? s.ref[nt].y : s.ref[nt].x;
-      const float ref = fmaxf(m, kHead - was - old) + (up - kHead), fade = half_of(-was - ref);
+      const float ref = fmaxf(m - kHead, -was), fade = half_of(-was - ref);
       was = -ref;
       float& sum = j ? s.sum[nt].y : s.sum[nt].x;
       sum = faded(sum, fade);
@@ -283,15 +275,16 @@ __device__ __forceinline__ void raise(Rows<T, D, G, NT>& s, float (&e)[NT][4], b
         s.out[nt][h][j] = faded(s.out[nt][h][j], fade);
         s.out[nt][h][2 + j] = faded(s.out[nt][h][2 + j], fade);
       }
-      e[nt][j] = rises ? ex2(e[nt][j] - ref) : faded(e[nt][j], fade);
-      e[nt][2 + j] = rises ? ex2(e[nt][2 + j] - ref) : faded(e[nt][2 + j], fade);
+      if (!rises) {
+        e[nt][j] = faded(e[nt][j], fade);
+        e[nt][2 + j] = faded(e[nt][2 + j], fade);
+      }
     }
-  weigh<T, D, G, NT, HALVES, true>(s, e, rises, reinterpret_cast<const float4*>(smem + S::kColumns) + 4 * tile0 + c, slice, token, to);
+  if (rises) weights<true, NT>(e, e, s.ref, columns, token);
+  weigh<T, D, G, NT, HALVES, true>(s, e, rises, columns, slice, token, to);
   __syncthreads();
-  if (rises) {   // nothing asked for any more
+  if (rises)   // nothing asked for any more
     for (int i = lane; i < 8 * NT; i += 32) rise[warp % kWarps * S::kRows + i] = -INFINITY;
-    if (lane == 0) wide[warp] = 0.f;
-  }
 }
 
 // Outputs of the warp's 32 channels and rows from its slices of a tile: tokens c + 4 i, i = 0..3, in pairs (c, c + 4) and (c + 8, c + 12).
@@ -355,8 +348,7 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
     tc::fence_mbar_init();
     *abort_flag = 0;
   }
-  for (int i = threadIdx.x; i < kWarps * kRows + kWarps * kHalves; i += kThreads)
-    reinterpret_cast<float*>(smem + S::kRise)[i] = i < kWarps * kRows ? -INFINITY : 0.f;
+  for (int i = threadIdx.x; i < kWarps * kRows; i += kThreads) reinterpret_cast<float*>(smem + S::kRise)[i] = -INFINITY;
   asm volatile("griddepcontrol.launch_dependents;");
   int request, base;
   Shares shares(0, 0, 1);
@@ -438,8 +430,6 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
 #pragma unroll
       for (int j = 0; j < 8; ++j) s.out[nt][j / 4][j % 4] = 0.f;
     }
-    s.cap = kLeastCap;
-    s.limit = kHead + kLazy - kLeastCapLog2;
     __syncthreads();
     const int all_see = p.length - p.count + p.row0 / group + 1;   // keys that every row of the unit sees
     const uint32_t area_at = tc::smem_u32(area);
@@ -453,8 +443,8 @@ __global__ void __launch_bounds__(32 * kWarps * HALVES, blocks_of(8 * NT * HALVE
       const uint32_t weights = area_at + (S::kBuffers == 2 && (i & 1) ? S::kWeights : 0) + tile0 * 256, to = weights + own * (S::kTiles * 256);
       float e[NT][4];
       if (S::kBuffers == 1 && i) __syncthreads();                          // the weights before have been used
-      const bool rises = there && t0 + 16 <= all_see ? first_try<T, D, G, NT, HALVES, false>(s, e, tile0, smem, slice, token, p.length, to)
-                                                     : first_try<T, D, G, NT, HALVES, true>(s, e, tile0, smem, slice, token, p.length, to);
+      const bool rises = there && t0 + 16 <= all_see ? first_try<T, D, G, NT, HALVES, false>(s, e, tile0, smem, slice, token, to)
+                                                     : first_try<T, D, G, NT, HALVES, true>(s, e, tile0, smem, slice, token, to);
       const bool move = __syncthreads_or(rises);
       if (warp == 0 && behind && !dead) copy_next(stage ? stage - 1 : kStages - 1);
       behind = true;

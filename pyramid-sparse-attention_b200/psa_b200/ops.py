@@ -1147,7 +1147,8 @@ def kv4_attention(q: torch.Tensor, data: torch.Tensor, table: torch.Tensor, leng
     query rows are a request's own (None: all of them).  Row i < counts[b] stands at lengths[b] - counts[b] + i and sees the keys up
     to its own place; rows that see nothing, and rows behind counts[b], are 0.  What lies behind a length is not read into the result.
     Returns [B, H, n, D] in q's order of dimensions, with return_lse also the logarithms of the sums, float32 [B, H, n] (-inf for a
-    row of nothing).  Values of a size from 1e-23 to 1e31 keep full precision.  No gradient."""
+    row of nothing).  Values of a size from 1e-23 to 1e31 keep full precision (of a token's groups, those whose steps are not below
+    2^-20 of its largest); no bit of a row depends on keys and values that it does not see.  No gradient."""
     sm_scale = sm_scale if sm_scale is None else float(sm_scale)
     done = _calls.attend(q, data, table, lengths, group, counts, sm_scale, bool(return_lse))
     if done is not None:

@@ -402,3 +402,46 @@ def test_numbers_beyond_32_bits_are_out_of_range(ops):
     q = randn(g, 1, 2, 2, 64, dtype=torch.bfloat16)
     assert not bool(ops.kv4_attention(q, data, table, lengths, 32, torch.tensor([-far + 2], device=DEV)).any())
     reported()
+
+
+@pytest.mark.parametrize("H,n", [(3, 2), (6, 2), (7, 3), (8, 4), (14, 3)])
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, 1e9), (torch.bfloat16, 1e30), (torch.float16, 6e4)], **names)
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32)])
+def test_attention_rows_do_not_feel_what_they_do_not_see(ops, dtype, value, D, group, H, n):
+    """Large values of later tokens of the same call, random or constant: the rows before them keep every bit."""
+    g = gen(81)
+    lengths = [300, 64, 17]
+    c = Filled(ops, g, lengths, 1, D, group, dtype, 16)
+    c.v *= 2.0 ** -10
+    ops.kv4_append(c.data, c.k, c.v, c.slots, group)
+    q = randn(g, 3, H, n, D, dtype=dtype)
+    clean = check_attention(ops, q, c)
+    for big in (value * torch.rand(3, 1, 1, D, generator=g, device=DEV), torch.full((3, 1, 1, D), value, device=DEV)):
+        v = c.v.clone()
+        for b, length in enumerate(lengths):
+            v[b, :, length - 1] = big[b, :, 0].to(dtype)
+        keep, c.v = c.v, v
+        ops.kv4_append(c.data, c.k, c.v, c.slots, group)
+        got = check_attention(ops, q, c)
+        c.v = keep
+        assert torch.equal(got[:, :, :n - 1], clean[:, :, :n - 1])
+
+
+@pytest.mark.parametrize("H,n", ROWS)
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, 1e10), (torch.bfloat16, 1e30), (torch.float16, 6e4)], **names)
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 64)])
+def test_attention_of_large_values_without_weight(ops, dtype, value, D, group, H, n):
+    """Keys that point away from every query, with values far beyond the others': what they are worth is what their weight times their value
+    is, and the others' codes keep their bits."""
+    g = gen(82)
+    c = Filled(ops, g, [900, 2000], 1, D, group, dtype, 64, k_scale=0.2)
+    u = torch.sign(randn(g, D))
+    q = (u + 0.3 * randn(g, 2, H, n, D)).to(dtype)
+    away = torch.rand(2, 1, 2000, 1, generator=g, device=DEV) < 0.03
+    away[:, :, -n:] = False
+    c.v *= 2.0 ** -10
+    size = {1e10: 20.0, 1e30: 40.0, 6e4: 20.0}[value] * 8 / D ** 0.5          # scores of some -8 size: 2^-230 and 2^-460
+    c.k = torch.where(away, (-size * u).to(dtype), c.k)
+    c.v = torch.where(away, (value * torch.rand(c.v.shape, generator=g, device=DEV)).to(dtype), c.v)
+    ops.kv4_append(c.data, c.k, c.v, c.slots, group)
+    check_attention(ops, q, c)
