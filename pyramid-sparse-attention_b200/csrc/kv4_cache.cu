@@ -27,14 +27,30 @@ struct CacheArgs {
 };
 
 // A quotient of which only the rounded value counts, as a product with the inverse.  The inverse is off by 2^-24 of itself at most, the
-// product by less than 2^-20; the sum with 24 rounds that to steps of 2^-19 or 2^-18, so that a tie is one again, and the sum with
-// 1.5 * 2^23 rounds to whole numbers, ties to even.  (What lies within 2^-19 of a tie counts as one; value - lowest in 32 bits is
-// off by 2^-21 already.)  With a division for each value their special function units bound the kernel: 77 us for what takes 24.
-constexpr float kTies = 24.f, kRound = 12582912.f;
+// product at a tie by less than 2^-20; the sum with 16 rounds that to steps of 2^-19, so that a tie is one again, and the sum with 1.5 * 2^23 rounds
+// to whole numbers, ties to even.  With a division for each value their special function units bound the kernel: 77 us for what takes 24.
+//
+// What lies within 2.9 * 2^-20 of a tie (half of 2^-19, the product, the difference) and is none would count as one.  Value, lowest and tie are whole
+// numbers of units in the last place of value, lowest and half a step: to be that near and not the same, the value or the lowest must be
+// below kTiny steps in size - 2^8 (f16: 2^11) such units are more than it - and not zero; and if it is the value, then -lowest / step is as near to a tie
+// as that.  Groups of which this holds (a thousandth of all, f16: a hundredth) look for such values and round them exactly: 32761
+// tokens of 4 heads x 128: bf16 23.1 us, f16 23.7; 22.6 without, 25.1-25.9 with a remainder for every value.
+constexpr float kTies = 16.f, kRound = 12582912.f;
 // Steps for which that holds, and which the type cuts off by less than 1/30 of themselves: 15 is the largest code by itself.
 template <typename T> constexpr float kLeastStep = 8.673617379884035e-19f;   // 2^-60
 template <> constexpr float kLeastStep<__half> = 6.103515625e-05f;           // 2^-14
 constexpr float kMostStep = 1.152921504606847e18f;                           // 2^60
+template <typename T> constexpr float kTiny = 7.2e-4f;                       // 2.95 * 2^-12
+template <> constexpr float kTiny<__half> = 5.77e-3f;                        // 2.95 * 2^-9
+
+// The code of a value: (x - lowest) / step rounded, ties to even, in 64 bits from the sign of x - lowest - (n + 1/2) step.
+__device__ __forceinline__ uint32_t exact_code(float x, float lowest, float step) {
+  const double d = (double)x - lowest;
+  const float n = fminf(floorf((float)d / step), 14.f);
+  const double rest = fma(-(double)(n + 0.5f), (double)step, d);
+  const uint32_t code = (uint32_t)n;
+  return code + (rest > 0. || (rest == 0. && (code & 1)));
+}
 
 // Largest number of the type that is not above x >= 0 (a NaN stays one).
 __device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
@@ -54,6 +70,30 @@ template <> struct Pair<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat162 make(__nv_bfloat16 a, __nv_bfloat16 b) { return __halves2bfloat162(a, b); }
   static __device__ __forceinline__ __nv_bfloat162 base() { return __float2bfloat162_rn(128.f); }
 };
+
+// Whether a thread's eight channels of a row need more than the product with the inverse: a step that is none, or nearly none, or far beyond any that
+// counts; a lowest value or a value near zero.
+template <typename T>
+__device__ __forceinline__ bool needs_more(const uint4& w, float s, float lo) {
+  using T2 = typename Pair<T>::type;
+  const T2* e = reinterpret_cast<const T2*>(&w);
+  const T2 least = __hmin2(__hmin2(__habs2(e[0]), __habs2(e[1])), __hmin2(__habs2(e[2]), __habs2(e[3])));
+  return !(s >= kLeastStep<T> && s < kMostStep) || fminf(fabsf(lo), Elem<T>::to_f(__hmin(least.x, least.y))) < s * kTiny<T>;
+}
+// Exact codes of a thread's eight channels of a row.
+template <typename T>
+__device__ __forceinline__ uint32_t exact_codes(uint4 w, float s, float lo) {
+  using T2 = typename Pair<T>::type;
+  uint32_t codes = 0;
+  if (!(s > 0.f)) return codes;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {   // two channels a round: their registers are the kernel's
+    const T2 x = *reinterpret_cast<const T2*>(&w.x);
+    codes = codes >> 8 | exact_code(Elem<T>::to_f(x.x), lo, s) << 24 | exact_code(Elem<T>::to_f(x.y), lo, s) << 28;
+    w = make_uint4(w.y, w.z, w.w, 0u);
+  }
+  return codes;
+}
 
 constexpr int kRows = 4;   // rows that a thread takes, their loads in flight together
 
@@ -138,7 +178,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const CacheArgs a) {
   // Every lane of a group knows them by now: of four neighbours each does one row's divisions.
   const int lane = threadIdx.x & 31, own = lane & 3;
   uint32_t pair;
-  float inverse;   // 0: not for the product with it
+  float inverse;   // 0: not for the product with it; negative: values near zero may lie near a tie
   {
     const uint32_t x = own & 2 ? (own & 1 ? ends[3] : ends[2]) : (own & 1 ? ends[1] : ends[0]);
     const bool skip = !(own & 2 ? (own & 1 ? to.good(3) : to.good(2)) : (own & 1 ? to.good(1) : to.good(0)));
@@ -149,16 +189,18 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const CacheArgs a) {
     const float s = Elem<T>::to_f(step);
     if (!isfinite(wide)) step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));   // an infinity or a NaN among them, or a range beyond 32 bits
     inverse = skip ? 1.f : s >= kLeastStep<T> && s < kMostStep && isfinite(wide) ? __frcp_rn(s) : 0.f;
+    const float at = fmaf(-Elem<T>::to_f(lowest), inverse, 0.5f), l = fabsf(Elem<T>::to_f(lowest));   // of zero, ties as whole numbers
+    if (!skip && (fabsf(at - rintf(at)) < 1.02f * kTiny<T> || l < s * kTiny<T>)) inverse = -inverse;
     const T2 both = Pair<T>::make(step, lowest);
     pair = *reinterpret_cast<const uint32_t*>(&both);
   }
   uint32_t pairs[kRows], codes[kRows];
-  bool plain = true;
+  uint32_t look = 0;   // rows with values that may need more than the product: a bit each
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
     pairs[j] = __shfl_sync(~0u, pair, (lane & ~3) | j);
     const float inv = __shfl_sync(~0u, inverse, (lane & ~3) | j);
-    plain = plain && inv != 0.f;
+    look |= inv > 0.f ? 0u : 1u << j;
     const T2* e = reinterpret_cast<const T2*>(&w[j]);
     const float lo = Elem<T>::to_f(reinterpret_cast<const T2*>(&pairs[j])->y);
     // a rounded quotient's bits are those of 1.5 * 2^23 plus the code: their sum with weights 16^i, less what the constant makes
@@ -166,20 +208,16 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const CacheArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = Elem<T>::to_f(i & 1 ? e[i / 2].y : e[i / 2].x) - lo;
-      codes[j] += __float_as_uint(fmaf(x, inv, kTies) + (kRound - kTies)) << (4 * i);
+      codes[j] += __float_as_uint(fmaf(x, fabsf(inv), kTies) + (kRound - kTies)) << (4 * i);
     }
   }
-  if (!plain) {   // some group's step is none, or nearly none, or far beyond any that counts
+  if (look) {
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
+      if (!(look >> j & 1)) continue;
       const T2 p = *reinterpret_cast<const T2*>(&pairs[j]);
-      const T* e = reinterpret_cast<const T*>(&w[j]);
-      const float s = Elem<T>::to_f(p.x), lo = Elem<T>::to_f(p.y);
-      codes[j] = 0;
-      if (s > 0.f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) codes[j] |= (__float_as_uint(fminf((Elem<T>::to_f(e[i]) - lo) / s, 15.f) + kRound) & 15u) << (4 * i);
-      }
+      const float step = Elem<T>::to_f(p.x), lo = Elem<T>::to_f(p.y);
+      if (needs_more<T>(w[j], step, lo)) codes[j] = exact_codes<T>(w[j], step, lo);
     }
   }
   const int g = to.u * 8 / G;

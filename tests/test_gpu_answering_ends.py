@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_answering import (DEV, HALF, SIZES, TINY, TYPES, Filled, angles, attention, check_attention, gen, names, near_turned, ops, randn,  # noqa: F401
+from test_gpu_answering import (DEV, HALF, SIZES, TINY, TYPES, Filled, angles, attention, check_attention, gen, names, near_turned, ops, randn, scales,  # noqa: F401
                                 stands_for)
 
 pytestmark = pytest.mark.gpu
@@ -445,3 +445,62 @@ def test_attention_of_large_values_without_weight(ops, dtype, value, D, group, H
     c.v = torch.where(away, (value * torch.rand(c.v.shape, generator=g, device=DEV)).to(dtype), c.v)
     ops.kv4_append(c.data, c.k, c.v, c.slots, group)
     check_attention(ops, q, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+@pytest.mark.parametrize("D,group", SIZES)
+def test_cache_rounds_next_to_a_tie(ops, dtype, D, group):
+    """Values and lowest values so near zero that the rest of a quotient lies next to a tie and is none: the nearer of the 16 values, where
+    they meet exactly the even one."""
+    tiny = [0.0, 2.0 ** -9, -2.0 ** -9, 2.0 ** -14, -2.0 ** -14, 2.0 ** -17, -2.0 ** -17, 2.0 ** -20, -2.0 ** -20, 2.0 ** -24, -2.0 ** -24]
+    if dtype == torch.bfloat16:
+        tiny += [2.0 ** -30, -2.0 ** -30]
+    rows, codes = [], []
+    for step in (1.0, 0.5, 3.0):
+        for k in range(15):
+            for x in tiny:                                      # (x - lowest) / step = k + 1/2 + x / step
+                row = torch.full((group,), 7 * step)
+                lowest = -(k + 0.5) * step
+                row[0], row[1], row[2:] = lowest, lowest + 15 * step, x
+                if bool((row.to(dtype).float() == row).all()):
+                    rows.append(row)
+                    codes.append(k + (1 if x > 0 or (x == 0 and k % 2) else 0))
+            for low in tiny:                                    # lowest near zero, values at ties: (k + 1/2) step - lowest
+                row = torch.full((group,), (k + 0.5) * step)
+                row[0], row[1] = low, 15 * step
+                if bool((row.to(dtype).float() == row).all()) and low < step / 2:
+                    wide = (torch.tensor(15 * step, dtype=torch.float64) - low) / 15
+                    if wide >= step and float(wide - step) < step * torch.finfo(dtype).eps / 2:          # cut off to the type: the step itself
+                        rows.append(row)
+                        codes.append(k + (1 if low < 0 or (low == 0 and k % 2) else 0))
+    assert len(rows) > 300
+    n, per = len(rows), D // group
+    x = torch.stack(rows).to(dtype).to(DEV).repeat(1, per)[None, None]
+    want = torch.tensor(codes, device=DEV)[:, None].expand(n, group).clone()
+    data = ops.kv4_empty((n + 15) // 16, 1, 16, D, group, DEV)
+    slots = torch.arange(n, device=DEV)[None]
+    ops.kv4_append(data, x, x, slots, group)
+    step, low, _ = scales(x, group)
+    for y in ops.kv4_read(data, slots, D, group, dtype):
+        z = y.double().unflatten(-1, (-1, group))
+        got = torch.round((z - low) / step)[0, 0]                # the value it stands for is off by a rounding, far less than half a step
+        for g in range(per):
+            assert torch.equal(got[:, g, 2:].long(), want[:, 2:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+@pytest.mark.parametrize("D,group", SIZES)
+def test_cache_codes_of_values_of_many_sizes(ops, dtype, D, group):
+    """Random values of sizes from 1 to 2^-20, whole numbers of a step among them, against quotients in 64 bits."""
+    g = gen(83)
+    n = 20000
+    x = randn(g, 1, 2, n, D) * 2.0 ** -torch.randint(0, 21, (1, 2, n, D), generator=g, device=DEV)
+    grid = torch.rand(1, 2, n, 1, generator=g, device=DEV) < 0.5
+    x = torch.where(grid & (torch.rand(x.shape, generator=g, device=DEV) < 0.8), torch.round(x * 8) / 4, x).to(dtype)
+    data = ops.kv4_empty(n // 16, 2, 16, D, group, DEV)
+    slots = torch.randperm(n, generator=g, device=DEV)[None]
+    ops.kv4_append(data, x, x.flip(-1), slots, group)
+    for v, y in zip((x, x.flip(-1)), ops.kv4_read(data, slots, D, group, dtype)):
+        want = stands_for(v, group)
+        assert bool(((y.double() - want).abs() <= HALF[dtype] * 1.001 * want.abs() + TINY[dtype]).all())
+    ops.check_status()
