@@ -6,7 +6,7 @@
 // misses by 15 units of its last place at most, an eighth of a step in bf16).  A group that holds an infinity or a NaN, or
 // whose range does not fit 32 bits, reads as NaN.
 //
-// The floor is HBM, 86 MB and 13.1 us each way for 32761 tokens of 4 heads x 128.  Reading takes 15.1 us.  Appending takes 23.1, bound by
+// The floor is HBM, 86 MB and 13.1 us each way for 32761 tokens of 4 heads x 128.  Reading takes 15.3 us.  Appending takes 23.1 (f16 24.1), bound by
 // instructions (some 560 a thread for 32 values; 72 % of the issue slots): unpacking, two sums and a product a value, the extrema.
 // (Divisions by page sizes and numbers of tokens that need none cost 1.5 us each way.)
 #include "kv4.cuh"
@@ -34,7 +34,7 @@ struct CacheArgs {
 // numbers of units in the last place of value, lowest and half a step: to be that near and not the same, the value or the lowest must be
 // below kTiny steps in size - 2^8 (f16: 2^11) such units are more than it - and not zero; and if it is the value, then -lowest / step is as near to a tie
 // as that.  Groups of which this holds (a thousandth of all, f16: a hundredth) look for such values and round them exactly: 32761
-// tokens of 4 heads x 128: bf16 23.1 us, f16 23.7; 22.6 without, 25.1-25.9 with a remainder for every value.
+// tokens of 4 heads x 128: bf16 23.1 us, f16 24.1; 22.6 without, 25.1-25.9 with a remainder for every value.
 constexpr float kTies = 16.f, kRound = 12582912.f;
 // Steps for which that holds, and which the type cuts off by less than 1/30 of themselves: 15 is the largest code by itself.
 template <typename T> constexpr float kLeastStep = 8.673617379884035e-19f;   // 2^-60
@@ -55,6 +55,9 @@ __device__ __forceinline__ uint32_t exact_code(float x, float lowest, float step
 // Largest number of the type that is not above x >= 0 (a NaN stays one).
 __device__ __forceinline__ __half cut_off(float x, __half) { return __float2half_rz(x); }
 __device__ __forceinline__ __nv_bfloat16 cut_off(float x, __nv_bfloat16) { return __float2bfloat16_rz(x); }
+// The next smaller number of a positive one.
+__device__ __forceinline__ __half below(__half x) { return __ushort_as_half(__half_as_ushort(x) - 1); }
+__device__ __forceinline__ __nv_bfloat16 below(__nv_bfloat16 x) { return __ushort_as_bfloat16(__bfloat16_as_ushort(x) - 1); }
 
 // Two numbers of the type in a word, and the number from which whole numbers up to 15 on are neighbours in it.
 template <typename T> struct Pair;
@@ -184,9 +187,14 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const CacheArgs a) {
     const bool skip = !(own & 2 ? (own & 1 ? to.good(3) : to.good(2)) : (own & 1 ? to.good(1) : to.good(0)));
     const T2 low = *reinterpret_cast<const T2*>(&x);
     T lowest = low.x;
-    const float wide = (-Elem<T>::to_f(low.y) - Elem<T>::to_f(lowest)) / 15.f;
+    const float highest = -Elem<T>::to_f(low.y), wide = (highest - Elem<T>::to_f(lowest)) / 15.f;
     T step = cut_off(wide, T());
-    const float s = Elem<T>::to_f(step);
+    float s = Elem<T>::to_f(step);
+    // the difference, or the quotient, was rounded up to a number of the type (the sum with the larger of the two loses nothing near zero)
+    if (fmaf(-15.f, s, fmaxf(highest, -Elem<T>::to_f(lowest))) < -fminf(highest, -Elem<T>::to_f(lowest))) {
+      step = below(step);
+      s = Elem<T>::to_f(step);
+    }
     if (!isfinite(wide)) step = lowest = Elem<T>::from_f(__int_as_float(0x7fffffff));   // an infinity or a NaN among them, or a range beyond 32 bits
     inverse = skip ? 1.f : s >= kLeastStep<T> && s < kMostStep && isfinite(wide) ? __frcp_rn(s) : 0.f;
     const float at = fmaf(-Elem<T>::to_f(lowest), inverse, 0.5f), l = fabsf(Elem<T>::to_f(lowest));   // of zero, ties as whole numbers

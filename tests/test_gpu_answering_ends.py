@@ -504,3 +504,33 @@ def test_cache_codes_of_values_of_many_sizes(ops, dtype, D, group):
         want = stands_for(v, group)
         assert bool(((y.double() - want).abs() <= HALF[dtype] * 1.001 * want.abs() + TINY[dtype]).all())
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES, **names)
+@pytest.mark.parametrize("D,group", SIZES)
+def test_cache_steps_are_cut_off_exactly(ops, dtype, D, group):
+    """A highest value that is 15 numbers of the type, and a lowest so little above zero that 32 bits do not see the difference: the step is the next
+    smaller number, and lowest + 15 steps is not above the highest."""
+    eps = torch.finfo(dtype).eps
+    rows = []
+    for step in (1.0, 3.0, 0.375, 1 + 8 * eps):
+        for low in (0.0, 2.0 ** -24, 2.0 ** -23, -2.0 ** -24, 2.0 ** -14, -2.0 ** -14):
+            row = torch.linspace(0, 15, group) * step
+            row[0], row[1] = low, 15 * step
+            row[2:] = row[2:].clamp(min=step / 4)
+            if bool((row[:2].to(dtype).float() == row[:2]).all()):
+                rows += [row, -row]
+    if dtype == torch.float16:      # the sum of highest and 15 steps does not fit 24 bits
+        for high, low in ((1023 * 2.0 ** -24, -1.0244140625), (2047 * 2.0 ** -24, -1.19921875)):
+            row = torch.linspace(low, high, group)
+            rows += [row, -row]
+    x = torch.stack(rows).to(dtype).to(DEV).repeat(1, D // group)[None, None]
+    n = x.shape[2]
+    data = ops.kv4_empty((n + 15) // 16, 1, 16, D, group, DEV)
+    slots = torch.arange(n, device=DEV)[None]
+    ops.kv4_append(data, x, x, slots, group)
+    want = stands_for(x, group)
+    for y in ops.kv4_read(data, slots, D, group, dtype):
+        assert bool(((y.double() - want).abs() <= HALF[dtype] * 1.001 * want.abs() + TINY[dtype]).all())
+    step, low, _ = scales(x, group)
+    assert bool((low + 15 * step <= x.double().unflatten(-1, (-1, group)).amax(-1, keepdim=True)).all())
