@@ -22,8 +22,8 @@
 //
 // The floor is the cache's bytes (160 a token and key head at head_dim 128, groups of 32).  mma.sync and not tcgen05: 8 query rows
 // against 128 rows of a tcgen05 tile, and operands that are made in registers; the products take a fifth of a warp's issue slots.  8 requests
-// of 131071 tokens, 28 heads on 4, bf16: 135-137 us (4.9-5.0 TB/s; 103 us at copy speed).  The copies alone take 104: what bounds it is issue
-// slots, 340 instructions a slice - 88 take the codes apart, 17 are products - at two thirds of a slot a cycle.  Waiting for tiles one by
+// of 131071 tokens, 28 heads on 4, bf16: 133-140 us (4.8-5.0 TB/s; 103 us at copy speed).  The copies alone take 104: what bounds it is issue
+// slots, 335 instructions a slice - 88 take the codes apart, 17 are products - at two thirds of a slot a cycle.  Waiting for tiles one by
 // one cost 30 instructions more (149 us), a ring of its own for every warp 170 us, outputs split by channels as in kv4_attn_rows.cu 164.
 #include "kv4_attn.cuh"
 

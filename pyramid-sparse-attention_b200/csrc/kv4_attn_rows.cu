@@ -7,12 +7,12 @@
 // 12 with 32; for 48 rows eight warps take half of them each.  All references of a row are one for the block, and move together.  The first
 // warp copies tiles ahead: when the block meets between a tile's scores and outputs, the tile before it is done with.
 //
-// 5 requests of 20000 tokens, 28 heads on 4, head_dim 128, groups of 64, bf16: 3 new tokens 38 us (as 32 rows 45, as two units of 16 in the other
-// kernel 53), 4 new ones 44 (eight warps with 16 rows each 50), 6 new ones 57 (as two units of 24 59; units of 16 in the other kernel 78;
-// four warps with 48 rows each 78: 168 registers, 8 warps on an SM, 36 % of the issue slots).  6 at 80000 tokens: 496 instructions for 24
-// rows and 16 tokens, half of the issue slots, tensor pipe 42 % (one m16n8k16 every 8 cycles: 576 TFLOP/s is what mma.sync has).  For 16
-// rows the other kernel is as good (32 us, 33 here).  Pieces of a prompt, 48 rows a unit: 64 new tokens of one request of 32768 187 us, 256 of
-// them 641 (190 TFLOP/s of the pairs that are seen), 2048 of 2048 462: each unit decodes the cache again, and goes through all of the
+// 5 requests of 20000 tokens, 28 heads on 4, head_dim 128, groups of 64, bf16: 3 new tokens 37-38 us (as 32 rows 45, as two units of 16 in the other
+// kernel 53), 4 new ones 44 (eight warps with 16 rows each 50), 6 new ones 59 (as two units of 24 59; units of 16 in the other kernel 78;
+// four warps with 48 rows each 78: 168 registers, 8 warps on an SM, 36 % of the issue slots).  6 at 80000 tokens: 506 instructions for 24
+// rows and 16 tokens, half of the issue slots, tensor pipe 41 % (one m16n8k16 every 8 cycles: 576 TFLOP/s is what mma.sync has).  For 16
+// rows the other kernel is as good (32 us, 33 here).  Pieces of a prompt, 48 rows a unit: 64 new tokens of one request of 32768 189 us, 256 of
+// them 661 (181 TFLOP/s of the pairs that are seen), 2048 of 2048 458: each unit decodes the cache again, and goes through all of the
 // request's tiles whatever its rows see.
 #include "kv4_attn.cuh"
 

@@ -7,7 +7,7 @@
 // whose range does not fit 32 bits, reads as NaN.
 //
 // The floor is HBM, 86 MB and 13.1 us each way for 32761 tokens of 4 heads x 128.  Reading takes 15.3 us.  Appending takes 23.1 (f16 24.1), bound by
-// instructions (some 560 a thread for 32 values; 72 % of the issue slots): unpacking, two sums and a product a value, the extrema.
+// instructions (some 590 a thread for 32 values; 74 % of the issue slots): unpacking, two sums and a product a value, the extrema.
 // (Divisions by page sizes and numbers of tokens that need none cost 1.5 us each way.)
 #include "kv4.cuh"
 
