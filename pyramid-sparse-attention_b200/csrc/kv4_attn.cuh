@@ -48,7 +48,7 @@ constexpr float kLowest = -3.4028234664e38f;   // reference of a row that has se
 // largest is still rounded to 11 bits.  A row looks at its own tokens alone: what it does not see, and what other rows see, changes no
 // bit of it.
 // Weights are up to 2^95 (f16 tensors: 2^63), 2^31 of them fit 32 bits, and so do as many of up to 2^79 times a lowest value.  Steps may be up to
-// 2^100 (below 2^-126 weights are 0).
+// 2^100 (below 2^-126 weights are 0).  Where zeros have nearly all the weight, what is left of an output below 2^-80 of its values' size loses bits.
 constexpr float kHead = 7.f, kMostLog2 = 15.f, kMost = 32768.f, kLowestShare = 5.421010862427522e-20f;
 // f16: 2^-64 of the largest number; a step is 2^-24 or more.
 template <typename T> constexpr float kLeastNeed = std::is_same<T, __half>::value ? 3.552713678800501e-15f : 8.271806125530277e-25f;   // 2^-48, 2^-80

@@ -120,7 +120,6 @@ def test_native_calls_of_other_versions_are_not_loaded(monkeypatch, tmp_path):
     here = os.path.dirname(_lib.__file__)
     now = calls_name()
     assert torch.__version__ in now and os.path.exists(os.path.join(here, now)) and _lib._calls is not _lib.NoCalls
-    assert [f for f in os.listdir(here) if f.startswith("_calls") and f.endswith(".so")] == [now]
     monkeypatch.setattr(torch, "__version__", "9.9.9")
     assert calls_name() != now
     with pytest.warns(RuntimeWarning, match="is not there"):
