@@ -959,8 +959,19 @@ class _RotateAxes(torch.autograd.Function):
         wanted = [g is not None and need for g, need in zip(grads, ctx.needs_input_grad[4:])]
         if not any(wanted):
             return (None,) * (4 + len(grads))
-        back = iter(_RotateAxes.apply(ctx.saved_tensors[0], plan, half, not inverse, *[g for g, w in zip(grads, wanted) if w]))
+        back = iter(_turned(ctx.saved_tensors[0], plan, half, not inverse, [g for g, w in zip(grads, wanted) if w]))
         return (None,) * 4 + tuple(next(back) if w else None for w in wanted)
+
+
+def _has_tangent(x: torch.Tensor) -> bool:
+    return forward_ad.unpack_dual(x).tangent is not None
+
+
+def _turned(positions, plan, half: bool, inverse: bool, xs):
+    """_RotateAxes of xs; one by one in forward mode, where an operand may have no tangent."""
+    if any(_has_tangent(x) for x in xs):
+        return [_RotateAxes.apply(positions, plan, half, inverse, x)[0] for x in xs]
+    return _RotateAxes.apply(positions, plan, half, inverse, *xs)
 
 
 def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, sections: Sequence[int], theta: float = 10000.0,
@@ -987,10 +998,8 @@ def rotate_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
         raise ValueError(f"rotate_axes: layout must be 'half' or 'pairs', got {layout!r}")
     if positions.dim() not in (2, 3) or positions.size(0) != len(sections):
         raise ValueError(f"rotate_axes: positions of shape {tuple(positions.shape)} are not [{len(sections)}, {q.size(0)}, {q.size(2)}]")
-    if any(forward_ad.unpack_dual(x).tangent is not None for x in xs):       # one by one: an operand may have none
-        outs = [_RotateAxes.apply(positions, plan, half, False, x)[0] for x in xs]
-    elif torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        outs = _RotateAxes.apply(positions, plan, half, False, *xs)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs) or any(_has_tangent(x) for x in xs):
+        outs = _turned(positions, plan, half, False, xs)
     else:
         outs = _rotate(xs, positions, plan, half, False)
     return outs[0] if k is None else tuple(outs)

@@ -142,3 +142,28 @@ def test_numbers_of_64_bits_keep_their_side_of_the_range():
     assert got.dtype == torch.int32 and got.tolist() == [5, -1] + [2 ** 31 - 1, -2 ** 31] * 2 + [2 ** 31 - 1]
     strided = torch.arange(8, dtype=torch.int32)[::2]
     assert ops._ints32("counts", strided, (4,)).is_contiguous() and ops._ints32("counts", strided, (4,)).tolist() == [0, 2, 4, 6]
+
+
+def test_derivatives_of_derivatives_in_either_mode(monkeypatch):
+    """Around a stand-in for the kernel (twice its operand, and half of it on the way back): tangents of operands and of the gradients that come
+    in, of one operand and not of the other."""
+    import torch
+    from torch.autograd import forward_ad
+
+    from psa_b200 import ops
+    monkeypatch.setattr(ops, "_rotate", lambda xs, positions, plan, half, inverse: tuple((0.5 if inverse else 2.0) * x for x in xs))
+    q, k, pos = torch.randn(1, 2, 3, 16), torch.randn(1, 1, 3, 16), torch.zeros(1, 3, dtype=torch.int64)
+    tq, tk, gq, gk = torch.randn_like(q), torch.randn_like(k), torch.randn_like(q), torch.randn_like(k)
+    with forward_ad.dual_level():
+        for of_q, of_k in ((True, True), (True, False), (False, True), (False, False)):
+            a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+            x, y = ops.rotate_axes(forward_ad.make_dual(a, tq) if of_q else a, forward_ad.make_dual(b, tk) if of_k else b, pos, (8,))
+            for out, t, has in ((x, tq, of_q), (y, tk, of_k)):
+                tangent = forward_ad.unpack_dual(out).tangent
+                assert torch.equal(tangent, 2 * t) if has else tangent is None
+            for in_q in (True, False):
+                up = forward_ad.make_dual(gq, tq) if in_q else gq
+                da, db = torch.autograd.grad((x, y), (a, b), (up, gk), retain_graph=True)
+                assert torch.equal(forward_ad.unpack_dual(da).primal, gq / 2) and torch.equal(db, gk / 2)
+                tangent = forward_ad.unpack_dual(da).tangent
+                assert torch.equal(tangent, tq / 2) if in_q else tangent is None
